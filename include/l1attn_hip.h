@@ -386,6 +386,34 @@ int l1attn_sparse_bidi_bwd_bf16(const void* dvo, const void* vf, const void* vb,
                                 int64_t B, int64_t T, int64_t H, int64_t W, int64_t Wv, int64_t E,
                                 int use_softmax, void* stream);
 
+/* ------------------------------------------------------------------- masked attention */
+/*
+ * Masked L1 attention with the value sum, for training and prefill; no counterpart in the reference.
+ *   a[t,s] = -1/sqrt(W) * sum_w |q[b,t,h,w] - k[b,s,hk,w]|,   hk = h / (H/Hk)
+ *   c = softcap * tanh(a / softcap)  (softcap > 0; else c = a),   x[t,s] = c - slopes[h] * |i - s|,   i = S - T + t
+ *   p[t,s] = exp(x) / (1 + sum_s exp(x)) over the visible s,   o[b,t,h,:] = sum_s p[t,s] * v[b,s,hk,:]
+ * s is visible to i where (not causal, or s <= i, or s < prefix[b]) and, with doc, doc[b,s] == doc[b,i] >= 0.  What is not
+ * visible has no influence, whatever its values; a row that sees nothing is zero.
+ * q [B,T,H,W], k [B,S,Hk,W], v [B,S,Hk,Wv], o and d_o [B,T,H,Wv], lse [B,T,H] float32 (log of the denominator; the forward
+ * takes NULL for it).  dtype 0 float32, 1 float16, 2 bfloat16; sums and softmax are float32 in each.
+ * doc [B,S] and prefix [B] are device pointers to int32 or NULL; slopes is a HOST pointer to H numbers >= 0, or NULL, read
+ * during the call.  T <= S, W and Wv <= 128, H <= 256.  Deterministic.
+ */
+typedef struct l1attn_masked_desc {
+    int64_t B, T, S, H, Hk, W, Wv;
+    int32_t dtype, causal;
+    float softcap;
+    const float* slopes;
+    const int32_t* doc;
+    const int32_t* prefix;
+} l1attn_masked_desc;
+
+int l1attn_masked_fwd(const l1attn_masked_desc* desc, const void* q, const void* k, const void* v, void* o, float* lse, void* stream);
+/* dq, dk, dv of o's gradient d_o, from the forward's o and lse; sign(0) = 0.  Shared key heads and rows are summed in a fixed order. */
+size_t l1attn_masked_bwd_workspace_bytes(const l1attn_masked_desc* desc);
+int l1attn_masked_bwd(const l1attn_masked_desc* desc, const void* q, const void* k, const void* v, const void* o, const float* lse,
+                      const void* d_o, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------- measurement aids (bench.py only) */
 /*
  * Not part of the operator boundary and no counterpart in the reference: nothing in the operators calls

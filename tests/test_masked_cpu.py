@@ -1,0 +1,88 @@
+"""CPU-only: what masked attention refuses, at the Python operator and at the C entry, before anything is launched."""
+import ctypes
+
+import pytest
+import torch
+
+import _l1attn_hip as drv
+
+
+@pytest.fixture()
+def no_gpu(monkeypatch):
+    monkeypatch.setattr(drv, "check_input", lambda x, name: None)
+
+
+def _q(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+def test_host_tensors_and_strides_are_refused():
+    import l1attn_masked_cuda as m
+    q = _q(1, 4, 2, 8)
+    with pytest.raises(RuntimeError, match="q must be a CUDA tensor"):
+        m.L1AttnMasked()(q, q, q)
+
+
+@pytest.mark.parametrize("what,match", [
+    (dict(k=_q(1, 4, 2, 9)), "q must be"), (dict(v=_q(1, 5, 2, 8)), "q must be"), (dict(k=_q(2, 4, 2, 8), v=_q(2, 4, 2, 8)), "q must be"),
+    (dict(k=_q(1, 3, 2, 8), v=_q(1, 3, 2, 8)), "last of the keys"), (dict(k=_q(1, 4, 3, 8), v=_q(1, 4, 3, 8)), "multiple"),
+    (dict(k=_q(1, 4, 2, 8).half()), "dtype"), (dict(q=_q(1, 4, 2, 8).double(), k=_q(1, 4, 2, 8).double(), v=_q(1, 4, 2, 8).double()), "float32, float16"),
+    (dict(v=_q(1, 4, 2, 129)), "1 to 128"), (dict(v=_q(1, 4, 2, 0)), "1 to 128"),
+    (dict(doc=torch.zeros(1, 3, dtype=torch.int32)), "doc"), (dict(doc=torch.zeros(1, 4, dtype=torch.int64)), "doc"),
+    (dict(prefix=torch.zeros(2, dtype=torch.int32)), "prefix"), (dict(prefix=torch.zeros(1, dtype=torch.int32), causal=False), "prefix"),
+    (dict(softcap=-1.0), "softcap"), (dict(softcap=float("nan")), "softcap"), (dict(slopes=(1.0,)), "slopes")])
+def test_refusals(no_gpu, what, match):
+    a = dict(q=_q(1, 4, 2, 8), k=_q(1, 4, 2, 8), v=_q(1, 4, 2, 8))
+    a.update(what)
+    with pytest.raises((RuntimeError, ValueError), match=match):
+        drv.masked_forward(**a)
+
+
+def test_slopes_are_constants_of_the_module():
+    import l1attn_masked_cuda as m
+    for bad in ((-1.0, 0.0), (float("nan"),), (float("inf"),)):
+        with pytest.raises(ValueError, match="slopes"):
+            m.L1AttnMasked(slopes=bad)
+
+
+def test_c_entry_codes():
+    L = drv.lib()
+    one = ctypes.c_void_p(16)
+
+    def fwd(q=one, o=one, **kw):
+        d = dict(B=1, T=4, S=4, H=2, Hk=2, W=8, Wv=8, dtype=0, causal=1, softcap=0.0)
+        d.update(kw)
+        slopes = d.pop("slope_values", None)
+        desc = drv.MaskedDesc(**d)
+        if slopes:
+            keep = (ctypes.c_float * len(slopes))(*slopes)
+            desc.slopes = ctypes.addressof(keep)
+        return L.l1attn_masked_fwd(ctypes.addressof(desc), q, one, one, o, None, None)
+    assert L.l1attn_masked_fwd(None, one, one, one, one, None, None) == -1
+    assert fwd(q=None) == -1 and fwd(o=None) == -1
+    for kw in (dict(T=5), dict(T=-1), dict(B=-1), dict(H=3), dict(Hk=0), dict(W=0), dict(dtype=3), dict(causal=2), dict(softcap=-1.0),
+               dict(softcap=float("nan")), dict(causal=0, prefix=16), dict(slope_values=(0.5, -1.0)), dict(slope_values=(0.5, float("nan")))):
+        assert fwd(**kw) == -1, kw
+    for kw in (dict(W=129), dict(Wv=129), dict(H=512), dict(S=1 << 31)):
+        assert fwd(**kw) == -3, kw
+    assert fwd(B=0) == 0 and fwd(T=0) == 0  # nothing to do
+    d = drv.MaskedDesc(1, 4, 4, 2, 2, 8, 8, 0, 1, 0.0, None, None, None)
+    n = L.l1attn_masked_bwd_workspace_bytes(ctypes.addressof(d))
+    assert n == 32
+    assert L.l1attn_masked_bwd(ctypes.addressof(d), *[one] * 9, None, n, None) == -2
+    assert L.l1attn_masked_bwd(ctypes.addressof(d), *[one] * 10, n - 1, None) == -2
+    assert L.l1attn_masked_bwd(ctypes.addressof(d), one, None, *[one] * 8, n, None) == -1
+
+
+def test_the_plain_statement_is_the_framework_s_own():
+    # without masks it is what the fused operator's closed form says, and its gradients are autograd's
+    import closed_forms as cf
+    import lm_forms as lf
+    g = torch.Generator().manual_seed(0)
+    q, k, v, do = (torch.randn(2, 9, 3, 5, generator=g, dtype=torch.float64) for _ in range(4))
+    q, k, v = (x.requires_grad_() for x in (q, k, v))
+    o = cf.dense_then_value(q, k, v)
+    want = [o, *torch.autograd.grad(o, (q, k, v), do)]
+    got, _ = lf.masked(q, k, v, do, causal=False)
+    for a, b in zip(got, want):
+        assert torch.allclose(a, b.detach(), atol=1e-12)

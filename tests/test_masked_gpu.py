@@ -1,0 +1,232 @@
+"""Masked L1 attention on the GPU: forward and gradients against the formulas in 64 bits."""
+import pytest
+import torch
+
+import lm_forms as lf
+
+pytestmark = pytest.mark.gpu
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def _op(**kw):
+    import l1attn_masked_cuda
+    return l1attn_masked_cuda.L1AttnMasked(**kw)
+
+
+def _inputs(B, T, S, H, Hk, W, Wv, dtype, seed, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    q, k, v, do = (torch.randn(B, n, h, w, generator=g) for n, h, w in ((T, H, W), (S, Hk, W), (S, Hk, Wv), (T, H, Wv)))
+    return [(x * s).to(dtype).cuda() for x, s in ((q, scale), (k, scale), (v, 1.0), (do, 1.0))]
+
+
+def _run(q, k, v, do, doc=None, prefix=None, causal=True, cap=0.0, slopes=None):
+    q, k, v = (x.detach().requires_grad_() for x in (q, k, v))
+    o = _op(causal=causal, softcap=cap, slopes=slopes)(q, k, v, doc=doc, prefix=prefix)
+    return [o.detach(), *torch.autograd.grad(o, (q, k, v), do)]
+
+
+def _check(q, k, v, do, **kw):
+    print("case", tuple(q.shape), tuple(k.shape), v.shape[-1], q.dtype, {n: x for n, x in kw.items() if not torch.is_tensor(x)}, flush=True)
+    ref, terms = lf.masked(q, k, v, do, **kw)
+    got = _run(q, k, v, do, **kw)
+    lf.check(got, ref, terms, q.dtype, q.shape[-1])
+    return got
+
+
+def _docs(B, S, n, seed, pad=0):
+    g = torch.Generator().manual_seed(seed)
+    cuts = torch.randint(0, S + 1, (B, n), generator=g).sort(1).values
+    doc = (torch.arange(S)[None, :, None] >= cuts[:, None]).sum(2).to(torch.int32)
+    if pad:
+        doc[:, -pad:] = -1
+    return doc.cuda()
+
+
+SLOPES = lambda H: tuple(2.0 ** (-8 * (h + 1) / H) for h in range(H))  # noqa: E731
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("B,T,S,H,Hk,W,Wv", [(1, 1, 1, 1, 1, 1, 1), (2, 1, 70, 4, 2, 32, 32), (1, 33, 33, 2, 1, 33, 65), (2, 64, 129, 4, 4, 64, 64),
+                                            (1, 65, 200, 3, 1, 65, 33), (1, 130, 130, 2, 2, 96, 128), (1, 100, 100, 2, 1, 128, 7),
+                                            (1, 257, 300, 8, 2, 64, 64), (1, 40, 90, 2, 2, 7, 128), (3, 31, 63, 2, 2, 16, 16)])
+def test_sizes(B, T, S, H, Hk, W, Wv, dtype):
+    _check(*_inputs(B, T, S, H, Hk, W, Wv, dtype, T + S + W))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rule", ["open", "docs", "docs_open", "prefix", "prefix_docs", "cap", "slopes", "all"])
+def test_masks(rule, dtype):
+    B, T, S, H, Hk, W = 2, 150, 201, 4, 2, 64
+    q, k, v, do = _inputs(B, T, S, H, Hk, W, 48, dtype, 5)
+    kw = {}
+    if "docs" in rule or rule == "all":
+        kw["doc"] = _docs(B, S, 5, 3, pad=9)
+    if "open" in rule:
+        kw["causal"] = False
+    if "prefix" in rule or rule == "all":
+        kw["prefix"] = torch.tensor([0, 130], dtype=torch.int32).cuda()
+    if rule in ("cap", "all"):
+        kw["cap"] = 5.0
+    if rule in ("slopes", "all"):
+        kw["slopes"] = SLOPES(H)
+    _check(q, k, v, do, **kw)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_documents_in_no_order_and_rows_that_see_nothing(dtype):
+    B, T, H, W = 2, 140, 2, 32
+    q, k, v, do = _inputs(B, T, T, H, 1, W, W, dtype, 8)
+    g = torch.Generator().manual_seed(1)
+    doc = torch.randint(-1, 3, (B, T), generator=g).to(torch.int32)
+    doc[1] = -1  # a whole sequence of padding
+    got = _check(q, k, v, do, doc=doc.cuda(), causal=False)
+    for x in got:
+        assert (x[1] == 0).all()
+    assert (got[0].cpu()[0][doc[0] < 0] == 0).all() and (got[1].cpu()[0][doc[0] < 0] == 0).all()
+    assert (got[2].cpu()[0][doc[0] < 0] == 0).all() and (got[3].cpu()[0][doc[0] < 0] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_what_is_hidden_may_hold_anything(bad, dtype):
+    B, T, H, W = 1, 130, 2, 64
+    q, k, v, do = _inputs(B, T, T, H, 1, W, W, dtype, 9)
+    doc = torch.zeros(B, T, dtype=torch.int32)
+    doc[:, 100:] = -1  # padding behind, in the middle of a tile
+    doc[:, 40:50] = -1  # and in between
+    hidden = doc[0] < 0
+    for x in (q, k, v, do):
+        x[0, hidden.cuda()] = bad
+    got = _check(q, k, v, do, doc=doc.cuda())
+    for x in got[1:]:
+        assert (x.cpu()[0][hidden] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_the_future_may_hold_anything(dtype):
+    # values behind a query's own place: not finite, and yet not seen by the rows before them
+    q, k, v, do = _inputs(1, 80, 80, 2, 2, 32, 32, dtype, 10)
+    clean = _run(q, k, v, do)[0]
+    k2, v2 = k.clone(), v.clone()
+    k2[0, 70:], v2[0, 70:] = float("nan"), float("inf")
+    with torch.no_grad():
+        o = _op()(q, k2, v2)
+    assert torch.equal(o[0, :70], clean[0, :70])
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("scale", [1e-3, 30.0])
+def test_small_and_large_inputs(scale, dtype):
+    _check(*_inputs(1, 120, 120, 2, 2, 64, 64, dtype, 11, scale))
+
+
+def test_ties_have_no_sign():
+    # integers: many pairs are equal in a column, and sign(0) = 0
+    g = torch.Generator().manual_seed(2)
+    for dtype in (F32, F16, BF16):
+        q, k = (torch.randint(-2, 3, (1, 90, 2, 64), generator=g).to(dtype).cuda() for _ in range(2))
+        v, do = (torch.randn(1, 90, 2, 64, generator=g).to(dtype).cuda() for _ in range(2))
+        _check(q, k, v, do)
+        same = torch.ones(1, 50, 1, 32, dtype=dtype, device="cuda")
+        out = _run(same, same, torch.randn(1, 50, 1, 32, generator=g).to(dtype).cuda(), torch.ones(1, 50, 1, 32, dtype=dtype, device="cuda"))
+        assert out[1].abs().max() <= 1e-5 and out[2].abs().max() <= 1e-5
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_unaligned_and_strided_inputs(dtype):
+    B, T, H, W = 1, 70, 2, 64
+    q, k, v, do = _inputs(B, T, T, H, H, W, W, dtype, 12)
+    ref = _run(q, k, v, do)
+
+    def shifted(x):  # contiguous, but starting one element into its storage
+        y = torch.empty(x.numel() + 1, dtype=x.dtype, device=x.device)[1:].view_as(x)
+        return y.copy_(x)
+    for a, b in zip(_run(*(shifted(x) for x in (q, k, v, do))), ref):
+        assert torch.equal(a, b)
+    wide = [torch.cat([x, x], 3)[..., :W] for x in (q, k, v, do)]
+    assert not wide[0].is_contiguous()
+    for a, b in zip(_run(*wide), ref):
+        assert torch.equal(a, b)
+
+
+def test_repeats_bit_for_bit_and_large_grids():
+    q, k, v, do = _inputs(2, 1100, 1100, 8, 2, 64, 64, BF16, 13)
+    doc = _docs(2, 1100, 4, 6)
+    a, b = _run(q, k, v, do, doc=doc), _run(q, k, v, do, doc=doc)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    ref, terms = lf.masked(q[:1, :, :4], k[:1, :, :1], v[:1, :, :1], do[:1, :, :4], doc=doc[:1])
+    lf.check([a[0][:1, :, :4], a[1][:1, :, :4], a[2][:1, :, :1], a[3][:1, :, :1]], ref, terms, BF16, 64)
+
+
+def test_more_tiles_than_are_classified_at_a_time():
+    # 70000 keys: over 1024 tiles of 64
+    q, k, v, do = _inputs(1, 3, 70000, 1, 1, 32, 32, F32, 14)
+    doc = torch.zeros(1, 70000, dtype=torch.int32)
+    doc[:, 100:69000] = 1
+    doc[:, 69990:] = 0
+    _check(q, k, v, do, doc=doc.cuda())
+
+
+def test_gradients_against_differences():
+    g = torch.Generator().manual_seed(3)
+    q, k, v, do = (torch.randn(1, 12, 2, 8, generator=g).cuda() for _ in range(4))
+    kw = dict(causal=True, cap=4.0, slopes=(0.5, 0.1))
+    _, dq, dk, dv = _run(q, k, v, do, **kw)
+
+    def loss(q, k, v):
+        return float((lf.masked(q, k, v, **kw)[0][0] * do.double().cpu()).sum())
+    eps = 1e-6
+    for n, x, d in ((0, q, dq), (1, k, dk), (2, v, dv)):
+        for at in ((0, 0, 0, 0), (0, 5, 1, 3), (0, 11, 0, 7), (0, 7, 1, 2)):
+            args = [y.double().cpu() for y in (q, k, v)]
+            args[n] = args[n].clone()
+            args[n][at] += eps
+            up = loss(*args)
+            args[n][at] -= 2 * eps
+            assert abs((up - loss(*args)) / (2 * eps) - float(d[at])) <= 1e-5 + 1e-4 * abs(float(d[at]))
+
+
+def test_other_streams_and_graph_replays():
+    q, k, v, do = _inputs(1, 200, 200, 4, 2, 64, 64, BF16, 15)
+    ref = _run(q, k, v, do)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = _run(q, k, v, do)
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(a, b) for a, b in zip(got, ref))
+    import _l1attn_hip as drv
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o, lse = drv.masked_forward(q, k, v)
+        grads = drv.masked_backward(do, q, k, v, o, lse)
+    fresh = _inputs(1, 200, 200, 4, 2, 64, 64, BF16, 16)
+    for seed in range(3):
+        for x, y in zip((q, k, v, do), fresh):
+            x.copy_(torch.roll(y, seed, 1))
+        eager = _run(q, k, v, do)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip([o, *grads], eager))
+
+
+def test_empty():
+    q = torch.zeros(0, 4, 2, 8, device="cuda", requires_grad=True)
+    o = _op()(q, q, q)
+    assert o.shape == (0, 4, 2, 8)
+    k = torch.randn(1, 5, 2, 8, device="cuda", requires_grad=True)
+    q = torch.zeros(1, 0, 2, 8, device="cuda", requires_grad=True)
+    o = _op()(q, k, k)
+    assert o.shape == (1, 0, 2, 8)
+    g = torch.autograd.grad(o, (q, k), torch.zeros_like(o))
+    assert g[0].shape == q.shape and (g[1] == 0).all()
+
+
+def test_it_trains():
+    torch.manual_seed(0)
+    lin = torch.nn.Linear(32, 3 * 64).cuda()
+    x = torch.randn(2, 50, 32, device="cuda")
+    q, k, v = lin(x).view(2, 50, 3, 2, 32).unbind(2)
+    o = _op(softcap=10.0, slopes=(0.1, 0.2))(q, k, v)
+    o.square().mean().backward()
+    assert torch.isfinite(lin.weight.grad).all() and lin.weight.grad.abs().max() > 0
