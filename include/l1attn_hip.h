@@ -414,6 +414,62 @@ size_t l1attn_masked_bwd_workspace_bytes(const l1attn_masked_desc* desc);
 int l1attn_masked_bwd(const l1attn_masked_desc* desc, const void* q, const void* k, const void* v, const void* o, const float* lse,
                       const void* d_o, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------- paged 8-bit cache */
+/*
+ * Keys and values of many sequences in pages of `page` (16, 32 or 64) tokens; no counterpart in the reference.
+ *   k_pages  [n_pages, Hk, page, W up to a multiple of 16] int8 codes, zero behind W; v_pages likewise with Wv; 16-byte aligned
+ *   k_scale, v_scale  [n_pages, Hk] float32: value = code * scale
+ *   table    [rows, row_pages] int32: the pages of each sequence in order (what lies behind its length does not count)
+ *   lens     [rows] int32: its tokens;   refs [n_pages] int32: how many rows hold the page
+ *   free_pages [n_pages] int32, n_free [1] int32: a stack of the pages that nobody holds, the top is taken first
+ * All are device memory, owned by the caller and changed in place; the struct itself is host memory, read during the call.
+ * The calls are asynchronous, deterministic and can be captured: nothing of the state is read on the host.  Lists (seqs,
+ * counts, keep, parents, children) are device int32, at most 1024 long; a sequence number out of range, or named twice in a
+ * list, is not served (the first naming is).  served [B] bytes: 1 where the entry was served; the others change nothing.
+ */
+typedef struct l1attn_cache {
+    int64_t n_pages, page, Hk, W, Wv, rows, row_pages;
+    int8_t *k_pages, *v_pages;
+    float *k_scale, *v_scale;
+    int32_t *table, *lens, *refs, *free_pages, *n_free;
+} l1attn_cache;
+
+/*
+ * The first counts[b] (all n without counts) rows of k [B,n,Hk,W], v [B,n,Hk,Wv] (dtype 0 float32, 1 float16, 2 bfloat16)
+ * behind sequence seqs[b] (b without seqs).  A page's scale is its values' largest magnitude over 127; where new tokens make
+ * it grow, the codes that are there become rint(code * old / new).  A partly filled page that others hold too is copied.
+ * Served as long as the pages last, in the order of the entries, and where the row of the table has room.
+ */
+size_t l1attn_cache_append_workspace_bytes(const l1attn_cache* cache, int64_t B, int64_t n);
+int l1attn_cache_append(const l1attn_cache* cache, int dtype, const void* k, const void* v, const int32_t* seqs, const int32_t* counts,
+                        int64_t B, int64_t n, uint8_t* served, void* workspace, size_t workspace_bytes, void* stream);
+/* Row children[b] (empty before) shares all pages of row parents[b], as they are before the call.  workspace: 4 B bytes. */
+int l1attn_cache_fork(const l1attn_cache* cache, const int32_t* parents, const int32_t* children, int64_t B, uint8_t* served,
+                      void* workspace, size_t workspace_bytes, void* stream);
+/* Sequences seqs[b] keep their first keep[b] tokens (none without keep); pages that nobody holds any more are free, in ascending order. */
+size_t l1attn_cache_free_workspace_bytes(const l1attn_cache* cache);
+int l1attn_cache_free(const l1attn_cache* cache, const int32_t* seqs, const int32_t* keep, int64_t B, void* workspace,
+                      size_t workspace_bytes, void* stream);
+/* Moves pages so that the ones in use are the first live[0] of the pool: the r-th of those behind goes into the r-th hole. */
+size_t l1attn_cache_compact_workspace_bytes(const l1attn_cache* cache);
+int l1attn_cache_compact(const l1attn_cache* cache, int32_t* live, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * o [B,n,H,Wv] of q [B,n,H,W]: the masked attention's formula, causal, of the last counts[b] (n without counts) tokens of
+ * sequence seqs[b] over all of it; query t is at place lens - counts[b] + t, rows t >= counts[b] are zero.  Head h reads key
+ * head h / (H / Hk).  slopes: H host numbers >= 0 or NULL.  H <= 256.
+ */
+typedef struct l1attn_attend_desc {
+    int64_t B, n, H;
+    int32_t dtype;
+    float softcap;
+    const float* slopes;
+} l1attn_attend_desc;
+
+size_t l1attn_cache_attend_workspace_bytes(const l1attn_cache* cache, const l1attn_attend_desc* desc);
+int l1attn_cache_attend(const l1attn_cache* cache, const l1attn_attend_desc* desc, const void* q, const int32_t* seqs, const int32_t* counts,
+                        void* o, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------- measurement aids (bench.py only) */
 /*
  * Not part of the operator boundary and no counterpart in the reference: nothing in the operators calls

@@ -10,7 +10,6 @@ the current stream only; every computation happens in the HIP library.  There is
 eager fallback: a missing library raises at import of the first operator.
 """
 import ctypes
-import functools
 import math
 import os
 
@@ -133,12 +132,6 @@ def lib():
                 f = getattr(L, name + sfx)
                 f.restype = _c_i
                 f.argtypes = [_c_p] * nptr + dims
-        L.l1attn_masked_fwd.restype = _c_i
-        L.l1attn_masked_fwd.argtypes = [_c_p] * 7
-        L.l1attn_masked_bwd_workspace_bytes.restype = _c_sz
-        L.l1attn_masked_bwd_workspace_bytes.argtypes = [_c_p]
-        L.l1attn_masked_bwd.restype = _c_i
-        L.l1attn_masked_bwd.argtypes = [_c_p] * 11 + [_c_sz, _c_p]
         _lib = L
     return _lib
 
@@ -586,105 +579,3 @@ def bidi_backward(dvo, vf, vb, q, k, coo, P, dst_mxlen, use_softmax, plan=None):
             B, T, H, W, Wv, E, int(bool(use_softmax)), stream_of(q))
     check(rc, "l1attn_sparse_bidi_bwd_" + sfx)
     return [dvf, dvb, dq, dk]
-
-
-# ----------------------------------------------------------------------------- masked attention
-
-_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-
-
-class MaskedDesc(ctypes.Structure):
-    """l1attn_masked_desc of the C header."""
-    _fields_ = [(n, _c_i64) for n in ("B", "T", "S", "H", "Hk", "W", "Wv")] + [
-        ("dtype", ctypes.c_int32), ("causal", ctypes.c_int32), ("softcap", ctypes.c_float), ("slopes", _c_p), ("doc", _c_p),
-        ("prefix", _c_p)]
-
-
-def slopes_of(slopes):
-    """The distance bias of each head as a tuple of finite numbers >= 0."""
-    t = tuple(float(x) for x in slopes)
-    if not all(0.0 <= x <= 3e38 for x in t):
-        raise ValueError("slopes must be finite numbers >= 0, one for each query head, got %r" % (t[:8],))
-    return t
-
-
-@functools.lru_cache(maxsize=64)
-def _slopes_array(slopes):
-    return (ctypes.c_float * len(slopes))(*slopes)
-
-
-def _index_tensor(x, name, shape, q):
-    if x is None:
-        return None
-    if x.dtype != torch.int32 or tuple(x.shape) != shape or x.device != q.device:
-        raise RuntimeError("%s must be an int32 tensor of shape %s on the device of q" % (name, list(shape)))
-    check_input(x, name)
-    return x.data_ptr()
-
-
-def _check_rule(H, softcap, slopes):
-    if not 0.0 <= softcap <= 3e38:
-        raise ValueError("softcap must be a finite number >= 0 (0: none), got %r" % (softcap,))
-    if slopes is not None and len(slopes) != H:
-        raise ValueError("slopes must hold one number for each of the %d query heads, got %d" % (H, len(slopes)))
-
-
-def _masked_desc(q, k, v, doc, prefix, causal, softcap, slopes):
-    for x, n in ((q, "q"), (k, "k"), (v, "v")):
-        check_input(x, n)
-    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4 or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3] \
-            or v.shape[:3] != k.shape[:3]:
-        raise RuntimeError("q must be [batch, n_query, n_heads, width], k [batch, n_ctx, n_key_heads, width] and v "
-                           "[batch, n_ctx, n_key_heads, value width]")
-    if not (q.dtype == k.dtype == v.dtype) or not (q.device == k.device == v.device):
-        raise RuntimeError("q, k, v must share dtype and device")
-    if q.dtype not in _DTYPES:
-        raise RuntimeError("q: masked attention takes float32, float16 and bfloat16, got %s" % q.dtype)
-    B, T, H, W = q.shape
-    S, Hk, Wv = k.shape[1], k.shape[2], v.shape[3]
-    if T > S:
-        raise RuntimeError("the queries are the last of the keys' tokens: n_query %d is more than n_ctx %d" % (T, S))
-    if Hk < 1 or H < 1 or H % Hk:
-        raise RuntimeError("n_heads must be a multiple of n_key_heads, got %d and %d" % (H, Hk))
-    if not (1 <= W <= 128 and 1 <= Wv <= 128):
-        raise RuntimeError("widths of masked attention are 1 to 128, got %d and %d" % (W, Wv))
-    if prefix is not None and not causal:
-        raise ValueError("prefix is an exception to the causal mask: it has no meaning without causal=True")
-    _check_rule(H, softcap, slopes)
-    return MaskedDesc(B, T, S, H, Hk, W, Wv, _DTYPES[q.dtype], int(bool(causal)), softcap,
-                      None if slopes is None else ctypes.addressof(_slopes_array(slopes)),
-                      _index_tensor(doc, "doc", (B, S), q), _index_tensor(prefix, "prefix", (B,), q))
-
-
-def masked_forward(q, k, v, doc=None, prefix=None, causal=True, softcap=0.0, slopes=None, want_lse=True):
-    """Masked L1 attention -> [o, lse]; lse [B,T,H] float32 is what the backward reads (None if not wanted)."""
-    d = _masked_desc(q, k, v, doc, prefix, causal, softcap, slopes)
-    o = torch.empty((d.B, d.T, d.H, d.Wv), dtype=q.dtype, device=q.device)
-    lse = torch.empty((d.B, d.T, d.H), dtype=torch.float32, device=q.device) if want_lse else None
-    with torch.cuda.device(q.device):
-        rc = lib().l1attn_masked_fwd(ctypes.addressof(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-                                     None if lse is None else lse.data_ptr(), stream_of(q))
-    check(rc, "l1attn_masked_fwd")
-    return [o, lse]
-
-
-def masked_backward(d_o, q, k, v, o, lse, doc=None, prefix=None, causal=True, softcap=0.0, slopes=None):
-    """Gradients of masked_forward -> [dq, dk, dv] from its o and lse."""
-    d = _masked_desc(q, k, v, doc, prefix, causal, softcap, slopes)
-    for x, n in ((d_o, "d_o"), (o, "o"), (lse, "lse")):
-        check_input(x, n)
-    shape = (d.B, d.T, d.H, d.Wv)
-    for x, n in ((d_o, "d_o"), (o, "o")):
-        if tuple(x.shape) != shape or x.dtype != q.dtype or x.device != q.device:
-            raise RuntimeError("%s must be [batch, n_query, n_heads, value width] with the dtype and device of q" % n)
-    if tuple(lse.shape) != shape[:3] or lse.dtype != torch.float32 or lse.device != q.device:
-        raise RuntimeError("lse must be the [batch, n_query, n_heads] float32 tensor that the forward returned")
-    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
-    L = lib()
-    with torch.cuda.device(q.device):
-        n = L.l1attn_masked_bwd_workspace_bytes(ctypes.addressof(d))
-        ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-        rc = L.l1attn_masked_bwd(ctypes.addressof(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(),
-                                 d_o.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), n, stream_of(q))
-    check(rc, "l1attn_masked_bwd")
-    return [dq, dk, dv]

@@ -21,7 +21,7 @@ from torch import nn
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
-import _l1attn_hip as _drv
+import _l1attn_lm_hip as _drv
 
 
 class L1AttnMaskedFn(Function):

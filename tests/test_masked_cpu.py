@@ -4,7 +4,7 @@ import ctypes
 import pytest
 import torch
 
-import _l1attn_hip as drv
+import _l1attn_lm_hip as drv
 
 
 @pytest.fixture()

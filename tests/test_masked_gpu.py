@@ -195,7 +195,7 @@ def test_other_streams_and_graph_replays():
         got = _run(q, k, v, do)
     torch.cuda.current_stream().wait_stream(s)
     assert all(torch.equal(a, b) for a, b in zip(got, ref))
-    import _l1attn_hip as drv
+    import _l1attn_lm_hip as drv
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         o, lse = drv.masked_forward(q, k, v)

@@ -1,0 +1,278 @@
+"""The paged 8-bit cache and the attention over it on the GPU, against a plain model of both: tables, codes and scales have to be
+equal, attention is held to its rounding (lm_forms.check)."""
+import pytest
+import torch
+
+import lm_forms as lf
+
+pytestmark = pytest.mark.gpu
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+class Pair:
+    """The cache on the GPU beside its plain model; every call goes to both, and their states are compared after it."""
+
+    def __init__(self, N=40, P=16, Hk=2, W=32, Wv=48, rows=6, M=12, dtype=BF16, seed=0):
+        import l1attn_paged_cuda as m
+        self.m, self.dtype = m, dtype
+        self.gpu = m.L1PagedCache.empty(N, P, Hk, W, rows, M, v_width=Wv, device="cuda")
+        self.plain = lf.PlainCache(N, P, Hk, W, Wv, rows, M)
+        self.g = torch.Generator().manual_seed(seed)
+
+    def data(self, B, n, scale=1.0):
+        p = self.plain
+        return [(torch.randn(B, n, p.Hk, w, generator=self.g) * scale).to(self.dtype) for w in (p.W, p.Wv)]
+
+    def ints(self, x):
+        return None if x is None else torch.tensor(x, dtype=torch.int32, device="cuda")
+
+    def append(self, B, n, seqs=None, counts=None, scale=1.0, data=None):
+        k, v = self.data(B, n, scale) if data is None else data
+        got = self.gpu.append(k.cuda(), v.cuda(), seqs=self.ints(seqs), counts=self.ints(counts))
+        want = self.plain.append(k, v, seqs, counts)
+        assert got.tolist() == want, (got.tolist(), want)
+        self.same()
+        return want
+
+    def fork(self, parents, children):
+        got, want = self.gpu.fork(self.ints(parents), self.ints(children)), self.plain.fork(parents, children)
+        assert got.tolist() == want
+        self.same()
+        return want
+
+    def free(self, seqs, keep=None):
+        self.gpu.free(self.ints(seqs), keep=self.ints(keep))
+        self.plain.free(seqs, keep)
+        self.same()
+
+    def compact(self):
+        assert int(self.gpu.compact()) == self.plain.compact()
+        self.same()
+
+    def same(self):
+        g, p = self.gpu, self.plain
+        assert g.lens.tolist() == p.lens
+        for s in range(p.rows):
+            used = -(-p.lens[s] // p.P)
+            assert g.table[s, :used].tolist() == p.table[s, :used].tolist()
+        assert g.refs.tolist() == p.refs
+        assert g.free_pages[:int(g.n_free)].tolist() == p.stack
+        for a, b in ((g.k_scale, p.scale[0]), (g.v_scale, p.scale[1])):
+            assert torch.equal(a.cpu(), b)
+        for a, b in ((g.k_pages, p.pages[0]), (g.v_pages, p.pages[1])):
+            assert torch.equal(a.cpu(), b)
+
+    def attend(self, B, n, H, seqs=None, counts=None, cap=0.0, slopes=None, dtype=None):
+        p, dtype = self.plain, dtype or self.dtype
+        q = torch.randn(B, n, H, p.W, generator=self.g).to(dtype)
+        print("case attend", B, n, H, p.Hk, p.W, p.Wv, p.P, dtype, seqs, counts, cap, flush=True)
+        o = self.m.l1attn_paged(q.cuda(), self.gpu, seqs=self.ints(seqs), counts=self.ints(counts), softcap=cap, slopes=slopes)
+        ref, terms = p.attend(q, seqs, counts, cap, slopes)
+        lf.check([o], [ref], [terms], dtype, p.W, names=("o",))
+        return o
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("P", [16, 32, 64])
+def test_append_in_all_alignments(P, dtype):
+    c = Pair(N=60, P=P, rows=4, M=16, dtype=dtype)
+    for n, counts in ((1, None), (5, [5, 0, 3, 9]), (P - 1, None), (P, None), (2 * P + 3, [2 * P + 3, P, -4, 1]), (1, None)):
+        c.append(4, n, counts=counts, scale=1 + n % 3)
+
+
+@pytest.mark.parametrize("W,Wv", [(1, 1), (7, 33), (64, 96), (65, 128), (128, 20)])
+def test_append_widths(W, Wv):
+    c = Pair(W=W, Wv=Wv, Hk=3, N=30, rows=2, M=8)
+    for n in (3, 20, 1, 30):
+        c.append(2, n)
+        c.attend(2, 1, 3)
+
+
+def test_scales_grow_and_old_codes_follow():
+    c = Pair(rows=1)
+    for scale in (0.01, 1.0, 0.1, 50.0, 0.0, 3.0):
+        c.append(1, 3, scale=scale)
+
+
+def test_values_that_are_not_finite_or_zero():
+    c = Pair(rows=2, dtype=F32)
+    k, v = c.data(2, 5)
+    k[0, 1, 0, 3], k[0, 2, 1, 5], v[0, 3, 0, 0], v[0, 4, 1, 1] = float("inf"), float("nan"), -float("inf"), float("nan")
+    k[1], v[1] = 0.0, 0.0
+    c.append(2, 5, data=(k, v))
+    c.attend(2, 1, 2, dtype=F32)
+    c.append(2, 4)
+
+
+def test_rows_that_are_not_served():
+    c = Pair(N=10, P=16, rows=6, M=4)
+    assert c.append(6, 20, seqs=[3, 3, -1, 6, 0, 5]) == [True, False, False, False, True, True]
+    # no room in the row (4 pages hold 64 tokens), and the pool: 6 pages taken, 4 left
+    assert c.append(3, 45, seqs=[3, 0, 5], counts=[45, 20, 44]) == [False, True, True]
+    assert c.append(4, 16, seqs=[1, 2, 4, 5], counts=[16, 16, 0, 0]) == [True, False, True, True]
+    assert c.append(2, 16, seqs=[2, 0], counts=[1, 8]) == [False, True]  # 8 tokens fit the page that is there
+    c.free([0, 0, 9, -3])
+    c.append(1, 40, seqs=[2])
+
+
+def test_fork_shares_and_copies_on_write():
+    c = Pair(N=40, rows=8, M=10)
+    c.append(2, 37, seqs=[0, 1])
+    assert c.fork([0, 0, 1, 7, 2, 0, 1, 0], [2, 3, 4, 5, 6, 2, 1, 7]) == [True, True, True, True, True, False, False, True]
+    c.append(4, 3, seqs=[2, 0, 3, 4], scale=2.0)
+    c.append(1, 3, seqs=[1], scale=0.5)  # the page that 4 left behind has one holder again: written in place
+    c.attend(5, 2, 4, seqs=[0, 1, 2, 3, 4])
+    c.free([2, 4], keep=[36, 10])
+    c.append(2, 30, seqs=[4, 2])
+    # all holders of a shared page write to it at once: it is free afterwards
+    c.free([0, 1, 2, 3, 4, 7])
+    c.append(1, 20, seqs=[0])
+    c.fork([0, 0], [1, 2])
+    c.append(3, 1, seqs=[2, 0, 1])
+    c.attend(3, 1, 2)
+
+
+def test_free_keeps_a_prefix_and_gives_back_in_order():
+    c = Pair(N=40, rows=5, M=10)
+    c.append(5, 70, counts=[70, 33, 16, 0, 64])
+    c.free([4, 0, 1], keep=[100, 32, 0])
+    c.free([2, 3], keep=[16, 5])
+    c.append(5, 40)
+    c.free([0, 1, 2, 3, 4])
+
+
+def test_compact_and_going_on():
+    c = Pair(N=64, rows=8, M=8)
+    c.append(8, 70, counts=[70, 20, 50, 64, 1, 33, 80, 16])
+    c.fork([0], [7]) if c.plain.lens[7] == 0 else c.free([7])
+    c.fork([0, 2], [7, 6])
+    c.free([0, 3, 5])
+    c.compact()
+    c.attend(8, 1, 2)
+    c.append(4, 30, seqs=[0, 3, 7, 5])
+    c.compact()
+    c.compact()  # nothing moves any more
+    c.free(list(range(8)))
+    c.compact()
+    c.append(8, 30)
+
+
+def test_pools_of_several_scan_chunks():
+    c = Pair(N=9000, P=16, Hk=1, W=16, Wv=16, rows=3, M=4096)
+    c.append(2, 40000, counts=[40000, 30000])
+    c.free([0], keep=[17])
+    c.append(1, 33, seqs=[2])
+    c.compact()
+    c.append(1, 100, seqs=[2])
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("Hk,H,n,W,Wv,P", [(1, 1, 1, 32, 32, 16), (2, 4, 1, 64, 64, 32), (2, 2, 3, 33, 65, 64), (1, 8, 1, 96, 128, 16), (2, 16, 5, 64, 64, 32),
+                                          (1, 24, 2, 128, 96, 64), (3, 9, 7, 17, 5, 16)])
+def test_attention(Hk, H, n, W, Wv, P, dtype):
+    c = Pair(N=140, P=P, Hk=Hk, W=W, Wv=Wv, rows=5, M=2200 // P, dtype=dtype, seed=H + W)
+    for counts in ([600, 1, 256, 0, 2], [3, 0, 1, 0, 255]):
+        c.append(5, 600, counts=counts)
+        c.attend(5, n, H)
+    slopes = tuple(2.0 ** (-8 * (h + 1) / H) for h in range(H))
+    c.attend(4, n, H, seqs=[2, 0, 0, 77], cap=5.0, slopes=slopes)
+    c.attend(3, n, H, seqs=[4, 1, 2], counts=[n, 0, max(0, n - 1)], slopes=slopes)
+
+
+def test_pages_that_are_not_there_give_no_tokens():
+    c = Pair(N=40, rows=2, M=8)
+    c.append(2, 100)
+    o = c.attend(1, 1, 2)
+    # a table that someone has damaged: the tokens of such pages are left out, nothing else is read
+    c.gpu.table[1, 2], c.gpu.table[1, 4] = 40, -7
+    q = torch.randn(2, 1, 2, 32).to(BF16).cuda()
+    a = c.m.l1attn_paged(q, c.gpu)
+    keep = torch.ones(100, dtype=torch.bool)
+    keep[32:48] = keep[64:80] = False
+    k, v = c.plain.tokens(1)
+    for h in range(2):
+        x = torch.exp(-(q[1, 0, h].double().cpu() - k[keep, h]).abs().sum(1) / 32 ** 0.5)
+        want = (x / (1 + x.sum())) @ v[keep, h]
+        assert (a[1, 0, h].double().cpu() - want).abs().max() <= 2.0 ** -8 * (v.abs().max())
+    assert torch.isfinite(o).all()
+
+
+def test_a_run_of_serving_calls_matches_the_training_operator():
+    # prompt, steps, a drafted token that is rejected, a fork: as the masked operator on the cache's values sees it
+    import l1attn_masked_cuda as mm
+    c = Pair(N=60, P=32, Hk=2, W=64, Wv=64, rows=3, M=10, dtype=F32)
+    c.append(2, 90, counts=[90, 41])
+    for step in range(3):
+        c.append(2, 1)
+    c.append(2, 4)
+    c.free([0, 1], keep=[93, 44])
+    c.fork([0], [2])
+    c.append(3, 2)
+    c.compact()
+    g = torch.Generator().manual_seed(1)
+    for s in range(3):
+        k, v = (x.float().cuda()[None] for x in c.plain.tokens(s))
+        q = torch.randn(1, 2, 4, 64, generator=g).cuda()
+        o = c.m.L1AttnPaged(softcap=9.0, slopes=(0.5, 0.1, 0.0, 0.2))(q, c.gpu, seqs=c.ints([s]))
+        with torch.no_grad():
+            want = mm.L1AttnMasked(softcap=9.0, slopes=(0.5, 0.1, 0.0, 0.2))(q, k, v)
+        # both in float32: see lm_forms for the bound of either
+        assert (o - want).abs().max() <= 2 * 2.0 ** -24 * (3 * 64 + 64 + 1) * v.abs().max()
+
+
+def test_graph_of_a_decode_step_and_other_streams():
+    import l1attn_paged_cuda as m
+
+    def fresh():
+        c = m.L1PagedCache.empty(64, 16, 2, 32, 4, 12, device="cuda")
+        g = torch.Generator().manual_seed(3)
+        k, v = (torch.randn(4, 45, 2, 32, generator=g).to(BF16).cuda() for _ in range(2))
+        assert c.append(k, v).all()
+        return c
+    state = lambda c: [x.clone() for x in (c.table, c.lens, c.refs, c.n_free, c.k_pages, c.v_pages, c.k_scale, c.v_scale)]  # noqa: E731
+    k, v = (torch.zeros(4, 1, 2, 32, dtype=BF16, device="cuda") for _ in range(2))
+    q = torch.zeros(4, 1, 4, 32, dtype=BF16, device="cuda")
+
+    def step(c):
+        served = c.append(k, v)
+        return served, m.l1attn_paged(q, c, slopes=(0.1, 0.2, 0.3, 0.4))
+    eager, captured, other = fresh(), fresh(), fresh()
+    step(fresh())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(captured)
+    s = torch.cuda.Stream()
+    for i in range(6):
+        g = torch.Generator().manual_seed(10 + i)
+        for x in (k, v, q):
+            x.copy_(torch.randn(x.shape, generator=g).to(BF16))
+        want = step(eager)
+        graph.replay()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got = step(other)
+        torch.cuda.synchronize()
+        for a in (out, got):
+            assert all(torch.equal(x, y) for x, y in zip(a, want))
+        for c in (captured, other):
+            assert all(torch.equal(x, y) for x, y in zip(state(c), state(eager)))
+
+
+def test_random_walk():
+    import random
+    r = random.Random(5)
+    c = Pair(N=50, P=16, Hk=2, W=20, Wv=36, rows=7, M=6, seed=9)
+    for step in range(60):
+        what = r.choice(("append", "append", "append", "fork", "free", "compact"))
+        seqs = r.sample(range(7), r.randint(1, 7))
+        if what == "append":
+            n = r.choice((1, 2, 17, 40))
+            c.append(len(seqs), n, seqs=seqs, counts=[r.randint(0, n) for _ in seqs], scale=r.choice((0.1, 1.0, 4.0)))
+        elif what == "fork":
+            c.fork([r.randrange(7) for _ in seqs], seqs)
+        elif what == "free":
+            c.free(seqs, keep=r.choice((None, [r.randint(0, 90) for _ in seqs])))
+        else:
+            c.compact()
+        if step % 6 == 0:
+            c.attend(7, 1, 2)
