@@ -397,7 +397,7 @@ int l1attn_sparse_bidi_bwd_bf16(const void* dvo, const void* vf, const void* vb,
  * q [B,T,H,W], k [B,S,Hk,W], v [B,S,Hk,Wv], o and d_o [B,T,H,Wv], lse [B,T,H] float32 (log of the denominator; the forward
  * takes NULL for it).  dtype 0 float32, 1 float16, 2 bfloat16; sums and softmax are float32 in each.
  * doc [B,S] and prefix [B] are device pointers to int32 or NULL; slopes is a HOST pointer to H numbers >= 0, or NULL, read
- * during the call.  T <= S, W and Wv <= 128, H <= 256.  Deterministic.
+ * during the call.  T <= S <= 4194240, W and Wv <= 128, H <= 256.  Deterministic.
  */
 typedef struct l1attn_masked_desc {
     int64_t B, T, S, H, Hk, W, Wv;
@@ -408,7 +408,9 @@ typedef struct l1attn_masked_desc {
     const int32_t* prefix;
 } l1attn_masked_desc;
 
-int l1attn_masked_fwd(const l1attn_masked_desc* desc, const void* q, const void* k, const void* v, void* o, float* lse, void* stream);
+size_t l1attn_masked_fwd_workspace_bytes(const l1attn_masked_desc* desc);
+int l1attn_masked_fwd(const l1attn_masked_desc* desc, const void* q, const void* k, const void* v, void* o, float* lse, void* workspace,
+                      size_t workspace_bytes, void* stream);
 /* dq, dk, dv of o's gradient d_o, from the forward's o and lse; sign(0) = 0.  Shared key heads and rows are summed in a fixed order. */
 size_t l1attn_masked_bwd_workspace_bytes(const l1attn_masked_desc* desc);
 int l1attn_masked_bwd(const l1attn_masked_desc* desc, const void* q, const void* k, const void* v, const void* o, const float* lse,

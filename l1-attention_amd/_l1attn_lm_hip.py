@@ -22,7 +22,9 @@ def lib():
     L = _hip.lib()
     if _bound is not L:
         L.l1attn_masked_fwd.restype = _c_i
-        L.l1attn_masked_fwd.argtypes = [_c_p] * 7
+        L.l1attn_masked_fwd.argtypes = [_c_p] * 7 + [_c_sz, _c_p]
+        L.l1attn_masked_fwd_workspace_bytes.restype = _c_sz
+        L.l1attn_masked_fwd_workspace_bytes.argtypes = [_c_p]
         L.l1attn_masked_bwd_workspace_bytes.restype = _c_sz
         L.l1attn_masked_bwd_workspace_bytes.argtypes = [_c_p]
         L.l1attn_masked_bwd.restype = _c_i
@@ -123,9 +125,12 @@ def masked_forward(q, k, v, doc=None, prefix=None, causal=True, softcap=0.0, slo
     d = _masked_desc(q, k, v, doc, prefix, causal, softcap, slopes)
     o = torch.empty((d.B, d.T, d.H, d.Wv), dtype=q.dtype, device=q.device)
     lse = torch.empty((d.B, d.T, d.H), dtype=torch.float32, device=q.device) if want_lse else None
+    L = lib()
     with torch.cuda.device(q.device):
-        rc = lib().l1attn_masked_fwd(ctypes.addressof(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-                                     None if lse is None else lse.data_ptr(), stream_of(q))
+        n = L.l1attn_masked_fwd_workspace_bytes(ctypes.addressof(d))
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+        rc = L.l1attn_masked_fwd(ctypes.addressof(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                                 None if lse is None else lse.data_ptr(), ws.data_ptr() if n else None, n, stream_of(q))
     check(rc, "l1attn_masked_fwd")
     return [o, lse]
 

@@ -1,0 +1,1252 @@
+// Masked L1 attention for gfx950, forward and backward, float32 / float16 / bfloat16, grouped key heads:
+//
+//   a[t,s] = -1/sqrt(W) * sum_w |q[t,w] - k[s,w]|         c = cap * tanh(a / cap)      (cap > 0, else c = a)
+//   x[t,s] = c - slope[h] * |i - s|                        i = S - T + t, the query's place among the S tokens
+//   p[t,s] = exp(x) / (1 + sum_s exp(x))                   over the visible s; the 1 is the no-op logit
+//   o[t]   = sum_s p[t,s] * v[s]
+//   visible: (not causal or s <= i or s < prefix[b]) and (no documents or doc[b,s] == doc[b,i] >= 0)
+//
+// Every logit is <= 0 (slopes are not negative) and the no-op logit is 0, so a row needs no running maximum: exp(x) <= 1,
+// the denominator is >= 1, partial sums over pieces of the keys add up, and a row that sees nothing comes out as zero.
+//
+// One wavefront owns 32 rows ("owners": queries in the forward and in the gradient of q, keys in that of k and v) and walks
+// the other side ("stream") in tiles of 64, which the waves of a workgroup share through LDS.  Three parts of a tile use
+// three maps of its 32 x 64 pairs onto the lanes, joined by a wave-private LDS scratch:
+//   distances  lane (i,j) = (lane & 7, lane >> 3) holds owners i + 8a (a < 4) and stream rows j + 8b (b < 8): 12 LDS reads of
+//              16 bytes feed 32 pairs; |q - k| is no contraction, so this is vector-ALU work
+//   products   p*v, do*v: matrix instructions; column order of a tile: c = 32*(b/4) + 4*j + b%4, so that a lane's four values
+//              of one half of the tile are neighbours
+//   signs      lane = column w; the 32 owners' sums live in registers, the score gradients come as broadcast LDS reads
+// LDS reads are issued one step ahead of their use, held there by scheduling barriers: left alone, the compiler puts each read
+// right before its use, and waits (signs: 12.9 -> 6.6 cycles per 64 pair-elements, float32 distances: 6.7 -> 5.2, at two waves
+// a SIMD and 2.4 GHz; the instructions alone are 5.2 and 5.2).
+//
+// 16-bit inputs: distances are sums of |difference| of 16-bit codes (v_sad_u16: two pair-elements an instruction; 2.5 cycles per
+// 64 pair-elements against 5.2 in float32).  The codes are a grid over the range [lo, hi] of the workgroup's owner rows; a stream
+// value x outside of it counts as |x - clip(x)|, summed per stream row, plus the code of clip(x): for an owner q within
+// the range |q - x| = |q - clip(x)| + |clip(x) - x|.  Each code is off by half a step u = (hi - lo) / 65535 at most, which moves a
+// logit by u * sqrt(1/6) = 0.41 u on average: below the rounding of p to 16 bits as long as hi - lo is at most kRange.  A
+// workgroup whose owners spread further (or are not finite) takes float32 distances, half of the columns at a time.  Signs do
+// not go by these codes but by the bits of the values themselves, as integers in order: sign(q - k) is exact.
+#pragma once
+#include "common.h"
+#include "masked.h"
+#include <math.h>
+
+namespace {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+
+constexpr int kOwn = 32;        // owner rows of a wave
+constexpr int kTile = 64;       // stream rows of a tile
+constexpr int kPad = 36;        // floats in a row of the scratch: 9 chunks of 16 bytes, odd, so rows spread over the banks
+constexpr int kPitch = 72;      // 16-bit values in a row of 64 (p in the scratch, transposed values): 9 chunks
+constexpr int kScratch = kOwn * kPad * 4;
+constexpr int kClasses = 1024;  // tiles whose visibility is worked out at a time
+constexpr float kMax = 3.402823466e38f;
+
+template <typename ST> constexpr bool k16 = sizeof(ST) == 2;
+// widest range of the owners' values for which 16-bit codes are fine enough: 0.41 * range / 65535 against half a step of the
+// type, 2^-12 (float16) and 2^-9 (bfloat16) on average
+template <typename ST> constexpr float kRange = 24.f;
+template <> constexpr float kRange<__bf16> = 160.f;
+// what a weight is multiplied by before it is rounded to 16 bits: p <= 1, and float16 has no room below 2^-14
+template <typename ST> constexpr float kWeight = 1.f;
+template <> constexpr float kWeight<_Float16> = 16384.f;
+
+// an odd number of 16-byte chunks for n of them: neighbouring rows start in different banks
+__host__ __device__ __forceinline__ int odd_chunks(int n) { return n | 1; }
+
+// LDS of a workgroup in bytes from the front, the same on host and device.  Rows: own/str distances' rows, oraw/raw the same
+// rows' ordered integers (16-bit backward), y the stream's values (float32: rows in product order; 16-bit: rows in product order in
+// the backward), yt the same transposed (16-bit, where they are multiplied by p).
+struct Layout {
+	int own, oraw, str, raw, y, yt, scratch, rows, total;
+	int so, sr, sy;  // bytes of a row of own/str, oraw/raw, y
+};
+
+template <typename ST>
+__host__ __device__ inline Layout masked_layout(int W, int Wv, int waves, bool backward, bool weigh)
+{
+	Layout l;
+	const int per = 16 / (int)sizeof(ST);
+	l.so = odd_chunks((W + per - 1) / per) * 16;
+	l.sr = (W + 7) / 8 * 16;
+	l.sy = odd_chunks(k16<ST> ? (Wv + 31) / 32 * 4 : (Wv + 3) / 4) * 16;
+	l.own = 0;
+	l.oraw = l.own + waves * kOwn * l.so;
+	l.str = l.oraw + (k16<ST> && backward ? waves * kOwn * l.sr : 0);
+	l.raw = l.str + kTile * l.so;
+	l.y = l.raw + (k16<ST> && backward ? kTile * l.sr : 0);
+	l.yt = l.y + (!k16<ST> || backward ? kTile * l.sy : 0);
+	l.scratch = l.yt + (k16<ST> && weigh ? (Wv + 15) / 16 * 16 * kPitch * 2 : 0);
+	l.rows = l.scratch + waves * kScratch;  // documents, lse, D, what lies outside of the range (64 each), 64 words for reductions, classes
+	l.total = l.rows + (4 * kTile + 64) * 4 + kClasses;
+	return l;
+}
+
+template <typename ST> __device__ __forceinline__ float to_f(ST x) { return (float)x; }
+
+// 16 bytes' worth of a row's elements, raw; elements past `n` are zero
+template <typename ST>
+__device__ __forceinline__ uint4 load_raw(const ST* __restrict__ p, int n, bool vec)
+{
+	constexpr int per = 16 / (int)sizeof(ST);
+	if (vec && n >= per) return *reinterpret_cast<const uint4*>(p);
+	ST h[per];
+#pragma unroll
+	for (int e = 0; e < per; e++) h[e] = e < n ? p[e] : (ST)0.f;
+	uint4 r;
+	__builtin_memcpy(&r, h, 16);
+	return r;
+}
+
+template <typename ST, int per = 16 / (int)sizeof(ST)>
+__device__ __forceinline__ void unpack(const uint4& r, float (&x)[per])
+{
+	ST h[per];
+	__builtin_memcpy(h, &r, 16);
+#pragma unroll
+	for (int e = 0; e < per; e++) x[e] = to_f(h[e]);
+}
+
+// The bits of a 16-bit float as an integer in the same order: -0 and 0 are 0, and equal values and no others are equal.
+__device__ __forceinline__ int ordered(unsigned bits) { return bits & 0x8000u ? -(int)(bits & 0x7fffu) : (int)bits; }
+
+// stream row r of a tile <-> its place c in the order of the products
+__device__ __forceinline__ int col_of(int r) { return 32 * (r >> 5) + 4 * (r & 7) + ((r >> 3) & 3); }
+__device__ __forceinline__ int row_of(int c) { return ((c >> 2) & 7) + 8 * (4 * (c >> 5) + (c & 3)); }
+
+// a wave's own stores to LDS before its loads of them (LDS works a wave's accesses off in order; this keeps the compiler to it)
+__device__ __forceinline__ void wave_sync()
+{
+	__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+	__builtin_amdgcn_wave_barrier();
+}
+
+__device__ __forceinline__ int wave_min(int x)
+{
+#pragma unroll
+	for (int m = 32; m; m >>= 1) x = min(x, __shfl_xor(x, m));
+	return x;
+}
+__device__ __forceinline__ int wave_max(int x)
+{
+#pragma unroll
+	for (int m = 32; m; m >>= 1) x = max(x, __shfl_xor(x, m));
+	return x;
+}
+__device__ __forceinline__ float wave_minf(float x)
+{
+#pragma unroll
+	for (int m = 32; m; m >>= 1) x = fminf(x, __shfl_xor(x, m));
+	return x;
+}
+__device__ __forceinline__ float wave_maxf(float x)
+{
+#pragma unroll
+	for (int m = 32; m; m >>= 1) x = fmaxf(x, __shfl_xor(x, m));
+	return x;
+}
+
+// ------------------------------------------------------------------------------------------------------------- distances
+
+// float32 rows, columns [0, 4 * chunks): acc[a][b] += L1 distance of owner i + 8a and stream row j + 8b.  Four terms are summed
+// as a tree before they join the sum: a quarter of the roundings there.
+__device__ __forceinline__ void distances32(const char* own, const char* str, int chunks, int stride, int i, int j, float (&acc)[4][8])
+{
+	const char *po = own + i * stride, *ps = str + j * stride;
+	f4 o[4], s[8];
+#pragma unroll
+	for (int a = 0; a < 4; a++) o[a] = *reinterpret_cast<const f4*>(po + 8 * a * stride);
+#pragma unroll
+	for (int b = 0; b < 8; b++) s[b] = *reinterpret_cast<const f4*>(ps + 8 * b * stride);
+#pragma unroll 2
+	for (int c = 0; c < chunks; c++) {
+		const int d = 16 * min(c + 1, chunks - 1);
+		f4 on[4], sn[8];
+#pragma unroll
+		for (int a = 0; a < 4; a++) on[a] = *reinterpret_cast<const f4*>(po + 8 * a * stride + d);
+#pragma unroll
+		for (int b = 0; b < 8; b++) sn[b] = *reinterpret_cast<const f4*>(ps + 8 * b * stride + d);
+		__builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+		for (int b = 0; b < 8; b++)
+#pragma unroll
+			for (int a = 0; a < 4; a++) {
+				const float d0 = o[a][0] - s[b][0], d1 = o[a][1] - s[b][1], d2 = o[a][2] - s[b][2], d3 = o[a][3] - s[b][3];
+				acc[a][b] += (__builtin_fabsf(d0) + __builtin_fabsf(d1)) + (__builtin_fabsf(d2) + __builtin_fabsf(d3));
+			}
+		__builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+		for (int a = 0; a < 4; a++) o[a] = on[a];
+#pragma unroll
+		for (int b = 0; b < 8; b++) s[b] = sn[b];
+	}
+}
+
+// rows of 16-bit codes, eight to a chunk
+__device__ __forceinline__ void distances16(const char* own, const char* str, int chunks, int stride, int i, int j, unsigned (&acc)[4][8])
+{
+	const char *po = own + i * stride, *ps = str + j * stride;
+	uint4 o[4], s[8];
+#pragma unroll
+	for (int a = 0; a < 4; a++) o[a] = *reinterpret_cast<const uint4*>(po + 8 * a * stride);
+#pragma unroll
+	for (int b = 0; b < 8; b++) s[b] = *reinterpret_cast<const uint4*>(ps + 8 * b * stride);
+#pragma unroll 2
+	for (int c = 0; c < chunks; c++) {
+		const int d = 16 * min(c + 1, chunks - 1);
+		uint4 on[4], sn[8];
+#pragma unroll
+		for (int a = 0; a < 4; a++) on[a] = *reinterpret_cast<const uint4*>(po + 8 * a * stride + d);
+#pragma unroll
+		for (int b = 0; b < 8; b++) sn[b] = *reinterpret_cast<const uint4*>(ps + 8 * b * stride + d);
+		__builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+		for (int b = 0; b < 8; b++)
+#pragma unroll
+			for (int a = 0; a < 4; a++) {
+				unsigned t = acc[a][b];
+				t = __builtin_amdgcn_sad_u16(o[a].x, s[b].x, t);
+				t = __builtin_amdgcn_sad_u16(o[a].y, s[b].y, t);
+				t = __builtin_amdgcn_sad_u16(o[a].z, s[b].z, t);
+				t = __builtin_amdgcn_sad_u16(o[a].w, s[b].w, t);
+				acc[a][b] = t;
+			}
+		__builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+		for (int a = 0; a < 4; a++) o[a] = on[a];
+#pragma unroll
+		for (int b = 0; b < 8; b++) s[b] = sn[b];
+	}
+}
+
+// --------------------------------------------------------------------------------------------------------------- staging
+
+// columns [w0, w0 + width) of rows [r0, r0 + n) of x as float32 rows of `stride` bytes
+template <typename ST>
+__device__ __forceinline__ void stage32(char* dst, const ST* __restrict__ x, int r0, int n, int L, int64_t pitch, int w0, int width,
+                                        int stride, bool vec, int tid, int threads)
+{
+	const int chunks = (width + 3) >> 2, j = tid & 7;
+	for (int r = tid >> 3; r < n; r += threads >> 3) {
+		const ST* row = x + (int64_t)(r0 + r) * pitch + w0;
+		for (int c = j; c < chunks; c += 8) {
+			f4 y = {0.f, 0.f, 0.f, 0.f};
+			if (r0 + r < L) {
+				if constexpr (!k16<ST>) {
+					if (vec && 4 * c + 4 <= width) y = *reinterpret_cast<const f4*>(row + 4 * c);
+					else
+#pragma unroll
+						for (int e = 0; e < 4; e++) y[e] = 4 * c + e < width ? to_f(row[4 * c + e]) : 0.f;
+				} else {
+#pragma unroll
+					for (int e = 0; e < 4; e++) y[e] = 4 * c + e < width ? to_f(row[4 * c + e]) : 0.f;
+				}
+			}
+			*reinterpret_cast<f4*>(dst + r * stride + 16 * c) = y;
+		}
+	}
+}
+
+// the grid of a workgroup's codes
+struct Grid { float lo, hi, sc, inv; };
+
+// Rows as codes.  OVER: each row's distance from the range into over[]; a wave of eight rows a step, eight lanes a row.
+// RAW: also the values' ordered integers.
+template <typename ST, bool OVER, bool RAW>
+__device__ __forceinline__ void stage16(char* dst, char* raw, float* over, const ST* __restrict__ x, int r0, int n, int L, int64_t pitch, int W,
+                                        int stride, int rstride, const Grid& G, bool vec, int tid, int threads)
+{
+	const int chunks = (W + 7) >> 3, j = tid & 7;
+	for (int r = tid >> 3; r < n; r += threads >> 3) {
+		const bool in = r0 + r < L;
+		const ST* row = x + (int64_t)(r0 + r) * pitch;
+		float out = 0.f;
+		for (int c = j; c < chunks; c += 8) {
+			uint4 bits = make_uint4(0, 0, 0, 0);
+			if (in) bits = load_raw(row + 8 * c, W - 8 * c, vec);
+			float v[8];
+			unsigned short code[8];
+			unpack<ST>(bits, v);
+#pragma unroll
+			for (int e = 0; e < 8; e++) {
+				const float y = __builtin_amdgcn_fmed3f(v[e], G.lo, G.hi);
+				if (OVER && 8 * c + e < W) out += __builtin_fabsf(v[e] - y);
+				code[e] = 8 * c + e < W ? (unsigned short)(unsigned)__builtin_fmaf(y - G.lo, G.sc, 0.5f) : (unsigned short)0;
+			}
+			uint4 packed;
+			__builtin_memcpy(&packed, code, 16);
+			*reinterpret_cast<uint4*>(dst + r * stride + 16 * c) = packed;
+			if (RAW) {
+				unsigned short b[8];
+				short s[8];
+				__builtin_memcpy(b, &bits, 16);
+#pragma unroll
+				for (int e = 0; e < 8; e++) s[e] = (short)ordered(b[e]);
+				__builtin_memcpy(&packed, s, 16);
+				*reinterpret_cast<uint4*>(raw + r * rstride + 16 * c) = packed;
+			}
+		}
+		if (OVER) {
+			out += __shfl_xor(out, 1);
+			out += __shfl_xor(out, 2);
+			out += __shfl_xor(out, 4);
+			if (j == 0) over[r] = out;
+		}
+	}
+}
+
+// A tile's values: rows in product order (dst, unless NULL) and transposed (dt, unless NULL).  Columns behind the width are
+// zero.  Whether a value was not finite.
+template <typename ST>
+__device__ __forceinline__ bool stage_values(char* dst, char* dt, const ST* __restrict__ x, int r0, int L, int64_t pitch, int Wv, int stride,
+                                             bool vec, int tid, int threads)
+{
+	bool bad = false;
+	if constexpr (!k16<ST>) {
+		const int chunks = stride >> 4, j = tid & 7;
+		for (int r = tid >> 3; r < kTile; r += threads >> 3) {
+			const ST* row = x + (int64_t)(r0 + r) * pitch;
+			for (int c = j; c < chunks; c += 8) {
+				f4 y = {0.f, 0.f, 0.f, 0.f};
+				if (r0 + r < L) {
+					const uint4 bits = load_raw(row + 4 * c, Wv - 4 * c, vec);
+					__builtin_memcpy(&y, &bits, 16);
+				}
+				*reinterpret_cast<f4*>(dst + col_of(r) * stride + 16 * c) = y;
+#pragma unroll
+				for (int e = 0; e < 4; e++) bad |= !(__builtin_fabsf(y[e]) <= kMax);
+			}
+		}
+	} else {
+		// two rows next to each other in the order of the products, eight columns: transposed they are eight pairs
+		const int chunks = (Wv + 7) >> 3, all = dst ? (Wv + 31) / 32 * 4 : (Wv + 15) / 16 * 2;
+		(void)chunks;
+		for (int x2 = tid; x2 < 32 * all; x2 += threads) {
+			const int c2 = x2 & 31, ch = x2 >> 5;
+			const int ra = row_of(2 * c2), rb = row_of(2 * c2 + 1);
+			uint4 A = make_uint4(0, 0, 0, 0), B = A;
+			if (r0 + ra < L && 8 * ch < Wv) A = load_raw(x + (int64_t)(r0 + ra) * pitch + 8 * ch, Wv - 8 * ch, vec);
+			if (r0 + rb < L && 8 * ch < Wv) B = load_raw(x + (int64_t)(r0 + rb) * pitch + 8 * ch, Wv - 8 * ch, vec);
+			if (dst) {
+				*reinterpret_cast<uint4*>(dst + 2 * c2 * stride + 16 * ch) = A;
+				*reinterpret_cast<uint4*>(dst + (2 * c2 + 1) * stride + 16 * ch) = B;
+			}
+			float f[8];
+			unpack<ST>(A, f);
+#pragma unroll
+			for (int e = 0; e < 8; e++) bad |= !(__builtin_fabsf(f[e]) <= kMax);
+			unpack<ST>(B, f);
+#pragma unroll
+			for (int e = 0; e < 8; e++) bad |= !(__builtin_fabsf(f[e]) <= kMax);
+			if (dt && 8 * ch < (Wv + 15) / 16 * 16) {
+				const unsigned a[4] = {A.x, A.y, A.z, A.w}, b[4] = {B.x, B.y, B.z, B.w};
+#pragma unroll
+				for (int e = 0; e < 4; e++) {
+					*reinterpret_cast<unsigned*>(dt + (8 * ch + 2 * e) * kPitch * 2 + 4 * c2) = (a[e] & 0xffffu) | (b[e] << 16);
+					*reinterpret_cast<unsigned*>(dt + (8 * ch + 2 * e + 1) * kPitch * 2 + 4 * c2) = (a[e] >> 16) | (b[e] & 0xffff0000u);
+				}
+			}
+		}
+	}
+	return bad;
+}
+
+// ---------------------------------------------------------------------------------------------------------------- products
+
+template <typename ST>
+__device__ __forceinline__ f4 mma16(const uint4& a, const uint4& b, f4 c)
+{
+	if constexpr (sizeof(ST) == 4) return c;
+	else if constexpr (__is_same(ST, _Float16)) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+	else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+
+// Weights of half a tile into the wave's scratch, and acc[tb][wb] += sum over its 32 columns c of value[c][16 wb + ..] * p[owner][c].
+// 16 bits: p times kWeight, rounded to the type (a relative error of half a step of the type in each weight, as the
+// product's other factor has).
+// `bad` (values that are not finite in a tile of which some is hidden): a hidden pair's weight of zero must not meet them, which
+// a matrix instruction cannot leave out.
+template <typename ST, int NB>
+__device__ __forceinline__ void weigh(f4 (&acc)[2][NB], char* scr, const char* y, const char* yt, int sy, int Wv, const float (&p)[4][4], int half,
+                                      int i, int j, int l16, int g, bool bad)
+{
+	constexpr int pitch = k16<ST> ? 80 : kPad * 4;  // bytes of an owner's 32 weights: odd chunks
+	wave_sync();
+#pragma unroll
+	for (int a = 0; a < 4; a++) {
+		if constexpr (k16<ST>) {
+			ST w[4];
+#pragma unroll
+			for (int e = 0; e < 4; e++) w[e] = (ST)(p[a][e] * kWeight<ST>);
+			uint2 packed;
+			__builtin_memcpy(&packed, w, 8);
+			*reinterpret_cast<uint2*>(scr + (i + 8 * a) * pitch + 8 * j) = packed;
+		} else {
+			const f4 w = {p[a][0], p[a][1], p[a][2], p[a][3]};
+			*reinterpret_cast<f4*>(scr + (i + 8 * a) * pitch + 16 * j) = w;
+		}
+	}
+	wave_sync();
+	if (bad) {
+		for (int c = 0; c < 32; c++)
+#pragma unroll
+			for (int tb = 0; tb < 2; tb++) {
+				const float w = to_f(*reinterpret_cast<const ST*>(scr + (l16 + 16 * tb) * pitch + (int)sizeof(ST) * c));
+				if (w != 0.f)
+#pragma unroll
+					for (int wb = 0; wb < NB; wb++)
+#pragma unroll
+						for (int e = 0; e < 4; e++) {
+							const int col = 16 * wb + 4 * g + e;
+							if (col < Wv) acc[tb][wb][e] += w * to_f(*reinterpret_cast<const ST*>(k16<ST> ? yt + col * kPitch * 2 + 64 * half + 2 * c : y + (32 * half + c) * sy + 4 * col));
+						}
+			}
+		return;
+	}
+	if constexpr (!k16<ST>) {
+		const char* val = y + 32 * half * sy;
+#pragma unroll
+		for (int kc = 0; kc < 2; kc++) {
+			f4 pb[2];
+#pragma unroll
+			for (int tb = 0; tb < 2; tb++) pb[tb] = *reinterpret_cast<const f4*>(scr + (l16 + 16 * tb) * pitch + 64 * kc + 16 * g);
+#pragma unroll
+			for (int e = 0; e < 4; e++) {
+				const char* row = val + (16 * kc + 4 * g + e) * sy + 4 * l16;
+#pragma unroll
+				for (int wb = 0; wb < NB; wb++) {
+					const float av = 16 * wb + l16 < Wv ? *reinterpret_cast<const float*>(row + 64 * wb) : 0.f;
+#pragma unroll
+					for (int tb = 0; tb < 2; tb++) acc[tb][wb] = __builtin_amdgcn_mfma_f32_16x16x4f32(av, pb[tb][e], acc[tb][wb], 0, 0, 0);
+				}
+			}
+		}
+	} else {
+		const int blocks = (Wv + 15) >> 4;
+		uint4 pb[2];
+#pragma unroll
+		for (int tb = 0; tb < 2; tb++) pb[tb] = *reinterpret_cast<const uint4*>(scr + (l16 + 16 * tb) * pitch + 16 * g);
+#pragma unroll
+		for (int wb = 0; wb < NB; wb++) {
+			if (wb >= blocks) break;
+			const uint4 av = *reinterpret_cast<const uint4*>(yt + (16 * wb + l16) * kPitch * 2 + 64 * half + 16 * g);
+#pragma unroll
+			for (int tb = 0; tb < 2; tb++) acc[tb][wb] = mma16<ST>(av, pb[tb], acc[tb][wb]);
+		}
+	}
+}
+
+// --------------------------------------------------------------------------------------------------------------- visibility
+
+struct Span { int lo, hi; };  // least and largest of the document numbers >= 0 (lo > hi: there is none), over a group of rows
+
+// What a tile of the stream is to a group of owners: 0 nothing of it is visible, 1 all of it, 2 some of it.
+// own_lo..own_hi, s_lo..s_hi: places among the S tokens.  OWNK: the owners are keys, the stream queries.
+template <bool OWNK>
+__device__ __forceinline__ int place_class(const L1MaskedArgs& A, int prefix, int own_lo, int own_hi, int s_lo, int s_hi, bool whole)
+{
+	if (!A.causal) return whole ? 1 : 2;
+	const int key_lo = OWNK ? own_lo : s_lo, key_hi = OWNK ? own_hi : s_hi;
+	const int q_lo = OWNK ? s_lo : own_lo, q_hi = OWNK ? s_hi : own_hi;
+	if (key_lo > q_hi && key_lo >= prefix) return 0;
+	return whole && (key_hi <= q_lo || key_hi < prefix) ? 1 : 2;
+}
+
+// the same with documents, by a whole wave; d: the document of stream row `lane` of the tile, -1 where there is none
+__device__ __forceinline__ int doc_class(int c, int d, Span own, bool own_whole)
+{
+	if (!__ballot(d >= 0 && d >= own.lo && d <= own.hi)) return 0;
+	return !own_whole || own.lo != own.hi || __ballot(d != own.lo) ? 2 : c;
+}
+
+// where a workgroup's owners lie and what the two sides are
+struct Block {
+	int b, h, hk, own0, nown;    // batch entry, query head, key head, the workgroup's first owner row, rows it has at most
+	int own_rows, str_rows;      // rows of the owners' and of the stream's side
+	int own_place0, str_place0;  // place of row 0 of either side
+};
+
+// classes of the tiles first + step * t, t < n, for the whole workgroup
+template <bool OWNK>
+__device__ __forceinline__ void classify(const L1MaskedArgs& A, const Block& K, const int* doc, int prefix, int own_lo, int own_hi, Span own_docs,
+                                         bool own_whole, int first, int step, int n, unsigned char* cls, int tid, int threads)
+{
+	const int lane = tid & 63;
+	for (int t = doc ? tid >> 6 : tid; t < n; t += doc ? threads >> 6 : threads) {
+		const int lo = (first + step * t) * kTile, hi = min(lo + kTile, K.str_rows);
+		int c = place_class<OWNK>(A, prefix, own_lo, own_hi, K.str_place0 + lo, K.str_place0 + hi - 1, hi - lo == kTile);
+		if (doc && c) c = doc_class(c, lo + lane < hi ? doc[K.str_place0 + lo + lane] : -1, own_docs, own_whole);
+		if (!doc || lane == 0) cls[t] = (unsigned char)c;
+	}
+}
+
+__device__ __forceinline__ bool sees(const L1MaskedArgs& A, int prefix, bool docs, int qp, int kp, int qd, int kd)
+{
+	bool ok = !A.causal || kp <= qp || kp < prefix;
+	if (docs) ok = ok && qd == kd && qd >= 0;
+	return ok;
+}
+
+// documents of a wave's own rows, and of the workgroup's (through `shared`); whole: each row belongs to one
+__device__ __forceinline__ void owner_docs(const int* doc, const Block& K, int row0, int* shared, int lane, int wave, int waves, Span& mine, bool& mine_whole,
+                                           Span& all, bool& all_whole)
+{
+	int lo = 0x7fffffff, hi = -1, none = 0;
+	if (doc && lane < kOwn && row0 + lane < K.own_rows) {
+		const int d = doc[K.own_place0 + row0 + lane];
+		if (d >= 0) lo = hi = d; else none = 1;
+	}
+	lo = wave_min(lo); hi = wave_max(hi); none = wave_max(none);
+	mine = {lo, hi};
+	mine_whole = !none;
+	if (lane == 0) { shared[3 * wave] = lo; shared[3 * wave + 1] = hi; shared[3 * wave + 2] = none; }
+	__syncthreads();
+	for (int w = 0; w < waves; w++) { lo = min(lo, shared[3 * w]); hi = max(hi, shared[3 * w + 1]); none = max(none, shared[3 * w + 2]); }
+	all = {lo, hi};
+	all_whole = !none;
+}
+
+// The grid over the workgroup's owner rows; false where their values spread too far for it, or are not finite.  Rows that
+// belong to no document are left out: they take part in nothing.
+template <typename ST>
+__device__ __forceinline__ bool owner_grid(const ST* __restrict__ x, const int* doc, const Block& K, int row0, int64_t pitch, int W, bool vec, float* shared,
+                                           int lane, int wave, int waves, Grid& G)
+{
+	float lo = kMax, hi = -kMax;
+	bool finite = true;
+	const int chunks = (W + 7) >> 3;
+	for (int r = lane >> 3; r < kOwn; r += 8) {
+		if (row0 + r >= K.own_rows || (doc && doc[K.own_place0 + row0 + r] < 0)) continue;
+		for (int c = lane & 7; c < chunks; c += 8) {
+			float v[8];
+			unpack<ST>(load_raw(x + (int64_t)(row0 + r) * pitch + 8 * c, W - 8 * c, vec), v);
+#pragma unroll
+			for (int e = 0; e < 8; e++)
+				if (8 * c + e < W) {
+					finite = finite && __builtin_fabsf(v[e]) <= kMax;
+					lo = fminf(lo, v[e]);
+					hi = fmaxf(hi, v[e]);
+				}
+		}
+	}
+	lo = wave_minf(lo); hi = wave_maxf(hi);
+	if (lane == 0) { shared[3 * wave] = lo; shared[3 * wave + 1] = hi; }
+	const bool all_finite = !__syncthreads_or(!finite);
+	for (int w = 0; w < waves; w++) { lo = fminf(lo, shared[3 * w]); hi = fmaxf(hi, shared[3 * w + 1]); }
+	if (lo > hi) lo = hi = 0.f;  // no row takes part
+	G.lo = lo;
+	G.hi = hi;
+	G.sc = hi > lo ? 65535.f / (hi - lo) : 0.f;
+	G.inv = (hi - lo) / 65535.f;
+	// a range so narrow that its scale overflows float32 has no use for codes either
+	return all_finite && hi - lo <= kRange<ST> && G.sc <= 1e30f;
+}
+
+// A wave's distances of one tile, acc[a][b] >= 0 scaled by 1/sqrt(W), NaN where a value is.  Called by all waves of the
+// workgroup; `active`: this wave needs them.  Without a grid 16-bit rows go through LDS as float32, half of the columns at a time.
+template <typename ST>
+__device__ __forceinline__ void tile_distances(char* own, char* str, const float* over, const Layout& Y, int W, float rw, const Grid& G, bool coded,
+                                               bool active, const ST* __restrict__ own_x, int own_r0, int own_rows, int64_t own_pitch,
+                                               const ST* __restrict__ str_x, int s0, int str_rows, int64_t str_pitch, int i, int j, int tid, int threads,
+                                               float (&x)[4][8])
+{
+	if constexpr (!k16<ST>) {
+#pragma unroll
+		for (int a = 0; a < 4; a++)
+#pragma unroll
+			for (int b = 0; b < 8; b++) x[a][b] = 0.f;
+		if (active) distances32(own, str, (W + 3) >> 2, Y.so, i, j, x);
+#pragma unroll
+		for (int a = 0; a < 4; a++)
+#pragma unroll
+			for (int b = 0; b < 8; b++) x[a][b] *= rw;
+	} else if (coded) {
+		if (!active) return;
+		unsigned acc[4][8];
+#pragma unroll
+		for (int a = 0; a < 4; a++)
+#pragma unroll
+			for (int b = 0; b < 8; b++) acc[a][b] = 0;
+		distances16(own, str, (W + 7) >> 3, Y.so, i, j, acc);
+		const float m = G.inv * rw;
+#pragma unroll
+		for (int b = 0; b < 8; b++) {
+			const float o = over[j + 8 * b] * rw;
+#pragma unroll
+			for (int a = 0; a < 4; a++) x[a][b] = __builtin_fmaf((float)acc[a][b], m, o);
+		}
+	} else {
+#pragma unroll
+		for (int a = 0; a < 4; a++)
+#pragma unroll
+			for (int b = 0; b < 8; b++) x[a][b] = 0.f;
+		const int part = 4 * (((W + 7) >> 3));  // columns that fit a row of codes
+		for (int w0 = 0; w0 < W; w0 += part) {
+			const int n = min(part, W - w0);
+			__syncthreads();
+			stage32(own, own_x, own_r0, kOwn, own_rows, own_pitch, w0, n, Y.so, false, tid & 63, 64);
+			stage32(str, str_x, s0, kTile, str_rows, str_pitch, w0, n, Y.so, false, tid, threads);
+			__syncthreads();
+			if (active) distances32(own, str, (n + 3) >> 2, Y.so, i, j, x);
+		}
+#pragma unroll
+		for (int a = 0; a < 4; a++)
+#pragma unroll
+			for (int b = 0; b < 8; b++) x[a][b] *= rw;
+	}
+}
+
+// capped score and, in fac, its derivative by the score, from the distance over sqrt(W)
+template <typename ST, bool CAP>
+__device__ __forceinline__ float score(float dist, float cap, float icap, float& fac)
+{
+	if constexpr (!CAP) {
+		fac = 1.f;
+		return -dist;
+	} else {
+		float th;
+		if constexpr (k16<ST>) {
+			// tanh(y) = (e^2y - 1) / (e^2y + 1) for y <= 0: off by 2^-23 absolutely, which is what a 16-bit result sees
+			const float e = __builtin_amdgcn_exp2f(dist * (-2.885390082f * icap));
+			th = (e - 1.f) * __builtin_amdgcn_rcpf(e + 1.f);
+		} else {
+			th = tanhf(-dist * icap);
+		}
+		fac = 1.f - th * th;
+		return cap * th;
+	}
+}
+
+template <typename ST>
+__device__ __forceinline__ float weight(float x)
+{
+	if constexpr (k16<ST>) return __builtin_amdgcn_exp2f(x * 1.442695041f);
+	else return expf(x);
+}
+
+// ----------------------------------------------------------------------------------------------------------------- forward
+
+// NB: 16-column blocks of the value width held by a wave.  Grid: x = batch * head (heads next to each other go to different
+// XCDs and one head's tiles to one), y = owner tiles, the last first: under causality it has the most to do; z = splits: split
+// z takes every gridDim.z-th tile of the stream.  part: NULL, or [splits][B][T][H][Wv + 1] sums to be joined, weights' sum last.
+template <typename ST, bool CAP, int NB, int THREADS>
+__global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* __restrict__ q, const ST* __restrict__ k,
+                                                      const ST* __restrict__ v, ST* __restrict__ o, float* __restrict__ lse, float* __restrict__ part)
+{
+	extern __shared__ __align__(16) char lds[];
+	const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 63, wave = tid >> 6, waves = threads >> 6;
+	const int i = lane & 7, j = lane >> 3, l16 = lane & 15, g = lane >> 4;
+	Block K;
+	K.b = blockIdx.x / A.H; K.h = blockIdx.x % A.H; K.hk = K.h / (A.H / A.Hk);
+	K.nown = waves * kOwn; K.own0 = (gridDim.y - 1 - blockIdx.y) * K.nown;
+	K.own_rows = A.T; K.str_rows = A.S; K.own_place0 = A.S - A.T; K.str_place0 = 0;
+	const int row0 = K.own0 + wave * kOwn;
+	const Layout Y = masked_layout<ST>(A.W, A.Wv, waves, false, true);
+	char *own = lds + Y.own + wave * kOwn * Y.so, *str = lds + Y.str, *y = lds + Y.y, *yt = lds + Y.yt, *scr = lds + Y.scratch + wave * kScratch;
+	int* docs = reinterpret_cast<int*>(lds + Y.rows);
+	float* over = reinterpret_cast<float*>(lds + Y.rows) + 3 * kTile;
+	float* red = over + kTile;
+	unsigned char* cls = reinterpret_cast<unsigned char*>(red + 64);
+	const int* doc = A.doc ? A.doc + (int64_t)K.b * A.S : nullptr;
+	const int prefix = A.prefix ? A.prefix[K.b] : 0;
+	const float slope = A.has_slopes ? A.slopes[K.h] : 0.f;
+	const int64_t qpitch = (int64_t)A.H * A.W, kpitch = (int64_t)A.Hk * A.W, vpitch = (int64_t)A.Hk * A.Wv;
+	const ST* qh = q + ((int64_t)K.b * A.T * A.H + K.h) * A.W;
+	const ST* kh = k + ((int64_t)K.b * A.S * A.Hk + K.hk) * A.W;
+	const ST* vh = v + ((int64_t)K.b * A.S * A.Hk + K.hk) * A.Wv;
+
+	Span mine, all;
+	bool mine_whole, all_whole;
+	owner_docs(doc, K, row0, reinterpret_cast<int*>(red), lane, wave, waves, mine, mine_whole, all, all_whole);
+	Grid G = {0.f, 0.f, 0.f, 0.f};
+	bool coded = false;
+	if constexpr (k16<ST>) {
+		coded = owner_grid(qh, doc, K, row0, qpitch, A.W, A.vec & 1, red + 32, lane, wave, waves, G);
+		if (coded) stage16<ST, false, false>(own, nullptr, nullptr, qh, row0, kOwn, A.T, qpitch, A.W, Y.so, 0, G, A.vec & 1, lane, 64);
+	} else {
+		stage32(own, qh, row0, kOwn, A.T, qpitch, 0, A.W, Y.so, A.vec & 1, lane, 64);
+	}
+	const int own_lo = K.own_place0 + K.own0, own_hi = K.own_place0 + min(K.own0 + K.nown, A.T) - 1;
+	const int my_lo = K.own_place0 + row0, my_hi = K.own_place0 + min(row0 + kOwn, A.T) - 1;
+	int od4[4];
+#pragma unroll
+	for (int a = 0; a < 4; a++) od4[a] = doc && row0 + i + 8 * a < A.T ? doc[my_lo + i + 8 * a] : -1;
+	f4 out[2][NB];
+	float den[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+	for (int tb = 0; tb < 2; tb++)
+#pragma unroll
+		for (int wb = 0; wb < NB; wb++) out[tb][wb] = (f4)(0.f);
+	const int s_end = A.causal ? min(A.S, max(own_hi + 1, prefix)) : A.S;  // nothing behind is visible
+	const int tiles = (s_end + kTile - 1) / kTile, step = gridDim.z;
+	for (int t0 = blockIdx.z; t0 < tiles; t0 += step * kClasses) {
+		const int n = min(kClasses, (tiles - t0 + step - 1) / step);
+		__syncthreads();
+		classify<false>(A, K, doc, prefix, own_lo, own_hi, all, all_whole, t0, step, n, cls, tid, threads);
+		__syncthreads();
+		for (int t = 0; t < n; t++) {
+			if (!cls[t]) continue;
+			const int kind = cls[t], s0 = (t0 + step * t) * kTile;
+			__syncthreads();
+			if constexpr (!k16<ST>) stage32(str, kh, s0, kTile, A.S, kpitch, 0, A.W, Y.so, A.vec & 2, tid, threads);
+			else if (coded) stage16<ST, true, false>(str, nullptr, over, kh, s0, kTile, A.S, kpitch, A.W, Y.so, 0, G, A.vec & 2, tid, threads);
+			bool bad = stage_values<ST>(k16<ST> ? nullptr : y, yt, vh, s0, A.S, vpitch, A.Wv, Y.sy, A.vec & 4, tid, threads);
+			if (tid < kTile) docs[tid] = doc && s0 + tid < A.S ? doc[s0 + tid] : -1;
+			bad = __syncthreads_or(bad && kind == 2);
+			// what the tile is to this wave's own rows
+			int mykind = row0 < A.T ? kind : 0;
+			if (mykind == 2) {
+				mykind = place_class<false>(A, prefix, my_lo, my_hi, s0, min(s0 + kTile, A.S) - 1, s0 + kTile <= A.S);
+				if (mykind && doc) mykind = doc_class(mykind, docs[lane], mine, mine_whole);
+			}
+			float x[4][8];
+			tile_distances<ST>(own, str, over, Y, A.W, A.rw, G, coded, mykind, qh, row0, A.T, qpitch, kh, s0, A.S, kpitch, i, j, tid, threads, x);
+			if (!mykind) continue;
+			// float32: a tile's sum on its own, then to the total: the roundings of either are fewer
+			f4 tile[2][NB];
+			if constexpr (!k16<ST>)
+#pragma unroll
+				for (int tb = 0; tb < 2; tb++)
+#pragma unroll
+					for (int wb = 0; wb < NB; wb++) tile[tb][wb] = (f4)(0.f);
+#pragma unroll
+			for (int half = 0; half < 2; half++) {
+				float p[4][4];
+#pragma unroll
+				for (int bb = 0; bb < 4; bb++) {
+					const int b = 4 * half + bb, s = s0 + j + 8 * b, sd = docs[j + 8 * b];
+#pragma unroll
+					for (int a = 0; a < 4; a++) {
+						const int place = my_lo + i + 8 * a;
+						float fac;
+						float w = weight<ST>(score<ST, CAP>(x[a][b], A.cap, A.icap, fac) - slope * (float)abs(place - s));
+						if (mykind == 2 && !(s < A.S && sees(A, prefix, doc, place, s, od4[a], sd))) w = 0.f;
+						den[a] += w;
+						p[a][bb] = w;
+					}
+				}
+				if constexpr (k16<ST>) weigh<ST, NB>(out, scr, y, yt, Y.sy, A.Wv, p, half, i, j, l16, g, bad);
+				else weigh<ST, NB>(tile, scr, y, yt, Y.sy, A.Wv, p, half, i, j, l16, g, bad);
+			}
+			if constexpr (!k16<ST>)
+#pragma unroll
+				for (int tb = 0; tb < 2; tb++)
+#pragma unroll
+					for (int wb = 0; wb < NB; wb++) out[tb][wb] += tile[tb][wb];
+		}
+	}
+	// a row's sum lies in the eight lanes j; then to the lanes that hold the row's output
+#pragma unroll
+	for (int a = 0; a < 4; a++) {
+		den[a] += __shfl_xor(den[a], 8);
+		den[a] += __shfl_xor(den[a], 16);
+		den[a] += __shfl_xor(den[a], 32);
+	}
+	float* sc = reinterpret_cast<float*>(scr);
+	wave_sync();
+	if (j == 0)
+#pragma unroll
+		for (int a = 0; a < 4; a++) sc[i + 8 * a] = den[a];
+	wave_sync();
+	const int64_t rows = (int64_t)A.B * A.T * A.H;
+#pragma unroll
+	for (int tb = 0; tb < 2; tb++) {
+		const int t = row0 + 16 * tb + l16;
+		const float d = sc[16 * tb + l16];
+		if (t >= A.T) continue;
+		const int64_t row = ((int64_t)K.b * A.T + t) * A.H + K.h;
+		float* to = part ? part + (blockIdx.z * rows + row) * (A.Wv + 1) : nullptr;
+		const float r = (part ? 1.f : 1.f / (1.f + d)) * (1.f / kWeight<ST>);
+		if (g == 0) {
+			if (part) to[A.Wv] = d;
+			else if (lse) lse[row] = log1pf(d);
+		}
+#pragma unroll
+		for (int wb = 0; wb < NB; wb++) {
+			const int w = 16 * wb + 4 * g;
+			if (!part && k16<ST> && A.vec & 8 && w + 4 <= A.Wv) {
+				ST h[4];
+#pragma unroll
+				for (int e = 0; e < 4; e++) h[e] = (ST)(out[tb][wb][e] * r);
+				uint2 packed;
+				__builtin_memcpy(&packed, h, 8);
+				*reinterpret_cast<uint2*>(o + row * A.Wv + w) = packed;
+			} else {
+#pragma unroll
+				for (int e = 0; e < 4; e++)
+					if (w + e < A.Wv) {
+						if (part) to[w + e] = out[tb][wb][e] * r;
+						else o[row * A.Wv + w + e] = (ST)(out[tb][wb][e] * r);
+					}
+			}
+		}
+	}
+}
+
+template <typename ST>
+__global__ void __launch_bounds__(256) masked_fwd_join(const float* __restrict__ part, int splits, int64_t rows, int Wv, ST* __restrict__ o, float* __restrict__ lse)
+{
+	const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+	if (row >= rows) return;
+	const int lane = threadIdx.x & 63;
+	float d = 0.f, y0 = 0.f, y1 = 0.f;
+	for (int z = 0; z < splits; z++) {
+		const float* p = part + (z * rows + row) * (Wv + 1);
+		d += p[Wv];
+		if (lane < Wv) y0 += p[lane];
+		if (lane + 64 < Wv) y1 += p[lane + 64];
+	}
+	const float r = 1.f / (1.f + d);
+	if (lse && lane == 0) lse[row] = log1pf(d);
+	if (lane < Wv) o[row * Wv + lane] = (ST)(y0 * r);
+	if (lane + 64 < Wv) o[row * Wv + lane + 64] = (ST)(y1 * r);
+}
+
+// ---------------------------------------------------------------------------------------------------------------- backward
+
+// D[row] = sum_w do * o, row = (b, t, h): what the softmax's gradient subtracts
+template <typename ST>
+__global__ void __launch_bounds__(256) masked_bwd_rows(const ST* __restrict__ dout, const ST* __restrict__ o, float* __restrict__ D,
+                                                       int64_t rows, int Wv)
+{
+	const int64_t row = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
+	float s = 0.f;
+	if (row < rows)
+		for (int w = threadIdx.x & 7; w < Wv; w += 8) s += to_f(dout[row * Wv + w]) * to_f(o[row * Wv + w]);
+	s += __shfl_xor(s, 1);
+	s += __shfl_xor(s, 2);
+	s += __shfl_xor(s, 4);
+	if (row < rows && (threadIdx.x & 7) == 0) D[row] = s;
+}
+
+// sum of the splits' gradients, in their order
+template <typename ST>
+__global__ void __launch_bounds__(256) masked_bwd_join(const float* __restrict__ part, int splits, int64_t n, ST* __restrict__ x)
+{
+	const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+	if (at >= n) return;
+	float s = 0.f;
+	for (int z = 0; z < splits; z++) s += part[z * n + at];
+	x[at] = (ST)s;
+}
+
+// Signs of one half tile: sum[u][r] += h * g over its 32 columns c, h = 1, 1/2, 0 for owner >, ==, < stream in column w = lane + 64 u.
+// Owner r = 4 i' + a' is row i' + 8 a'; scr: the gradients g [c][r].
+// 16 bits: the values as integers in order, own + 1/2: h = clamp(own + 1/2 - str, 0, 1), exact.  float32: h =
+// clamp((own - str) * 2^127 + 1/2, 0, 1), exact but for differences below 2^-128, which count in part.
+template <typename ST, int WL>
+__device__ __forceinline__ void signs(float (&sum)[WL][32], const float (&ov)[WL][32], const float* sc, const char* str, int stride, int half, int lane)
+{
+	const auto value = [&](int c, int u) {
+		const char* row = str + row_of(32 * half + c) * stride;
+		if constexpr (k16<ST>) return (float)*reinterpret_cast<const short*>(row + 2 * lane + 128 * u);
+		else return *reinterpret_cast<const float*>(row + 4 * lane + 256 * u);
+	};
+	const int cols = stride / (k16<ST> ? 2 : 4);
+	bool in[WL];
+#pragma unroll
+	for (int u = 0; u < WL; u++) in[u] = lane + 64 * u < cols;
+	f4 g[8];
+	float s[WL];
+#pragma unroll
+	for (int r = 0; r < 8; r++) g[r] = *reinterpret_cast<const f4*>(sc + 4 * r);
+#pragma unroll
+	for (int u = 0; u < WL; u++) s[u] = in[u] ? value(0, u) : 0.f;
+#pragma unroll 2
+	for (int c = 0; c < 32; c++) {
+		const int d = min(c + 1, 31);
+		f4 gn[8];
+		float sn[WL];
+#pragma unroll
+		for (int u = 0; u < WL; u++) sn[u] = in[u] ? value(d, u) : 0.f;
+#pragma unroll
+		for (int r = 0; r < 8; r++) gn[r] = *reinterpret_cast<const f4*>(sc + d * kPad + 4 * r);
+		__builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+		for (int r = 0; r < 32; r++)
+#pragma unroll
+			for (int u = 0; u < WL; u++) {
+				const float df = ov[u][r] - s[u];
+				const float hv = __builtin_amdgcn_fmed3f(k16<ST> ? df : __builtin_fmaf(df, 0x1p127f, 0.5f), 0.f, 1.f);
+				sum[u][r] = __builtin_fmaf(hv, g[r >> 2][r & 3], sum[u][r]);
+			}
+		__builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+		for (int r = 0; r < 8; r++) g[r] = gn[r];
+#pragma unroll
+		for (int u = 0; u < WL; u++) s[u] = sn[u];
+	}
+}
+
+// Gradients of one side.  OWNK false: owners are queries, dx = dq.  OWNK true: owners are keys, dx = dk and dy = dv, summed
+// over the query heads that share them.  WL: columns w a lane holds in the sign part (W <= 64 * WL).  With g = the gradient of
+// the score: sum g * sign = 2 * sum g * h - sum g.  Grid as in the forward; px, py: NULL, or [splits][rows][W], [splits][rows][Wv].
+template <typename ST, bool OWNK, bool CAP, int WL, int NB, int THREADS>
+__global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* __restrict__ q, const ST* __restrict__ k,
+                                                      const ST* __restrict__ v, const ST* __restrict__ dout,
+                                                      const float* __restrict__ lse, const float* __restrict__ D,
+                                                      ST* __restrict__ dx, ST* __restrict__ dy, float* __restrict__ px, float* __restrict__ py)
+{
+	extern __shared__ __align__(16) char lds[];
+	const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 63, wave = tid >> 6, waves = threads >> 6;
+	const int i = lane & 7, j = lane >> 3, l16 = lane & 15, g = lane >> 4;
+	const int group = A.H / A.Hk, heads = OWNK ? A.Hk : A.H;
+	Block K;
+	K.b = blockIdx.x / heads;
+	K.h = blockIdx.x % heads;
+	K.hk = OWNK ? K.h : K.h / group;
+	K.nown = waves * kOwn;
+	// the workgroups with the most to do under causality come first: late queries, early keys
+	K.own0 = (OWNK ? blockIdx.y : gridDim.y - 1 - blockIdx.y) * K.nown;
+	K.own_rows = OWNK ? A.S : A.T;
+	K.str_rows = OWNK ? A.T : A.S;
+	K.own_place0 = OWNK ? 0 : A.S - A.T;
+	K.str_place0 = OWNK ? A.S - A.T : 0;
+	const int row0 = K.own0 + wave * kOwn;
+	const Layout Y = masked_layout<ST>(A.W, A.Wv, waves, true, OWNK);
+	char *own = lds + Y.own + wave * kOwn * Y.so, *str = lds + Y.str, *raw = lds + Y.raw, *y = lds + Y.y, *yt = lds + Y.yt;
+	char* scr = lds + Y.scratch + wave * kScratch;
+	float* sc = reinterpret_cast<float*>(scr);
+	int* docs = reinterpret_cast<int*>(lds + Y.rows);
+	float *slse = reinterpret_cast<float*>(docs) + kTile, *sD = slse + kTile, *over = sD + kTile, *red = over + kTile;
+	unsigned char* cls = reinterpret_cast<unsigned char*>(red + 64);
+	const int* doc = A.doc ? A.doc + (int64_t)K.b * A.S : nullptr;
+	const int prefix = A.prefix ? A.prefix[K.b] : 0;
+	const int64_t qpitch = (int64_t)A.H * A.W, kpitch = (int64_t)A.Hk * A.W;
+	const int64_t opitch = (int64_t)A.H * A.Wv, vpitch = (int64_t)A.Hk * A.Wv;
+	const ST* kh = k + ((int64_t)K.b * A.S * A.Hk + K.hk) * A.W;
+	const ST* vh = v + ((int64_t)K.b * A.S * A.Hk + K.hk) * A.Wv;
+	const ST* own_x = OWNK ? kh : q + ((int64_t)K.b * A.T * A.H + K.h) * A.W;
+	const int64_t own_pitch = OWNK ? kpitch : qpitch, str_pitch = OWNK ? qpitch : kpitch;
+	const bool own_vec = A.vec & (OWNK ? 2 : 1), str_vec = A.vec & (OWNK ? 1 : 2);
+
+	Span mine, all;
+	bool mine_whole, all_whole;
+	owner_docs(doc, K, row0, reinterpret_cast<int*>(red), lane, wave, waves, mine, mine_whole, all, all_whole);
+	Grid G = {0.f, 0.f, 0.f, 0.f};
+	bool coded = false;
+	if constexpr (k16<ST>) {
+		coded = owner_grid(own_x, doc, K, row0, own_pitch, A.W, own_vec, red + 32, lane, wave, waves, G);
+		stage16<ST, false, true>(own, lds + Y.oraw + wave * kOwn * Y.sr, nullptr, own_x, row0, kOwn, K.own_rows, own_pitch, A.W, Y.so, Y.sr, G, own_vec, lane, 64);
+	} else {
+		stage32(own, own_x, row0, kOwn, K.own_rows, own_pitch, 0, A.W, Y.so, own_vec, lane, 64);
+	}
+	const int own_lo = K.own_place0 + K.own0, own_hi = K.own_place0 + min(K.own0 + K.nown, K.own_rows) - 1;
+	const int my_lo = K.own_place0 + row0, my_hi = K.own_place0 + min(row0 + kOwn, K.own_rows) - 1;
+	float sum[WL][32];
+#pragma unroll
+	for (int u = 0; u < WL; u++)
+#pragma unroll
+		for (int r = 0; r < 32; r++) sum[u][r] = 0.f;
+	int od4[4];
+#pragma unroll
+	for (int a = 0; a < 4; a++) od4[a] = doc && row0 + i + 8 * a < K.own_rows ? doc[my_lo + i + 8 * a] : -1;
+	float gsum[4] = {0.f, 0.f, 0.f, 0.f};
+	constexpr int NY = OWNK ? NB : 1;
+	f4 dyv[2][NY];
+#pragma unroll
+	for (int tb = 0; tb < 2; tb++)
+#pragma unroll
+		for (int wb = 0; wb < NY; wb++) dyv[tb][wb] = (f4)(0.f);
+	constexpr int NX = k16<ST> ? (NB + 1) / 2 : NB;  // 16 bytes of a lane each: 32 columns of 16 bits, 16 of float32
+	const int xstep = k16<ST> ? 32 : 16, xlane = k16<ST> ? 8 * g : 4 * g;
+
+	for (int hg = 0; hg < (OWNK ? group : 1); hg++) {
+		const int h = OWNK ? K.hk * group + hg : K.h;
+		const float slope = A.has_slopes ? A.slopes[h] : 0.f;
+		const ST* qh = q + ((int64_t)K.b * A.T * A.H + h) * A.W;
+		const ST* oh = dout + ((int64_t)K.b * A.T * A.H + h) * A.Wv;
+		const ST* str_x = OWNK ? qh : kh;
+		// the owners' rows of the second product (v of the keys, do of the queries), as its right operand
+		uint4 xr[2][NX];
+#pragma unroll
+		for (int ob = 0; ob < 2; ob++) {
+			const int r = row0 + 16 * ob + l16;
+			const ST* row = OWNK ? vh + (int64_t)r * vpitch : oh + (int64_t)r * opitch;
+#pragma unroll
+			for (int kc = 0; kc < NX; kc++) {
+				const int w = xstep * kc + xlane;
+				xr[ob][kc] = make_uint4(0, 0, 0, 0);
+				if (r < K.own_rows && w < A.Wv) xr[ob][kc] = load_raw(row + w, A.Wv - w, OWNK ? A.vec & 4 : A.vec & 8);
+			}
+		}
+		float olse[4], oD[4];
+#pragma unroll
+		for (int a = 0; a < 4; a++) {
+			const int t = row0 + i + 8 * a;
+			const bool in = !OWNK && t < A.T;
+			olse[a] = in ? lse[((int64_t)K.b * A.T + t) * A.H + h] : 0.f;
+			oD[a] = in ? D[((int64_t)K.b * A.T + t) * A.H + h] : 0.f;
+		}
+		int first = 0, last = (K.str_rows + kTile - 1) / kTile;
+		if (A.causal) {
+			if (OWNK) { if (own_lo >= prefix) first = max(0, own_lo - K.str_place0) / kTile; }
+			else last = (min(A.S, max(own_hi + 1, prefix)) + kTile - 1) / kTile;
+		}
+		const int step = gridDim.z;
+		for (int t0 = first + blockIdx.z; t0 < last; t0 += step * kClasses) {
+			const int n = min(kClasses, (last - t0 + step - 1) / step);
+			__syncthreads();
+			classify<OWNK>(A, K, doc, prefix, own_lo, own_hi, all, all_whole, t0, step, n, cls, tid, threads);
+			__syncthreads();
+			for (int t = 0; t < n; t++) {
+				if (!cls[t]) continue;
+				const int kind = cls[t], s0 = (t0 + step * t) * kTile;
+				__syncthreads();
+				if constexpr (!k16<ST>) {
+					stage32(str, str_x, s0, kTile, K.str_rows, str_pitch, 0, A.W, Y.so, str_vec, tid, threads);
+				} else {
+					// without a grid the codes come out as nonsense that nobody reads; the ordered integers are wanted all the same
+					stage16<ST, true, true>(str, raw, over, str_x, s0, kTile, K.str_rows, str_pitch, A.W, Y.so, Y.sr, G, str_vec, tid, threads);
+				}
+				bool bad = stage_values<ST>(y, k16<ST> && OWNK ? yt : nullptr, OWNK ? oh : vh, s0, K.str_rows, OWNK ? opitch : vpitch, A.Wv, Y.sy,
+				                            OWNK ? A.vec & 8 : A.vec & 4, tid, threads);
+				if (tid < kTile) {
+					const bool in = s0 + tid < K.str_rows;
+					docs[tid] = doc && in ? doc[K.str_place0 + s0 + tid] : -1;
+					if (OWNK) {
+						slse[tid] = in ? lse[((int64_t)K.b * A.T + s0 + tid) * A.H + h] : 0.f;
+						sD[tid] = in ? D[((int64_t)K.b * A.T + s0 + tid) * A.H + h] : 0.f;
+					}
+				}
+				bad = __syncthreads_or(bad && kind == 2);
+				int mykind = row0 < K.own_rows ? kind : 0;
+				if (mykind == 2) {
+					mykind = place_class<OWNK>(A, prefix, my_lo, my_hi, K.str_place0 + s0, K.str_place0 + min(s0 + kTile, K.str_rows) - 1, s0 + kTile <= K.str_rows);
+					if (mykind && doc) mykind = doc_class(mykind, docs[lane], mine, mine_whole);
+				}
+				float x[4][8];
+				tile_distances<ST>(own, str, over, Y, A.W, A.rw, G, coded, mykind, own_x, row0, K.own_rows, own_pitch, str_x, s0, K.str_rows, str_pitch, i, j, tid, threads, x);
+				if (!mykind) continue;
+#pragma unroll
+				for (int half = 0; half < 2; half++) {
+					float p[4][4], pf[4][4];  // weights, and times the score's derivative
+#pragma unroll
+					for (int bb = 0; bb < 4; bb++) {
+						const int b = 4 * half + bb, r = j + 8 * b, sp = K.str_place0 + s0 + r, sd = docs[r];
+						const float sl = OWNK ? slse[r] : 0.f;
+#pragma unroll
+						for (int a = 0; a < 4; a++) {
+							const int place = my_lo + i + 8 * a;
+							float fac;
+							float w = weight<ST>(score<ST, CAP>(x[a][b], A.cap, A.icap, fac) - slope * (float)abs(place - sp) - (OWNK ? sl : olse[a]));
+							if (mykind == 2 && !(s0 + r < K.str_rows && (OWNK ? sees(A, prefix, doc, sp, place, sd, od4[a]) : sees(A, prefix, doc, place, sp, od4[a], sd)))) w = 0.f;
+							p[a][bb] = w;
+							pf[a][bb] = w * (CAP ? fac * A.rw : A.rw);
+						}
+					}
+					if constexpr (OWNK) weigh<ST, NY>(dyv, scr, y, yt, Y.sy, A.Wv, p, half, i, j, l16, g, bad);
+					// dp of this half's 32 columns
+					f4 dp[2][2];
+#pragma unroll
+					for (int cb = 0; cb < 2; cb++) {
+						dp[cb][0] = (f4)(0.f);
+						dp[cb][1] = (f4)(0.f);
+#pragma unroll
+						for (int kc = 0; kc < NX; kc++) {
+							const int w = xstep * kc + xlane;
+							if (xstep * kc >= A.Wv) break;
+							const uint4 ya = *reinterpret_cast<const uint4*>(y + (32 * half + 16 * cb + l16) * Y.sy + w * (int)sizeof(ST));
+							if constexpr (k16<ST>) {
+#pragma unroll
+								for (int ob = 0; ob < 2; ob++) dp[cb][ob] = mma16<ST>(ya, xr[ob][kc], dp[cb][ob]);
+							} else {
+								const f4 yf = w * 4 < Y.sy ? __builtin_bit_cast(f4, ya) : (f4)(0.f);
+#pragma unroll
+								for (int e = 0; e < 4; e++)
+#pragma unroll
+									for (int ob = 0; ob < 2; ob++) dp[cb][ob] = __builtin_amdgcn_mfma_f32_16x16x4f32(yf[e], __builtin_bit_cast(f4, xr[ob][kc])[e], dp[cb][ob], 0, 0, 0);
+							}
+						}
+					}
+					wave_sync();
+#pragma unroll
+					for (int cb = 0; cb < 2; cb++)
+#pragma unroll
+						for (int ob = 0; ob < 2; ob++) *reinterpret_cast<f4*>(sc + (l16 + 16 * ob) * kPad + 16 * cb + 4 * g) = dp[cb][ob];
+					wave_sync();
+					f4 d4[4];
+#pragma unroll
+					for (int a = 0; a < 4; a++) d4[a] = *reinterpret_cast<const f4*>(sc + (i + 8 * a) * kPad + 4 * j);
+					wave_sync();
+#pragma unroll
+					for (int bb = 0; bb < 4; bb++) {
+						const int b = 4 * half + bb;
+						const float dD = OWNK ? sD[j + 8 * b] : 0.f;
+						f4 gr;
+#pragma unroll
+						for (int a = 0; a < 4; a++) {
+							// a hidden pair's dp may come from values that are not finite
+							gr[a] = p[a][bb] != 0.f ? pf[a][bb] * ((OWNK ? dD : oD[a]) - d4[a][bb]) : 0.f;
+							gsum[a] += gr[a];
+						}
+						*reinterpret_cast<f4*>(sc + (4 * j + bb) * kPad + 4 * i) = gr;
+					}
+					wave_sync();
+					float ov[WL][32];  // the owners' columns: register r = 4 i' + a' is row i' + 8 a'
+#pragma unroll
+					for (int u = 0; u < WL; u++)
+#pragma unroll
+						for (int r = 0; r < 32; r++) {
+							const int row = (r >> 2) + 8 * (r & 3);
+							const bool in = lane + 64 * u < (k16<ST> ? Y.sr / 2 : Y.so / 4);
+							if constexpr (k16<ST>) ov[u][r] = in ? (float)*reinterpret_cast<const short*>(lds + Y.oraw + (wave * kOwn + row) * Y.sr + 2 * lane + 128 * u) + 0.5f : 0.f;
+							else ov[u][r] = in ? *reinterpret_cast<const float*>(own + row * Y.so + 4 * lane + 256 * u) : 0.f;
+						}
+					if constexpr (k16<ST>) {
+						signs<ST, WL>(sum, ov, sc, raw, Y.sr, half, lane);
+					} else {
+						// half a tile's sum on its own, then to the total: the roundings of either are fewer
+						float part[WL][32];
+#pragma unroll
+						for (int u = 0; u < WL; u++)
+#pragma unroll
+							for (int r = 0; r < 32; r++) part[u][r] = 0.f;
+						signs<ST, WL>(part, ov, sc, str, Y.so, half, lane);
+#pragma unroll
+						for (int u = 0; u < WL; u++)
+#pragma unroll
+							for (int r = 0; r < 32; r++) sum[u][r] += part[u][r];
+					}
+					wave_sync();
+				}
+			}
+		}
+	}
+#pragma unroll
+	for (int a = 0; a < 4; a++) {
+		gsum[a] += __shfl_xor(gsum[a], 8);
+		gsum[a] += __shfl_xor(gsum[a], 16);
+		gsum[a] += __shfl_xor(gsum[a], 32);
+	}
+	wave_sync();
+	if (j == 0)
+#pragma unroll
+		for (int a = 0; a < 4; a++) sc[4 * i + a] = gsum[a];
+	wave_sync();
+	const int64_t rows = (int64_t)A.B * K.own_rows * heads;
+#pragma unroll
+	for (int r = 0; r < 32; r++) {
+		const int t = row0 + (r >> 2) + 8 * (r & 3);
+		const float gs = sc[r];
+		if (t >= K.own_rows) continue;
+		const int64_t row = ((int64_t)K.b * K.own_rows + t) * heads + K.h;
+#pragma unroll
+		for (int u = 0; u < WL; u++)
+			if (lane + 64 * u < A.W) {
+				const float y1 = 2.f * sum[u][r] - gs;
+				if (px) px[(blockIdx.z * rows + row) * A.W + lane + 64 * u] = y1;
+				else dx[row * A.W + lane + 64 * u] = (ST)y1;
+			}
+	}
+	if constexpr (OWNK) {
+#pragma unroll
+		for (int tb = 0; tb < 2; tb++) {
+			const int s = row0 + 16 * tb + l16;
+			if (s >= A.S) continue;
+			const int64_t row = ((int64_t)K.b * A.S + s) * A.Hk + K.hk;
+#pragma unroll
+			for (int wb = 0; wb < NY; wb++)
+#pragma unroll
+				for (int e = 0; e < 4; e++) {
+					const int w = 16 * wb + 4 * g + e;
+					if (w >= A.Wv) continue;
+					const float y1 = dyv[tb][wb][e] * (1.f / kWeight<ST>);
+					if (py) py[(blockIdx.z * rows + row) * A.Wv + w] = y1;
+					else dy[row * A.Wv + w] = (ST)y1;
+				}
+		}
+	}
+}
+
+// ------------------------------------------------------------------------------------------------------------------- host
+
+template <typename F>
+int launch(F* f, dim3 grid, int waves, int bytes, hipStream_t st, void** args)
+{
+	L1_HIP_CHECK(hipFuncSetAttribute((const void*)f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+	L1_HIP_CHECK(hipLaunchKernel((const void*)f, grid, dim3(64 * waves), args, bytes, st));
+	return L1ATTN_OK;
+}
+
+template <typename ST>
+struct MaskedImpl {
+	template <bool CAP>
+	static int fwd_cap(L1MaskedArgs& A, const L1MaskedPlan& P, const void* q, const void* k, const void* v, void* o, float* lse, float* part, hipStream_t st)
+	{
+		const dim3 grid((unsigned)(A.B * A.H), (unsigned)l1_cdiv(A.T, kOwn * P.waves), (unsigned)P.splits);
+		const int bytes = masked_layout<ST>(A.W, A.Wv, P.waves, false, true).total;
+		void* args[] = {&A, &q, &k, &v, &o, &lse, &part};
+		if (A.Wv > 64) return launch(masked_fwd<ST, CAP, 8, 256>, grid, P.waves, bytes, st, args);
+		return launch(masked_fwd<ST, CAP, 4, 512>, grid, P.waves, bytes, st, args);
+	}
+	static int fwd(L1MaskedArgs& A, const L1MaskedPlan& P, const void* q, const void* k, const void* v, void* o, float* lse, float* part, hipStream_t st)
+	{
+		const int rc = A.cap > 0.f ? fwd_cap<true>(A, P, q, k, v, o, lse, part, st) : fwd_cap<false>(A, P, q, k, v, o, lse, part, st);
+		if (rc != L1ATTN_OK || !part) return rc;
+		const int64_t rows = (int64_t)A.B * A.T * A.H;
+		hipLaunchKernelGGL(masked_fwd_join<ST>, dim3((unsigned)l1_cdiv(rows, 4)), dim3(256), 0, st, part, P.splits, rows, A.Wv, (ST*)o, lse);
+		L1_LAUNCH_CHECK();
+		return L1ATTN_OK;
+	}
+	static int rows(const void* dout, const void* o, float* D, int64_t rows, int Wv, hipStream_t st)
+	{
+		hipLaunchKernelGGL(masked_bwd_rows<ST>, dim3((unsigned)l1_cdiv(rows, 32)), dim3(256), 0, st, (const ST*)dout, (const ST*)o, D, rows, Wv);
+		L1_LAUNCH_CHECK();
+		return L1ATTN_OK;
+	}
+	template <bool OWNK, bool CAP>
+	static int side_cap(L1MaskedArgs& A, const L1MaskedPlan& P, const void* q, const void* k, const void* v, const void* dout, const float* lse, const float* D,
+	                    void* dx, void* dy, float* px, float* py, hipStream_t st)
+	{
+		const int64_t heads = (int64_t)A.B * (OWNK ? A.Hk : A.H), n = OWNK ? A.S : A.T;
+		const dim3 grid((unsigned)heads, (unsigned)l1_cdiv(n, kOwn * P.waves), (unsigned)P.splits);
+		const int bytes = masked_layout<ST>(A.W, A.Wv, P.waves, true, OWNK).total;
+		void* args[] = {&A, &q, &k, &v, &dout, &lse, &D, &dx, &dy, &px, &py};
+		if (A.W > 64) return launch(masked_bwd<ST, OWNK, CAP, 2, 8, 256>, grid, P.waves, bytes, st, args);
+		if (A.Wv > 64) return launch(masked_bwd<ST, OWNK, CAP, 1, 8, 256>, grid, P.waves, bytes, st, args);
+		return launch(masked_bwd<ST, OWNK, CAP, 1, 4, 512>, grid, P.waves, bytes, st, args);
+	}
+	template <bool OWNK>
+	static int side(L1MaskedArgs& A, const L1MaskedPlan& P, const void* q, const void* k, const void* v, const void* dout, const float* lse, const float* D,
+	                void* dx, void* dy, float* part, hipStream_t st)
+	{
+		const int64_t nx = (int64_t)A.B * (OWNK ? (int64_t)A.S * A.Hk : (int64_t)A.T * A.H) * A.W, ny = OWNK ? nx / A.W * A.Wv : 0;
+		float *px = P.splits > 1 ? part : nullptr, *py = P.splits > 1 && OWNK ? part + P.splits * nx : nullptr;
+		const int rc = A.cap > 0.f ? side_cap<OWNK, true>(A, P, q, k, v, dout, lse, D, dx, dy, px, py, st)
+		                           : side_cap<OWNK, false>(A, P, q, k, v, dout, lse, D, dx, dy, px, py, st);
+		if (rc != L1ATTN_OK || !px) return rc;
+		hipLaunchKernelGGL(masked_bwd_join<ST>, dim3((unsigned)l1_cdiv(nx, 256)), dim3(256), 0, st, px, P.splits, nx, (ST*)dx);
+		L1_LAUNCH_CHECK();
+		if (OWNK) {
+			hipLaunchKernelGGL(masked_bwd_join<ST>, dim3((unsigned)l1_cdiv(ny, 256)), dim3(256), 0, st, py, P.splits, ny, (ST*)dy);
+			L1_LAUNCH_CHECK();
+		}
+		return L1ATTN_OK;
+	}
+	static int side_q(L1MaskedArgs& A, const L1MaskedPlan& P, const void* q, const void* k, const void* v, const void* dout, const float* lse, const float* D,
+	                  void* dq, float* part, hipStream_t st)
+	{
+		return side<false>(A, P, q, k, v, dout, lse, D, dq, nullptr, part, st);
+	}
+	static int side_k(L1MaskedArgs& A, const L1MaskedPlan& P, const void* q, const void* k, const void* v, const void* dout, const float* lse, const float* D,
+	                  void* dk, void* dv, float* part, hipStream_t st)
+	{
+		return side<true>(A, P, q, k, v, dout, lse, D, dk, dv, part, st);
+	}
+	static int lds(int W, int Wv, int waves, bool backward, bool weigh) { return masked_layout<ST>(W, Wv, waves, backward, weigh).total; }
+};
+
+}  // namespace
+
+#define L1_MASKED_TABLE(name, ST)                                                                                                      \
+	const L1MaskedTable& name()                                                                                                        \
+	{                                                                                                                                  \
+		static const L1MaskedTable t = {MaskedImpl<ST>::fwd, MaskedImpl<ST>::rows, MaskedImpl<ST>::side_q, MaskedImpl<ST>::side_k, MaskedImpl<ST>::lds}; \
+		return t;                                                                                                                      \
+	}

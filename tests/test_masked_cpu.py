@@ -57,18 +57,23 @@ def test_c_entry_codes():
         if slopes:
             keep = (ctypes.c_float * len(slopes))(*slopes)
             desc.slopes = ctypes.addressof(keep)
-        return L.l1attn_masked_fwd(ctypes.addressof(desc), q, one, one, o, None, None)
-    assert L.l1attn_masked_fwd(None, one, one, one, one, None, None) == -1
+        return L.l1attn_masked_fwd(ctypes.addressof(desc), q, one, one, o, None, None, 0, None)
+    assert L.l1attn_masked_fwd(None, one, one, one, one, None, None, 0, None) == -1
     assert fwd(q=None) == -1 and fwd(o=None) == -1
     for kw in (dict(T=5), dict(T=-1), dict(B=-1), dict(H=3), dict(Hk=0), dict(W=0), dict(dtype=3), dict(causal=2), dict(softcap=-1.0),
                dict(softcap=float("nan")), dict(causal=0, prefix=16), dict(slope_values=(0.5, -1.0)), dict(slope_values=(0.5, float("nan")))):
         assert fwd(**kw) == -1, kw
-    for kw in (dict(W=129), dict(Wv=129), dict(H=512), dict(S=1 << 31)):
+    for kw in (dict(W=129), dict(Wv=129), dict(H=512), dict(S=1 << 23)):
         assert fwd(**kw) == -3, kw
     assert fwd(B=0) == 0 and fwd(T=0) == 0  # nothing to do
+    d = drv.MaskedDesc(1, 100, 500, 2, 2, 8, 8, 0, 1, 0.0, None, None, None)
+    n = L.l1attn_masked_fwd_workspace_bytes(ctypes.addressof(d))
+    assert n > 0 and n % (100 * 2 * 9 * 4) == 0  # one [B,T,H,Wv+1] for each split
+    assert L.l1attn_masked_fwd(ctypes.addressof(d), one, one, one, one, None, None, n, None) == -2
+    assert L.l1attn_masked_fwd(ctypes.addressof(d), one, one, one, one, None, one, n - 1, None) == -2
     d = drv.MaskedDesc(1, 4, 4, 2, 2, 8, 8, 0, 1, 0.0, None, None, None)
     n = L.l1attn_masked_bwd_workspace_bytes(ctypes.addressof(d))
-    assert n == 32
+    assert n == 256
     assert L.l1attn_masked_bwd(ctypes.addressof(d), *[one] * 9, None, n, None) == -2
     assert L.l1attn_masked_bwd(ctypes.addressof(d), *[one] * 10, n - 1, None) == -2
     assert L.l1attn_masked_bwd(ctypes.addressof(d), one, None, *[one] * 8, n, None) == -1

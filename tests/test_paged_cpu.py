@@ -148,7 +148,7 @@ def test_binding_matches_the_header():
     import test_abi_signatures_cpu as sig
     declared = {n: s for n, s in sig._prototypes(open(os.path.join(sig.ROOT, "include", "l1attn_hip.h")).read(), ";").items()
                 if n.startswith(("l1attn_masked_", "l1attn_cache_"))}
-    assert len(declared) == 12 and sig._check_binding(drv.lib(), declared, set(declared)) == 12
+    assert len(declared) == 13 and sig._check_binding(drv.lib(), declared, set(declared)) == 13
     # the structs, member by member
     text = sig._strip_comments(open(os.path.join(sig.ROOT, "include", "l1attn_hip.h")).read())
     import re
