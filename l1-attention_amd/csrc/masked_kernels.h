@@ -126,6 +126,14 @@ __device__ __forceinline__ void wave_sync()
 	__builtin_amdgcn_wave_barrier();
 }
 
+// The same value, but unknown to the compiler: what is computed from it is computed here, instead of once for the whole loop and
+// kept in registers that the loop needs.
+__device__ __forceinline__ int here(int x)
+{
+	asm volatile("" : "+v"(x));
+	return x;
+}
+
 __device__ __forceinline__ int wave_min(int x)
 {
 #pragma unroll
@@ -417,10 +425,10 @@ __device__ __forceinline__ void weigh(f4 (&acc)[2][NB], char* scr, const char* y
 			for (int tb = 0; tb < 2; tb++) pb[tb] = *reinterpret_cast<const f4*>(scr + (l16 + 16 * tb) * pitch + 64 * kc + 16 * g);
 #pragma unroll
 			for (int e = 0; e < 4; e++) {
-				const char* row = val + (16 * kc + 4 * g + e) * sy + 4 * l16;
+				const char* row = val + (16 * kc + 4 * g + e) * sy;
 #pragma unroll
 				for (int wb = 0; wb < NB; wb++) {
-					const float av = 16 * wb + l16 < Wv ? *reinterpret_cast<const float*>(row + 64 * wb) : 0.f;
+					const float av = *reinterpret_cast<const float*>(row + 4 * min(16 * wb + l16, Wv - 1));  // rows behind the width are not written
 #pragma unroll
 					for (int tb = 0; tb < 2; tb++) acc[tb][wb] = __builtin_amdgcn_mfma_f32_16x16x4f32(av, pb[tb][e], acc[tb][wb], 0, 0, 0);
 				}
@@ -485,11 +493,10 @@ __device__ __forceinline__ void classify(const L1MaskedArgs& A, const Block& K, 
 	}
 }
 
-__device__ __forceinline__ bool sees(const L1MaskedArgs& A, int prefix, bool docs, int qp, int kp, int qd, int kd)
+// no short cuts: a branch for every pair would cost more than the comparisons
+__device__ __forceinline__ bool sees(bool open, int prefix, bool nodocs, int qp, int kp, int qd, int kd)
 {
-	bool ok = !A.causal || kp <= qp || kp < prefix;
-	if (docs) ok = ok && qd == kd && qd >= 0;
-	return ok;
+	return (open | (kp <= qp) | (kp < prefix)) & (nodocs | ((qd == kd) & (qd >= 0)));
 }
 
 // documents of a wave's own rows, and of the workgroup's (through `shared`); whole: each row belongs to one
@@ -692,6 +699,7 @@ __global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* 
 		for (int t = 0; t < n; t++) {
 			if (!cls[t]) continue;
 			const int kind = cls[t], s0 = (t0 + step * t) * kTile;
+			const int tid = here(threadIdx.x), lane = tid & 63, i = lane & 7, j = lane >> 3, l16 = lane & 15, g = lane >> 4;
 			__syncthreads();
 			if constexpr (!k16<ST>) stage32(str, kh, s0, kTile, A.S, kpitch, 0, A.W, Y.so, A.vec & 2, tid, threads);
 			else if (coded) stage16<ST, true, false>(str, nullptr, over, kh, s0, kTile, A.S, kpitch, A.W, Y.so, 0, G, A.vec & 2, tid, threads);
@@ -719,17 +727,27 @@ __global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* 
 				float p[4][4];
 #pragma unroll
 				for (int bb = 0; bb < 4; bb++) {
-					const int b = 4 * half + bb, s = s0 + j + 8 * b, sd = docs[j + 8 * b];
+					const int b = 4 * half + bb;
+					const float s = (float)(s0 + j + 8 * b - my_lo - i);
 #pragma unroll
 					for (int a = 0; a < 4; a++) {
-						const int place = my_lo + i + 8 * a;
 						float fac;
-						float w = weight<ST>(score<ST, CAP>(x[a][b], A.cap, A.icap, fac) - slope * (float)abs(place - s));
-						if (mykind == 2 && !(s < A.S && sees(A, prefix, doc, place, s, od4[a], sd))) w = 0.f;
-						den[a] += w;
-						p[a][bb] = w;
+						p[a][bb] = weight<ST>(__builtin_fmaf(-slope, __builtin_fabsf(s - 8.f * a), score<ST, CAP>(x[a][b], A.cap, A.icap, fac)));
 					}
 				}
+				if (mykind == 2) {
+#pragma unroll
+					for (int bb = 0; bb < 4; bb++) {
+						const int s = s0 + j + 8 * (4 * half + bb), sd = docs[j + 8 * (4 * half + bb)];
+#pragma unroll
+						for (int a = 0; a < 4; a++)
+							p[a][bb] = (s < A.S) & sees(!A.causal, prefix, !doc, my_lo + i + 8 * a, s, od4[a], sd) ? p[a][bb] : 0.f;
+					}
+				}
+#pragma unroll
+				for (int bb = 0; bb < 4; bb++)
+#pragma unroll
+					for (int a = 0; a < 4; a++) den[a] += p[a][bb];
 				if constexpr (k16<ST>) weigh<ST, NB>(out, scr, y, yt, Y.sy, A.Wv, p, half, i, j, l16, g, bad);
 				else weigh<ST, NB>(tile, scr, y, yt, Y.sy, A.Wv, p, half, i, j, l16, g, bad);
 			}
@@ -840,30 +858,26 @@ __global__ void __launch_bounds__(256) masked_bwd_join(const float* __restrict__
 // 16 bits: the values as integers in order, own + 1/2: h = clamp(own + 1/2 - str, 0, 1), exact.  float32: h =
 // clamp((own - str) * 2^127 + 1/2, 0, 1), exact but for differences below 2^-128, which count in part.
 template <typename ST, int WL>
-__device__ __forceinline__ void signs(float (&sum)[WL][32], const float (&ov)[WL][32], const float* sc, const char* str, int stride, int half, int lane)
+__device__ __forceinline__ void signs(float (&sum)[WL][32], const float (&ov)[WL][32], const float* sc, const char* str, int stride, int half, int lane, int W)
 {
 	const auto value = [&](int c, int u) {
-		const char* row = str + row_of(32 * half + c) * stride;
-		if constexpr (k16<ST>) return (float)*reinterpret_cast<const short*>(row + 2 * lane + 128 * u);
-		else return *reinterpret_cast<const float*>(row + 4 * lane + 256 * u);
+		const char* at = str + row_of(32 * half + c) * stride + (int)sizeof(ST) * min(lane + 64 * u, W - 1);
+		if constexpr (k16<ST>) return (float)*reinterpret_cast<const short*>(at);
+		else return *reinterpret_cast<const float*>(at);
 	};
-	const int cols = stride / (k16<ST> ? 2 : 4);
-	bool in[WL];
-#pragma unroll
-	for (int u = 0; u < WL; u++) in[u] = lane + 64 * u < cols;
 	f4 g[8];
 	float s[WL];
 #pragma unroll
 	for (int r = 0; r < 8; r++) g[r] = *reinterpret_cast<const f4*>(sc + 4 * r);
 #pragma unroll
-	for (int u = 0; u < WL; u++) s[u] = in[u] ? value(0, u) : 0.f;
+	for (int u = 0; u < WL; u++) s[u] = value(0, u);
 #pragma unroll 2
 	for (int c = 0; c < 32; c++) {
 		const int d = min(c + 1, 31);
 		f4 gn[8];
 		float sn[WL];
 #pragma unroll
-		for (int u = 0; u < WL; u++) sn[u] = in[u] ? value(d, u) : 0.f;
+		for (int u = 0; u < WL; u++) sn[u] = value(d, u);
 #pragma unroll
 		for (int r = 0; r < 8; r++) gn[r] = *reinterpret_cast<const f4*>(sc + d * kPad + 4 * r);
 		__builtin_amdgcn_sched_barrier(0);
@@ -997,6 +1011,7 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 			for (int t = 0; t < n; t++) {
 				if (!cls[t]) continue;
 				const int kind = cls[t], s0 = (t0 + step * t) * kTile;
+				const int tid = here(threadIdx.x), lane = tid & 63, i = lane & 7, j = lane >> 3, l16 = lane & 15, g = lane >> 4;
 				__syncthreads();
 				if constexpr (!k16<ST>) {
 					stage32(str, str_x, s0, kTile, K.str_rows, str_pitch, 0, A.W, Y.so, str_vec, tid, threads);
@@ -1025,19 +1040,30 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 				if (!mykind) continue;
 #pragma unroll
 				for (int half = 0; half < 2; half++) {
-					float p[4][4], pf[4][4];  // weights, and times the score's derivative
+					const int lane = here(tid & 63), i = lane & 7, j = lane >> 3, l16 = lane & 15, g = lane >> 4;
+					float p[4][4], pf[4][4];  // weights, and the derivative of their argument by the distance's sum
 #pragma unroll
 					for (int bb = 0; bb < 4; bb++) {
-						const int b = 4 * half + bb, r = j + 8 * b, sp = K.str_place0 + s0 + r, sd = docs[r];
-						const float sl = OWNK ? slse[r] : 0.f;
+						const int b = 4 * half + bb, r = j + 8 * b;
+						const float s = (float)(K.str_place0 + s0 + r - my_lo - i), sl = OWNK ? slse[r] : 0.f;
 #pragma unroll
 						for (int a = 0; a < 4; a++) {
-							const int place = my_lo + i + 8 * a;
 							float fac;
-							float w = weight<ST>(score<ST, CAP>(x[a][b], A.cap, A.icap, fac) - slope * (float)abs(place - sp) - (OWNK ? sl : olse[a]));
-							if (mykind == 2 && !(s0 + r < K.str_rows && (OWNK ? sees(A, prefix, doc, sp, place, sd, od4[a]) : sees(A, prefix, doc, place, sp, od4[a], sd)))) w = 0.f;
-							p[a][bb] = w;
-							pf[a][bb] = w * (CAP ? fac * A.rw : A.rw);
+							const float c = score<ST, CAP>(x[a][b], A.cap, A.icap, fac);
+							p[a][bb] = weight<ST>(__builtin_fmaf(-slope, __builtin_fabsf(s - 8.f * a), c) - (OWNK ? sl : olse[a]));
+							pf[a][bb] = CAP ? fac * A.rw : A.rw;
+						}
+					}
+					if (mykind == 2) {
+#pragma unroll
+						for (int bb = 0; bb < 4; bb++) {
+							const int r = j + 8 * (4 * half + bb), sp = K.str_place0 + s0 + r, sd = docs[r];
+#pragma unroll
+							for (int a = 0; a < 4; a++) {
+								const int place = my_lo + i + 8 * a;
+								const bool ok = OWNK ? sees(!A.causal, prefix, !doc, sp, place, sd, od4[a]) : sees(!A.causal, prefix, !doc, place, sp, od4[a], sd);
+								p[a][bb] = (s0 + r < K.str_rows) & ok ? p[a][bb] : 0.f;
+							}
 						}
 					}
 					if constexpr (OWNK) weigh<ST, NY>(dyv, scr, y, yt, Y.sy, A.Wv, p, half, i, j, l16, g, bad);
@@ -1082,7 +1108,7 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 #pragma unroll
 						for (int a = 0; a < 4; a++) {
 							// a hidden pair's dp may come from values that are not finite
-							gr[a] = p[a][bb] != 0.f ? pf[a][bb] * ((OWNK ? dD : oD[a]) - d4[a][bb]) : 0.f;
+							gr[a] = p[a][bb] != 0.f ? p[a][bb] * pf[a][bb] * ((OWNK ? dD : oD[a]) - d4[a][bb]) : 0.f;
 							gsum[a] += gr[a];
 						}
 						*reinterpret_cast<f4*>(sc + (4 * j + bb) * kPad + 4 * i) = gr;
@@ -1094,12 +1120,12 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 #pragma unroll
 						for (int r = 0; r < 32; r++) {
 							const int row = (r >> 2) + 8 * (r & 3);
-							const bool in = lane + 64 * u < (k16<ST> ? Y.sr / 2 : Y.so / 4);
-							if constexpr (k16<ST>) ov[u][r] = in ? (float)*reinterpret_cast<const short*>(lds + Y.oraw + (wave * kOwn + row) * Y.sr + 2 * lane + 128 * u) + 0.5f : 0.f;
-							else ov[u][r] = in ? *reinterpret_cast<const float*>(own + row * Y.so + 4 * lane + 256 * u) : 0.f;
+							const int w = min(lane + 64 * u, A.W - 1);  // columns behind the width are worked on and not written
+							if constexpr (k16<ST>) ov[u][r] = (float)*reinterpret_cast<const short*>(lds + Y.oraw + (wave * kOwn + row) * Y.sr + 2 * w) + 0.5f;
+							else ov[u][r] = *reinterpret_cast<const float*>(own + row * Y.so + 4 * w);
 						}
 					if constexpr (k16<ST>) {
-						signs<ST, WL>(sum, ov, sc, raw, Y.sr, half, lane);
+						signs<ST, WL>(sum, ov, sc, raw, Y.sr, half, lane, A.W);
 					} else {
 						// half a tile's sum on its own, then to the total: the roundings of either are fewer
 						float part[WL][32];
@@ -1107,7 +1133,7 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 						for (int u = 0; u < WL; u++)
 #pragma unroll
 							for (int r = 0; r < 32; r++) part[u][r] = 0.f;
-						signs<ST, WL>(part, ov, sc, str, Y.so, half, lane);
+						signs<ST, WL>(part, ov, sc, str, Y.so, half, lane, A.W);
 #pragma unroll
 						for (int u = 0; u < WL; u++)
 #pragma unroll
