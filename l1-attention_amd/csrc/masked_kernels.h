@@ -163,9 +163,27 @@ __device__ __forceinline__ float wave_maxf(float x)
 
 // float32 rows, columns [0, 4 * chunks): acc[a][b] += L1 distance of owner i + 8a and stream row j + 8b.  Four terms are summed
 // as a tree before they join the sum: a quarter of the roundings there.
+template <bool AHEAD>
 __device__ __forceinline__ void distances32(const char* own, const char* str, int chunks, int stride, int i, int j, float (&acc)[4][8])
 {
 	const char *po = own + i * stride, *ps = str + j * stride;
+	if constexpr (!AHEAD) {
+		for (int c = 0; c < chunks; c++, po += 16, ps += 16) {
+			f4 o[4];
+#pragma unroll
+			for (int a = 0; a < 4; a++) o[a] = *reinterpret_cast<const f4*>(po + 8 * a * stride);
+#pragma unroll
+			for (int b = 0; b < 8; b++) {
+				const f4 s = *reinterpret_cast<const f4*>(ps + 8 * b * stride);
+#pragma unroll
+				for (int a = 0; a < 4; a++) {
+					const float d0 = o[a][0] - s[0], d1 = o[a][1] - s[1], d2 = o[a][2] - s[2], d3 = o[a][3] - s[3];
+					acc[a][b] += (__builtin_fabsf(d0) + __builtin_fabsf(d1)) + (__builtin_fabsf(d2) + __builtin_fabsf(d3));
+				}
+			}
+		}
+		return;
+	}
 	f4 o[4], s[8];
 #pragma unroll
 	for (int a = 0; a < 4; a++) o[a] = *reinterpret_cast<const f4*>(po + 8 * a * stride);
@@ -195,10 +213,33 @@ __device__ __forceinline__ void distances32(const char* own, const char* str, in
 	}
 }
 
-// rows of 16-bit codes, eight to a chunk
+// Rows of 16-bit codes, eight to a chunk.  AHEAD: reads one step ahead, 48 registers more (2.5 instead of 2.75 cycles per 64
+// pair-elements; the backward, where distances are a seventh of the work, needs the registers elsewhere).
+template <bool AHEAD>
 __device__ __forceinline__ void distances16(const char* own, const char* str, int chunks, int stride, int i, int j, unsigned (&acc)[4][8])
 {
 	const char *po = own + i * stride, *ps = str + j * stride;
+	if constexpr (!AHEAD) {
+		for (int c = 0; c < chunks; c++, po += 16, ps += 16) {
+			uint4 o[4];
+#pragma unroll
+			for (int a = 0; a < 4; a++) o[a] = *reinterpret_cast<const uint4*>(po + 8 * a * stride);
+#pragma unroll
+			for (int b = 0; b < 8; b++) {
+				const uint4 s = *reinterpret_cast<const uint4*>(ps + 8 * b * stride);
+#pragma unroll
+				for (int a = 0; a < 4; a++) {
+					unsigned t = acc[a][b];
+					t = __builtin_amdgcn_sad_u16(o[a].x, s.x, t);
+					t = __builtin_amdgcn_sad_u16(o[a].y, s.y, t);
+					t = __builtin_amdgcn_sad_u16(o[a].z, s.z, t);
+					t = __builtin_amdgcn_sad_u16(o[a].w, s.w, t);
+					acc[a][b] = t;
+				}
+			}
+		}
+		return;
+	}
 	uint4 o[4], s[8];
 #pragma unroll
 	for (int a = 0; a < 4; a++) o[a] = *reinterpret_cast<const uint4*>(po + 8 * a * stride);
@@ -263,106 +304,189 @@ __device__ __forceinline__ void stage32(char* dst, const ST* __restrict__ x, int
 // the grid of a workgroup's codes
 struct Grid { float lo, hi, sc, inv; };
 
-// Rows as codes.  OVER: each row's distance from the range into over[]; a wave of eight rows a step, eight lanes a row.
-// RAW: also the values' ordered integers.
-template <typename ST, bool OVER, bool RAW>
-__device__ __forceinline__ void stage16(char* dst, char* raw, float* over, const ST* __restrict__ x, int r0, int n, int L, int64_t pitch, int W,
-                                        int stride, int rstride, const Grid& G, bool vec, int tid, int threads)
+// eight values as codes, the first n of them; over: plus what lies outside of the range
+template <typename ST>
+__device__ __forceinline__ uint4 codes_of(const uint4& bits, int n, const Grid& G, float& over)
 {
-	const int chunks = (W + 7) >> 3, j = tid & 7;
-	for (int r = tid >> 3; r < n; r += threads >> 3) {
-		const bool in = r0 + r < L;
-		const ST* row = x + (int64_t)(r0 + r) * pitch;
-		float out = 0.f;
-		for (int c = j; c < chunks; c += 8) {
-			uint4 bits = make_uint4(0, 0, 0, 0);
-			if (in) bits = load_raw(row + 8 * c, W - 8 * c, vec);
-			float v[8];
-			unsigned short code[8];
-			unpack<ST>(bits, v);
+	float v[8];
+	unsigned code[8];
+	unpack<ST>(bits, v);
 #pragma unroll
-			for (int e = 0; e < 8; e++) {
-				const float y = __builtin_amdgcn_fmed3f(v[e], G.lo, G.hi);
-				if (OVER && 8 * c + e < W) out += __builtin_fabsf(v[e] - y);
-				code[e] = 8 * c + e < W ? (unsigned short)(unsigned)__builtin_fmaf(y - G.lo, G.sc, 0.5f) : (unsigned short)0;
-			}
-			uint4 packed;
-			__builtin_memcpy(&packed, code, 16);
-			*reinterpret_cast<uint4*>(dst + r * stride + 16 * c) = packed;
-			if (RAW) {
-				unsigned short b[8];
-				short s[8];
-				__builtin_memcpy(b, &bits, 16);
-#pragma unroll
-				for (int e = 0; e < 8; e++) s[e] = (short)ordered(b[e]);
-				__builtin_memcpy(&packed, s, 16);
-				*reinterpret_cast<uint4*>(raw + r * rstride + 16 * c) = packed;
-			}
-		}
-		if (OVER) {
-			out += __shfl_xor(out, 1);
-			out += __shfl_xor(out, 2);
-			out += __shfl_xor(out, 4);
-			if (j == 0) over[r] = out;
-		}
+	for (int e = 0; e < 8; e++) {
+		const float y = __builtin_amdgcn_fmed3f(v[e], G.lo, G.hi);
+		over += e < n ? __builtin_fabsf(v[e] - y) : 0.f;
+		code[e] = e < n ? (unsigned)__builtin_fmaf(y - G.lo, G.sc, 0.5f) : 0u;
 	}
+	return make_uint4(code[0] | code[1] << 16, code[2] | code[3] << 16, code[4] | code[5] << 16, code[6] | code[7] << 16);
 }
 
-// A tile's values: rows in product order (dst, unless NULL) and transposed (dt, unless NULL).  Columns behind the width are
-// zero.  Whether a value was not finite.
-template <typename ST>
-__device__ __forceinline__ bool stage_values(char* dst, char* dt, const ST* __restrict__ x, int r0, int L, int64_t pitch, int Wv, int stride,
-                                             bool vec, int tid, int threads)
+__device__ __forceinline__ uint4 ordered8(const uint4& bits)
 {
-	bool bad = false;
-	if constexpr (!k16<ST>) {
-		const int chunks = stride >> 4, j = tid & 7;
-		for (int r = tid >> 3; r < kTile; r += threads >> 3) {
-			const ST* row = x + (int64_t)(r0 + r) * pitch;
-			for (int c = j; c < chunks; c += 8) {
-				f4 y = {0.f, 0.f, 0.f, 0.f};
-				if (r0 + r < L) {
-					const uint4 bits = load_raw(row + 4 * c, Wv - 4 * c, vec);
-					__builtin_memcpy(&y, &bits, 16);
-				}
-				*reinterpret_cast<f4*>(dst + col_of(r) * stride + 16 * c) = y;
+	unsigned short b[8];
+	short s[8];
+	__builtin_memcpy(b, &bits, 16);
 #pragma unroll
-				for (int e = 0; e < 4; e++) bad |= !(__builtin_fabsf(y[e]) <= kMax);
+	for (int e = 0; e < 8; e++) s[e] = (short)ordered(b[e]);
+	uint4 r;
+	__builtin_memcpy(&r, s, 16);
+	return r;
+}
+
+// The owner rows of a wave as codes, and (raw, unless NULL) as ordered integers.
+template <typename ST>
+__device__ __forceinline__ void stage_own16(char* dst, char* raw, const ST* __restrict__ x, int r0, int L, int64_t pitch, int W, int stride, int rstride,
+                                            const Grid& G, bool vec, int lane)
+{
+	const int chunks = (W + 7) >> 3;
+	for (int r = lane >> 3; r < kOwn; r += 8)
+		for (int c = lane & 7; c < chunks; c += 8) {
+			uint4 bits = make_uint4(0, 0, 0, 0);
+			if (r0 + r < L) bits = load_raw(x + (int64_t)(r0 + r) * pitch + 8 * c, W - 8 * c, vec);
+			float over = 0.f;
+			*reinterpret_cast<uint4*>(dst + r * stride + 16 * c) = codes_of<ST>(bits, W - 8 * c, G, over);
+			if (raw) *reinterpret_cast<uint4*>(raw + r * rstride + 16 * c) = ordered8(bits);
+		}
+}
+
+// A tile of the stream on its way from memory to LDS.  fetch() issues the loads, one tile ahead of their use: they are under way
+// while the tile before is worked on; place() converts and stores.  What a thread has of a tile beyond KN (rows) and VN
+// (values) 16-byte pieces is loaded in place().
+template <typename ST, int KN, int VN>
+struct Stream {
+	uint4 k[KN], va[VN], vb[VN];
+	int d;
+	float l, dd;
+
+	static __device__ __forceinline__ uint4 piece(const ST* __restrict__ x, int r, int L, int64_t pitch, int w, int width, bool vec)
+	{
+		if (r < L && w < width) return load_raw(x + (int64_t)r * pitch + w, width - w, vec);
+		return make_uint4(0, 0, 0, 0);
+	}
+
+	__device__ __forceinline__ void fetch(const ST* __restrict__ x, int64_t xpitch, int W, bool xvec, const ST* __restrict__ y, int64_t ypitch, int Wv,
+	                                      bool yvec, int s0, int L, const int* doc, const float* lse, const float* D, int rpitch, int tid, int threads)
+	{
+		constexpr int per = 16 / (int)sizeof(ST);
+		const int ncg = ((W + per - 1) / per + 7) >> 3, steps = 512 / threads;
+#pragma unroll
+		for (int u = 0; u < KN; u++) {
+			const int ur = u / ncg, r = (tid >> 3) + ur * (threads >> 3), c = (tid & 7) + 8 * (u - ur * ncg);
+			k[u] = ur < steps ? piece(x, s0 + r, L, xpitch, per * c, W, xvec) : make_uint4(0, 0, 0, 0);
+		}
+		if constexpr (k16<ST>) {
+#pragma unroll
+			for (int u = 0; u < VN; u++) {
+				const int x2 = tid + threads * u, c2 = x2 & 31, ch = x2 >> 5;
+				va[u] = piece(y, s0 + row_of(2 * c2), L, ypitch, 8 * ch, Wv, yvec);
+				vb[u] = piece(y, s0 + row_of(2 * c2 + 1), L, ypitch, 8 * ch, Wv, yvec);
+			}
+		} else {
+			const int nvg = ((Wv + 3) / 4 + 7) >> 3;
+#pragma unroll
+			for (int u = 0; u < VN; u++) {
+				const int ur = u / nvg, r = (tid >> 3) + ur * (threads >> 3), c = (tid & 7) + 8 * (u - ur * nvg);
+				va[u] = ur < steps ? piece(y, s0 + r, L, ypitch, 4 * c, Wv, yvec) : make_uint4(0, 0, 0, 0);
 			}
 		}
-	} else {
-		// two rows next to each other in the order of the products, eight columns: transposed they are eight pairs
-		const int chunks = (Wv + 7) >> 3, all = dst ? (Wv + 31) / 32 * 4 : (Wv + 15) / 16 * 2;
-		(void)chunks;
-		for (int x2 = tid; x2 < 32 * all; x2 += threads) {
-			const int c2 = x2 & 31, ch = x2 >> 5;
-			const int ra = row_of(2 * c2), rb = row_of(2 * c2 + 1);
-			uint4 A = make_uint4(0, 0, 0, 0), B = A;
-			if (r0 + ra < L && 8 * ch < Wv) A = load_raw(x + (int64_t)(r0 + ra) * pitch + 8 * ch, Wv - 8 * ch, vec);
-			if (r0 + rb < L && 8 * ch < Wv) B = load_raw(x + (int64_t)(r0 + rb) * pitch + 8 * ch, Wv - 8 * ch, vec);
-			if (dst) {
-				*reinterpret_cast<uint4*>(dst + 2 * c2 * stride + 16 * ch) = A;
-				*reinterpret_cast<uint4*>(dst + (2 * c2 + 1) * stride + 16 * ch) = B;
-			}
-			float f[8];
-			unpack<ST>(A, f);
-#pragma unroll
-			for (int e = 0; e < 8; e++) bad |= !(__builtin_fabsf(f[e]) <= kMax);
-			unpack<ST>(B, f);
-#pragma unroll
-			for (int e = 0; e < 8; e++) bad |= !(__builtin_fabsf(f[e]) <= kMax);
-			if (dt && 8 * ch < (Wv + 15) / 16 * 16) {
-				const unsigned a[4] = {A.x, A.y, A.z, A.w}, b[4] = {B.x, B.y, B.z, B.w};
-#pragma unroll
-				for (int e = 0; e < 4; e++) {
-					*reinterpret_cast<unsigned*>(dt + (8 * ch + 2 * e) * kPitch * 2 + 4 * c2) = (a[e] & 0xffffu) | (b[e] << 16);
-					*reinterpret_cast<unsigned*>(dt + (8 * ch + 2 * e + 1) * kPitch * 2 + 4 * c2) = (a[e] >> 16) | (b[e] & 0xffff0000u);
-				}
+		if (tid < kTile) {
+			const bool in = s0 + tid < L;
+			d = doc && in ? doc[s0 + tid] : -1;
+			if (lse) {
+				l = in ? lse[(int64_t)(s0 + tid) * rpitch] : 0.f;
+				dd = in ? D[(int64_t)(s0 + tid) * rpitch] : 0.f;
 			}
 		}
 	}
-	return bad;
-}
+
+	// str: distance rows; raw, over, y, yt, slse, sD: see Layout, NULL where not wanted.  Whether a value was not finite.
+	__device__ __forceinline__ bool place(char* str, char* raw, float* over, char* ydst, char* yt, int* docs, float* slse, float* sD, const Layout& Y,
+	                                      const Grid& G, const ST* __restrict__ x, int64_t xpitch, int W, bool xvec, const ST* __restrict__ y,
+	                                      int64_t ypitch, int Wv, bool yvec, int s0, int L, int tid, int threads)
+	{
+		constexpr int per = 16 / (int)sizeof(ST);
+		const int chunks = (W + per - 1) / per, ncg = (chunks + 7) >> 3, steps = 512 / threads, j = tid & 7;
+		bool bad = false;
+		float out = 0.f;
+		const auto rows = [&](const uint4& bits, int r, int cg) {
+			const int c = j + 8 * cg;
+			if constexpr (!k16<ST>) {
+				if (c < chunks) *reinterpret_cast<uint4*>(str + r * Y.so + 16 * c) = bits;
+			} else {
+				if (cg == 0) out = 0.f;
+				if (c < chunks) {
+					*reinterpret_cast<uint4*>(str + r * Y.so + 16 * c) = codes_of<ST>(bits, W - 8 * c, G, out);
+					if (raw) *reinterpret_cast<uint4*>(raw + r * Y.sr + 16 * c) = ordered8(bits);
+				}
+				if (cg == ncg - 1) {
+					float o = out;
+					o += __shfl_xor(o, 1);
+					o += __shfl_xor(o, 2);
+					o += __shfl_xor(o, 4);
+					if (j == 0) over[r] = o;
+				}
+			}
+		};
+#pragma unroll
+		for (int u = 0; u < KN; u++)
+			if (u < steps * ncg) rows(k[u], (tid >> 3) + (u / ncg) * (threads >> 3), u % ncg);
+		for (int u = KN; u < steps * ncg; u++) {
+			const int r = (tid >> 3) + (u / ncg) * (threads >> 3), cg = u % ncg;
+			rows(piece(x, s0 + r, L, xpitch, per * (j + 8 * cg), W, xvec), r, cg);
+		}
+		if constexpr (!k16<ST>) {
+			const int vchunks = Y.sy >> 4, nvg = ((Wv + 3) / 4 + 7) >> 3;
+			const auto values = [&](const uint4& bits, int r, int cg) {
+				const int c = j + 8 * cg;
+				if (c < vchunks) *reinterpret_cast<uint4*>(ydst + col_of(r) * Y.sy + 16 * c) = bits;
+				const f4 v = __builtin_bit_cast(f4, bits);
+#pragma unroll
+				for (int e = 0; e < 4; e++) bad |= !(__builtin_fabsf(v[e]) <= kMax);
+			};
+#pragma unroll
+			for (int u = 0; u < VN; u++)
+				if (u < steps * nvg) values(va[u], (tid >> 3) + (u / nvg) * (threads >> 3), u % nvg);
+			for (int u = VN; u < steps * nvg; u++) {
+				const int r = (tid >> 3) + (u / nvg) * (threads >> 3), cg = u % nvg;
+				values(piece(y, s0 + r, L, ypitch, 4 * (j + 8 * cg), Wv, yvec), r, cg);
+			}
+		} else {
+			// two rows next to each other in the order of the products, eight columns: transposed they are eight pairs
+			const int all = 32 * (ydst ? (Wv + 31) / 32 * 4 : (Wv + 15) / 16 * 2), tcols = (Wv + 15) / 16 * 16;
+			const auto pair = [&](const uint4& A, const uint4& B, int x2) {
+				const int c2 = x2 & 31, ch = x2 >> 5;
+				if (ydst) {
+					*reinterpret_cast<uint4*>(ydst + 2 * c2 * Y.sy + 16 * ch) = A;
+					*reinterpret_cast<uint4*>(ydst + (2 * c2 + 1) * Y.sy + 16 * ch) = B;
+				}
+				if (yt) {
+					const unsigned a[4] = {A.x, A.y, A.z, A.w}, b[4] = {B.x, B.y, B.z, B.w};
+					// not finite: all bits of the exponent
+					constexpr unsigned em = __is_same(ST, _Float16) ? 0x7c00u : 0x7f80u;
+#pragma unroll
+					for (int e = 0; e < 4; e++) {
+						bad |= (a[e] & em) == em || (a[e] >> 16 & em) == em || (b[e] & em) == em || (b[e] >> 16 & em) == em;
+						if (8 * ch < tcols) {
+							*reinterpret_cast<unsigned*>(yt + (8 * ch + 2 * e) * kPitch * 2 + 4 * c2) = (a[e] & 0xffffu) | (b[e] << 16);
+							*reinterpret_cast<unsigned*>(yt + (8 * ch + 2 * e + 1) * kPitch * 2 + 4 * c2) = (a[e] >> 16) | (b[e] & 0xffff0000u);
+						}
+					}
+				}
+			};
+#pragma unroll
+			for (int u = 0; u < VN; u++)
+				if (tid + threads * u < all) pair(va[u], vb[u], tid + threads * u);
+			for (int x2 = tid + threads * VN; x2 < all; x2 += threads) {
+				const int c2 = x2 & 31, ch = x2 >> 5;
+				pair(piece(y, s0 + row_of(2 * c2), L, ypitch, 8 * ch, Wv, yvec), piece(y, s0 + row_of(2 * c2 + 1), L, ypitch, 8 * ch, Wv, yvec), x2);
+			}
+		}
+		if (tid < kTile) {
+			docs[tid] = d;
+			if (slse) { slse[tid] = l; sD[tid] = dd; }
+		}
+		return bad;
+	}
+};
 
 // ---------------------------------------------------------------------------------------------------------------- products
 
@@ -493,6 +617,12 @@ __device__ __forceinline__ void classify(const L1MaskedArgs& A, const Block& K, 
 	}
 }
 
+__device__ __forceinline__ int next_tile(const unsigned char* cls, int t, int n)
+{
+	while (t < n && !cls[t]) t++;
+	return t;
+}
+
 // no short cuts: a branch for every pair would cost more than the comparisons
 __device__ __forceinline__ bool sees(bool open, int prefix, bool nodocs, int qp, int kp, int qd, int kd)
 {
@@ -556,7 +686,7 @@ __device__ __forceinline__ bool owner_grid(const ST* __restrict__ x, const int* 
 
 // A wave's distances of one tile, acc[a][b] >= 0 scaled by 1/sqrt(W), NaN where a value is.  Called by all waves of the
 // workgroup; `active`: this wave needs them.  Without a grid 16-bit rows go through LDS as float32, half of the columns at a time.
-template <typename ST>
+template <typename ST, bool AHEAD>
 __device__ __forceinline__ void tile_distances(char* own, char* str, const float* over, const Layout& Y, int W, float rw, const Grid& G, bool coded,
                                                bool active, const ST* __restrict__ own_x, int own_r0, int own_rows, int64_t own_pitch,
                                                const ST* __restrict__ str_x, int s0, int str_rows, int64_t str_pitch, int i, int j, int tid, int threads,
@@ -567,7 +697,7 @@ __device__ __forceinline__ void tile_distances(char* own, char* str, const float
 		for (int a = 0; a < 4; a++)
 #pragma unroll
 			for (int b = 0; b < 8; b++) x[a][b] = 0.f;
-		if (active) distances32(own, str, (W + 3) >> 2, Y.so, i, j, x);
+		if (active) distances32<AHEAD>(own, str, (W + 3) >> 2, Y.so, i, j, x);
 #pragma unroll
 		for (int a = 0; a < 4; a++)
 #pragma unroll
@@ -579,7 +709,7 @@ __device__ __forceinline__ void tile_distances(char* own, char* str, const float
 		for (int a = 0; a < 4; a++)
 #pragma unroll
 			for (int b = 0; b < 8; b++) acc[a][b] = 0;
-		distances16(own, str, (W + 7) >> 3, Y.so, i, j, acc);
+		distances16<AHEAD>(own, str, (W + 7) >> 3, Y.so, i, j, acc);
 		const float m = G.inv * rw;
 #pragma unroll
 		for (int b = 0; b < 8; b++) {
@@ -599,7 +729,7 @@ __device__ __forceinline__ void tile_distances(char* own, char* str, const float
 			stage32(own, own_x, own_r0, kOwn, own_rows, own_pitch, w0, n, Y.so, false, tid & 63, 64);
 			stage32(str, str_x, s0, kTile, str_rows, str_pitch, w0, n, Y.so, false, tid, threads);
 			__syncthreads();
-			if (active) distances32(own, str, (n + 3) >> 2, Y.so, i, j, x);
+			if (active) distances32<false>(own, str, (n + 3) >> 2, Y.so, i, j, x);
 		}
 #pragma unroll
 		for (int a = 0; a < 4; a++)
@@ -645,6 +775,7 @@ template <typename ST, bool CAP, int NB, int THREADS>
 __global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* __restrict__ q, const ST* __restrict__ k,
                                                       const ST* __restrict__ v, ST* __restrict__ o, float* __restrict__ lse, float* __restrict__ part)
 {
+	constexpr int KN = k16<ST> && NB == 8 ? 4 : 2, VN = k16<ST> && NB < 8 ? 1 : 2;
 	extern __shared__ __align__(16) char lds[];
 	const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 63, wave = tid >> 6, waves = threads >> 6;
 	const int i = lane & 7, j = lane >> 3, l16 = lane & 15, g = lane >> 4;
@@ -674,7 +805,7 @@ __global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* 
 	bool coded = false;
 	if constexpr (k16<ST>) {
 		coded = owner_grid(qh, doc, K, row0, qpitch, A.W, A.vec & 1, red + 32, lane, wave, waves, G);
-		if (coded) stage16<ST, false, false>(own, nullptr, nullptr, qh, row0, kOwn, A.T, qpitch, A.W, Y.so, 0, G, A.vec & 1, lane, 64);
+		if (coded) stage_own16(own, (char*)nullptr, qh, row0, A.T, qpitch, A.W, Y.so, 0, G, A.vec & 1, lane);
 	} else {
 		stage32(own, qh, row0, kOwn, A.T, qpitch, 0, A.W, Y.so, A.vec & 1, lane, 64);
 	}
@@ -696,15 +827,17 @@ __global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* 
 		__syncthreads();
 		classify<false>(A, K, doc, prefix, own_lo, own_hi, all, all_whole, t0, step, n, cls, tid, threads);
 		__syncthreads();
-		for (int t = 0; t < n; t++) {
-			if (!cls[t]) continue;
-			const int kind = cls[t], s0 = (t0 + step * t) * kTile;
+		Stream<ST, KN, VN> F;
+		int next = next_tile(cls, 0, n);
+		if (next < n) F.fetch(kh, kpitch, A.W, A.vec & 2, vh, vpitch, A.Wv, A.vec & 4, (t0 + step * next) * kTile, A.S, doc, nullptr, nullptr, 0, tid, threads);
+		while (next < n) {
+			const int kind = cls[next], s0 = (t0 + step * next) * kTile;
 			const int tid = here(threadIdx.x), lane = tid & 63, i = lane & 7, j = lane >> 3, l16 = lane & 15, g = lane >> 4;
 			__syncthreads();
-			if constexpr (!k16<ST>) stage32(str, kh, s0, kTile, A.S, kpitch, 0, A.W, Y.so, A.vec & 2, tid, threads);
-			else if (coded) stage16<ST, true, false>(str, nullptr, over, kh, s0, kTile, A.S, kpitch, A.W, Y.so, 0, G, A.vec & 2, tid, threads);
-			bool bad = stage_values<ST>(k16<ST> ? nullptr : y, yt, vh, s0, A.S, vpitch, A.Wv, Y.sy, A.vec & 4, tid, threads);
-			if (tid < kTile) docs[tid] = doc && s0 + tid < A.S ? doc[s0 + tid] : -1;
+			bool bad = F.place(str, nullptr, over, k16<ST> ? nullptr : y, yt, docs, nullptr, nullptr, Y, G, kh, kpitch, A.W, A.vec & 2, vh, vpitch, A.Wv,
+			                   A.vec & 4, s0, A.S, tid, threads);
+			next = next_tile(cls, next + 1, n);
+			if (next < n) F.fetch(kh, kpitch, A.W, A.vec & 2, vh, vpitch, A.Wv, A.vec & 4, (t0 + step * next) * kTile, A.S, doc, nullptr, nullptr, 0, tid, threads);
 			bad = __syncthreads_or(bad && kind == 2);
 			// what the tile is to this wave's own rows
 			int mykind = row0 < A.T ? kind : 0;
@@ -713,7 +846,7 @@ __global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* 
 				if (mykind && doc) mykind = doc_class(mykind, docs[lane], mine, mine_whole);
 			}
 			float x[4][8];
-			tile_distances<ST>(own, str, over, Y, A.W, A.rw, G, coded, mykind, qh, row0, A.T, qpitch, kh, s0, A.S, kpitch, i, j, tid, threads, x);
+			tile_distances<ST, true>(own, str, over, Y, A.W, A.rw, G, coded, mykind, qh, row0, A.T, qpitch, kh, s0, A.S, kpitch, i, j, tid, threads, x);
 			if (!mykind) continue;
 			// float32: a tile's sum on its own, then to the total: the roundings of either are fewer
 			f4 tile[2][NB];
@@ -865,33 +998,37 @@ __device__ __forceinline__ void signs(float (&sum)[WL][32], const float (&ov)[WL
 		if constexpr (k16<ST>) return (float)*reinterpret_cast<const short*>(at);
 		else return *reinterpret_cast<const float*>(at);
 	};
-	f4 g[8];
+	f4 g[4], gn[4];  // the gradients of 16 owners, and of the next 16
 	float s[WL];
 #pragma unroll
-	for (int r = 0; r < 8; r++) g[r] = *reinterpret_cast<const f4*>(sc + 4 * r);
+	for (int r = 0; r < 4; r++) g[r] = *reinterpret_cast<const f4*>(sc + 4 * r);
 #pragma unroll
 	for (int u = 0; u < WL; u++) s[u] = value(0, u);
-#pragma unroll 2
-	for (int c = 0; c < 32; c++) {
-		const int d = min(c + 1, 31);
-		f4 gn[8];
-		float sn[WL];
+	const auto add = [&](const f4(&x)[4], int r0) {
 #pragma unroll
-		for (int u = 0; u < WL; u++) sn[u] = value(d, u);
-#pragma unroll
-		for (int r = 0; r < 8; r++) gn[r] = *reinterpret_cast<const f4*>(sc + d * kPad + 4 * r);
-		__builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-		for (int r = 0; r < 32; r++)
+		for (int r = 0; r < 16; r++)
 #pragma unroll
 			for (int u = 0; u < WL; u++) {
-				const float df = ov[u][r] - s[u];
+				const float df = ov[u][r0 + r] - s[u];
 				const float hv = __builtin_amdgcn_fmed3f(k16<ST> ? df : __builtin_fmaf(df, 0x1p127f, 0.5f), 0.f, 1.f);
-				sum[u][r] = __builtin_fmaf(hv, g[r >> 2][r & 3], sum[u][r]);
+				sum[u][r0 + r] = __builtin_fmaf(hv, x[r >> 2][r & 3], sum[u][r0 + r]);
 			}
+	};
+	for (int c = 0; c < 32; c++) {
+		const int d = min(c + 1, 31);
+		float sn[WL];
+#pragma unroll
+		for (int r = 0; r < 4; r++) gn[r] = *reinterpret_cast<const f4*>(sc + c * kPad + 16 + 4 * r);
+#pragma unroll
+		for (int u = 0; u < WL; u++) sn[u] = value(d, u);
+		__builtin_amdgcn_sched_barrier(0);
+		add(g, 0);
 		__builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-		for (int r = 0; r < 8; r++) g[r] = gn[r];
+		for (int r = 0; r < 4; r++) g[r] = *reinterpret_cast<const f4*>(sc + d * kPad + 4 * r);
+		__builtin_amdgcn_sched_barrier(0);
+		add(gn, 16);
+		__builtin_amdgcn_sched_barrier(0);
 #pragma unroll
 		for (int u = 0; u < WL; u++) s[u] = sn[u];
 	}
@@ -909,6 +1046,7 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 	extern __shared__ __align__(16) char lds[];
 	const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 63, wave = tid >> 6, waves = threads >> 6;
 	const int i = lane & 7, j = lane >> 3, l16 = lane & 15, g = lane >> 4;
+	constexpr int KN = k16<ST> && NB == 8 ? 4 : 2, VN = k16<ST> && NB < 8 ? 1 : 2;
 	const int group = A.H / A.Hk, heads = OWNK ? A.Hk : A.H;
 	Block K;
 	K.b = blockIdx.x / heads;
@@ -946,7 +1084,7 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 	bool coded = false;
 	if constexpr (k16<ST>) {
 		coded = owner_grid(own_x, doc, K, row0, own_pitch, A.W, own_vec, red + 32, lane, wave, waves, G);
-		stage16<ST, false, true>(own, lds + Y.oraw + wave * kOwn * Y.sr, nullptr, own_x, row0, kOwn, K.own_rows, own_pitch, A.W, Y.so, Y.sr, G, own_vec, lane, 64);
+		stage_own16(own, lds + Y.oraw + wave * kOwn * Y.sr, own_x, row0, K.own_rows, own_pitch, A.W, Y.so, Y.sr, G, own_vec, lane);
 	} else {
 		stage32(own, own_x, row0, kOwn, K.own_rows, own_pitch, 0, A.W, Y.so, own_vec, lane, 64);
 	}
@@ -1008,27 +1146,23 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 			__syncthreads();
 			classify<OWNK>(A, K, doc, prefix, own_lo, own_hi, all, all_whole, t0, step, n, cls, tid, threads);
 			__syncthreads();
-			for (int t = 0; t < n; t++) {
-				if (!cls[t]) continue;
-				const int kind = cls[t], s0 = (t0 + step * t) * kTile;
+			Stream<ST, KN, VN> F;
+			const ST* str_y = OWNK ? oh : vh;
+			const int64_t y_pitch = OWNK ? opitch : vpitch;
+			const bool y_vec = A.vec & (OWNK ? 8 : 4);
+			const int* str_doc = doc ? doc + K.str_place0 : nullptr;
+			const float *lh = OWNK ? lse + (int64_t)K.b * A.T * A.H + h : nullptr, *Dh = OWNK ? D + (int64_t)K.b * A.T * A.H + h : nullptr;
+			int next = next_tile(cls, 0, n);
+			if (next < n) F.fetch(str_x, str_pitch, A.W, str_vec, str_y, y_pitch, A.Wv, y_vec, (t0 + step * next) * kTile, K.str_rows, str_doc, lh, Dh, A.H, tid, threads);
+			while (next < n) {
+				const int kind = cls[next], s0 = (t0 + step * next) * kTile;
 				const int tid = here(threadIdx.x), lane = tid & 63, i = lane & 7, j = lane >> 3, l16 = lane & 15, g = lane >> 4;
 				__syncthreads();
-				if constexpr (!k16<ST>) {
-					stage32(str, str_x, s0, kTile, K.str_rows, str_pitch, 0, A.W, Y.so, str_vec, tid, threads);
-				} else {
-					// without a grid the codes come out as nonsense that nobody reads; the ordered integers are wanted all the same
-					stage16<ST, true, true>(str, raw, over, str_x, s0, kTile, K.str_rows, str_pitch, A.W, Y.so, Y.sr, G, str_vec, tid, threads);
-				}
-				bool bad = stage_values<ST>(y, k16<ST> && OWNK ? yt : nullptr, OWNK ? oh : vh, s0, K.str_rows, OWNK ? opitch : vpitch, A.Wv, Y.sy,
-				                            OWNK ? A.vec & 8 : A.vec & 4, tid, threads);
-				if (tid < kTile) {
-					const bool in = s0 + tid < K.str_rows;
-					docs[tid] = doc && in ? doc[K.str_place0 + s0 + tid] : -1;
-					if (OWNK) {
-						slse[tid] = in ? lse[((int64_t)K.b * A.T + s0 + tid) * A.H + h] : 0.f;
-						sD[tid] = in ? D[((int64_t)K.b * A.T + s0 + tid) * A.H + h] : 0.f;
-					}
-				}
+				// without a grid the codes come out as nonsense that nobody reads; the ordered integers are wanted all the same
+				bool bad = F.place(str, raw, over, y, k16<ST> && OWNK ? yt : nullptr, docs, OWNK ? slse : nullptr, sD, Y, G, str_x, str_pitch, A.W, str_vec,
+				                   str_y, y_pitch, A.Wv, y_vec, s0, K.str_rows, tid, threads);
+				next = next_tile(cls, next + 1, n);
+				if (next < n) F.fetch(str_x, str_pitch, A.W, str_vec, str_y, y_pitch, A.Wv, y_vec, (t0 + step * next) * kTile, K.str_rows, str_doc, lh, Dh, A.H, tid, threads);
 				bad = __syncthreads_or(bad && kind == 2);
 				int mykind = row0 < K.own_rows ? kind : 0;
 				if (mykind == 2) {
@@ -1036,7 +1170,7 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 					if (mykind && doc) mykind = doc_class(mykind, docs[lane], mine, mine_whole);
 				}
 				float x[4][8];
-				tile_distances<ST>(own, str, over, Y, A.W, A.rw, G, coded, mykind, own_x, row0, K.own_rows, own_pitch, str_x, s0, K.str_rows, str_pitch, i, j, tid, threads, x);
+				tile_distances<ST, false>(own, str, over, Y, A.W, A.rw, G, coded, mykind, own_x, row0, K.own_rows, own_pitch, str_x, s0, K.str_rows, str_pitch, i, j, tid, threads, x);
 				if (!mykind) continue;
 #pragma unroll
 				for (int half = 0; half < 2; half++) {
