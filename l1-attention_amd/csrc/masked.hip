@@ -53,10 +53,10 @@ L1MaskedPlan plan_of(const L1MaskedTable& t, int64_t owners, int64_t stream, int
 {
 	L1MaskedPlan p;
 	const bool wide = W > 64 || Wv > 64;
-	p.waves = wide ? 4 : 8;
+	p.waves = wide || t.lds(64, 64, 1, false, false) < 26000 ? 4 : 8;
 	while (p.waves > 2 && (t.lds(W, Wv, p.waves, backward, weigh) > 160 * 1024 || heads * l1_cdiv(owners, 32 * p.waves) < 256)) p.waves >>= 1;
 	const int64_t groups = heads * l1_cdiv(owners, 32 * p.waves), tiles = l1_cdiv(stream, 64);
-	int64_t s = l1_cdiv(512, groups);
+	int64_t s = l1_cdiv(1024, groups);
 	if (s > tiles / 2) s = tiles / 2;
 	p.splits = (int)(s < 1 ? 1 : s > 16 ? 16 : s);
 	return p;

@@ -40,9 +40,9 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 
 constexpr int kOwn = 32;        // owner rows of a wave
-constexpr int kTile = 64;       // stream rows of a tile
 constexpr int kPad = 36;        // floats in a row of the scratch: 9 chunks of 16 bytes, odd, so rows spread over the banks
-constexpr int kPitch = 72;      // 16-bit values in a row of 64 (p in the scratch, transposed values): 9 chunks
+constexpr int kPitch(int TB) { return 8 * TB + 8; }  // 16-bit values in a row of transposed values: an odd number of chunks
+template <int TB> constexpr int kTile = 8 * TB;  // stream rows of a tile: TB for each of the eight lanes j
 constexpr int kScratch = kOwn * kPad * 4;
 constexpr int kClasses = 1024;  // tiles whose visibility is worked out at a time
 constexpr float kMax = 3.402823466e38f;
@@ -67,7 +67,7 @@ struct Layout {
 	int so, sr, sy;  // bytes of a row of own/str, oraw/raw, y
 };
 
-template <typename ST>
+template <typename ST, int TB>
 __host__ __device__ inline Layout masked_layout(int W, int Wv, int waves, bool backward, bool weigh)
 {
 	Layout l;
@@ -78,12 +78,12 @@ __host__ __device__ inline Layout masked_layout(int W, int Wv, int waves, bool b
 	l.own = 0;
 	l.oraw = l.own + waves * kOwn * l.so;
 	l.str = l.oraw + (k16<ST> && backward ? waves * kOwn * l.sr : 0);
-	l.raw = l.str + kTile * l.so;
-	l.y = l.raw + (k16<ST> && backward ? kTile * l.sr : 0);
-	l.yt = l.y + (!k16<ST> || backward ? kTile * l.sy : 0);
-	l.scratch = l.yt + (k16<ST> && weigh ? (Wv + 15) / 16 * 16 * kPitch * 2 : 0);
+	l.raw = l.str + kTile<TB> * l.so;
+	l.y = l.raw + (k16<ST> && backward ? kTile<TB> * l.sr : 0);
+	l.yt = l.y + (!k16<ST> || backward ? kTile<TB> * l.sy : 0);
+	l.scratch = l.yt + (k16<ST> && weigh ? (Wv + 15) / 16 * 16 * kPitch(TB) * 2 : 0);
 	l.rows = l.scratch + waves * kScratch;  // documents, lse, D, what lies outside of the range (64 each), 64 words for reductions, classes
-	l.total = l.rows + (4 * kTile + 64) * 4 + kClasses;
+	l.total = l.rows + (4 * kTile<TB> + 64) * 4 + kClasses;
 	return l;
 }
 
@@ -163,8 +163,8 @@ __device__ __forceinline__ float wave_maxf(float x)
 
 // float32 rows, columns [0, 4 * chunks): acc[a][b] += L1 distance of owner i + 8a and stream row j + 8b.  Four terms are summed
 // as a tree before they join the sum: a quarter of the roundings there.
-template <bool AHEAD>
-__device__ __forceinline__ void distances32(const char* own, const char* str, int chunks, int stride, int i, int j, float (&acc)[4][8])
+template <bool AHEAD, int TB>
+__device__ __forceinline__ void distances32(const char* own, const char* str, int chunks, int stride, int i, int j, float (&acc)[4][TB])
 {
 	const char *po = own + i * stride, *ps = str + j * stride;
 	if constexpr (!AHEAD) {
@@ -173,7 +173,7 @@ __device__ __forceinline__ void distances32(const char* own, const char* str, in
 #pragma unroll
 			for (int a = 0; a < 4; a++) o[a] = *reinterpret_cast<const f4*>(po + 8 * a * stride);
 #pragma unroll
-			for (int b = 0; b < 8; b++) {
+			for (int b = 0; b < TB; b++) {
 				const f4 s = *reinterpret_cast<const f4*>(ps + 8 * b * stride);
 #pragma unroll
 				for (int a = 0; a < 4; a++) {
@@ -184,39 +184,39 @@ __device__ __forceinline__ void distances32(const char* own, const char* str, in
 		}
 		return;
 	}
-	f4 o[4], s[8];
+	const auto load = [&](f4(&o)[4], f4(&s)[TB], int c) {
+		const int d = 16 * min(c, chunks - 1);
 #pragma unroll
-	for (int a = 0; a < 4; a++) o[a] = *reinterpret_cast<const f4*>(po + 8 * a * stride);
+		for (int a = 0; a < 4; a++) o[a] = *reinterpret_cast<const f4*>(po + 8 * a * stride + d);
 #pragma unroll
-	for (int b = 0; b < 8; b++) s[b] = *reinterpret_cast<const f4*>(ps + 8 * b * stride);
-#pragma unroll 2
-	for (int c = 0; c < chunks; c++) {
-		const int d = 16 * min(c + 1, chunks - 1);
-		f4 on[4], sn[8];
-#pragma unroll
-		for (int a = 0; a < 4; a++) on[a] = *reinterpret_cast<const f4*>(po + 8 * a * stride + d);
-#pragma unroll
-		for (int b = 0; b < 8; b++) sn[b] = *reinterpret_cast<const f4*>(ps + 8 * b * stride + d);
+		for (int b = 0; b < TB; b++) s[b] = *reinterpret_cast<const f4*>(ps + 8 * b * stride + d);
 		__builtin_amdgcn_sched_barrier(0);
+	};
+	const auto work = [&](const f4(&o)[4], const f4(&s)[TB]) {
 #pragma unroll
-		for (int b = 0; b < 8; b++)
+		for (int b = 0; b < TB; b++)
 #pragma unroll
 			for (int a = 0; a < 4; a++) {
 				const float d0 = o[a][0] - s[b][0], d1 = o[a][1] - s[b][1], d2 = o[a][2] - s[b][2], d3 = o[a][3] - s[b][3];
 				acc[a][b] += (__builtin_fabsf(d0) + __builtin_fabsf(d1)) + (__builtin_fabsf(d2) + __builtin_fabsf(d3));
 			}
 		__builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-		for (int a = 0; a < 4; a++) o[a] = on[a];
-#pragma unroll
-		for (int b = 0; b < 8; b++) s[b] = sn[b];
+	};
+	f4 o0[4], s0[TB], o1[4], s1[TB];
+	load(o0, s0, 0);
+	for (int c = 0; c < chunks; c += 2) {
+		load(o1, s1, c + 1);
+		work(o0, s0);
+		if (c + 1 >= chunks) break;
+		load(o0, s0, c + 2);
+		work(o1, s1);
 	}
 }
 
 // Rows of 16-bit codes, eight to a chunk.  AHEAD: reads one step ahead, 48 registers more (2.5 instead of 2.75 cycles per 64
 // pair-elements; the backward, where distances are a seventh of the work, needs the registers elsewhere).
-template <bool AHEAD>
-__device__ __forceinline__ void distances16(const char* own, const char* str, int chunks, int stride, int i, int j, unsigned (&acc)[4][8])
+template <bool AHEAD, int TB>
+__device__ __forceinline__ void distances16(const char* own, const char* str, int chunks, int stride, int i, int j, unsigned (&acc)[4][TB])
 {
 	const char *po = own + i * stride, *ps = str + j * stride;
 	if constexpr (!AHEAD) {
@@ -225,7 +225,7 @@ __device__ __forceinline__ void distances16(const char* own, const char* str, in
 #pragma unroll
 			for (int a = 0; a < 4; a++) o[a] = *reinterpret_cast<const uint4*>(po + 8 * a * stride);
 #pragma unroll
-			for (int b = 0; b < 8; b++) {
+			for (int b = 0; b < TB; b++) {
 				const uint4 s = *reinterpret_cast<const uint4*>(ps + 8 * b * stride);
 #pragma unroll
 				for (int a = 0; a < 4; a++) {
@@ -240,22 +240,17 @@ __device__ __forceinline__ void distances16(const char* own, const char* str, in
 		}
 		return;
 	}
-	uint4 o[4], s[8];
+	const auto load = [&](uint4(&o)[4], uint4(&s)[TB], int c) {
+		const int d = 16 * min(c, chunks - 1);
 #pragma unroll
-	for (int a = 0; a < 4; a++) o[a] = *reinterpret_cast<const uint4*>(po + 8 * a * stride);
+		for (int a = 0; a < 4; a++) o[a] = *reinterpret_cast<const uint4*>(po + 8 * a * stride + d);
 #pragma unroll
-	for (int b = 0; b < 8; b++) s[b] = *reinterpret_cast<const uint4*>(ps + 8 * b * stride);
-#pragma unroll 2
-	for (int c = 0; c < chunks; c++) {
-		const int d = 16 * min(c + 1, chunks - 1);
-		uint4 on[4], sn[8];
-#pragma unroll
-		for (int a = 0; a < 4; a++) on[a] = *reinterpret_cast<const uint4*>(po + 8 * a * stride + d);
-#pragma unroll
-		for (int b = 0; b < 8; b++) sn[b] = *reinterpret_cast<const uint4*>(ps + 8 * b * stride + d);
+		for (int b = 0; b < TB; b++) s[b] = *reinterpret_cast<const uint4*>(ps + 8 * b * stride + d);
 		__builtin_amdgcn_sched_barrier(0);
+	};
+	const auto work = [&](const uint4(&o)[4], const uint4(&s)[TB]) {
 #pragma unroll
-		for (int b = 0; b < 8; b++)
+		for (int b = 0; b < TB; b++)
 #pragma unroll
 			for (int a = 0; a < 4; a++) {
 				unsigned t = acc[a][b];
@@ -266,10 +261,15 @@ __device__ __forceinline__ void distances16(const char* own, const char* str, in
 				acc[a][b] = t;
 			}
 		__builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-		for (int a = 0; a < 4; a++) o[a] = on[a];
-#pragma unroll
-		for (int b = 0; b < 8; b++) s[b] = sn[b];
+	};
+	uint4 o0[4], s0[TB], o1[4], s1[TB];
+	load(o0, s0, 0);
+	for (int c = 0; c < chunks; c += 2) {
+		load(o1, s1, c + 1);
+		work(o0, s0);
+		if (c + 1 >= chunks) break;
+		load(o0, s0, c + 2);
+		work(o1, s1);
 	}
 }
 
@@ -351,7 +351,7 @@ __device__ __forceinline__ void stage_own16(char* dst, char* raw, const ST* __re
 // A tile of the stream on its way from memory to LDS.  fetch() issues the loads, one tile ahead of their use: they are under way
 // while the tile before is worked on; place() converts and stores.  What a thread has of a tile beyond KN (rows) and VN
 // (values) 16-byte pieces is loaded in place().
-template <typename ST, int KN, int VN>
+template <typename ST, int TB, int KN, int VN>
 struct Stream {
 	uint4 k[KN], va[VN], vb[VN];
 	int d;
@@ -367,16 +367,16 @@ struct Stream {
 	                                      bool yvec, int s0, int L, const int* doc, const float* lse, const float* D, int rpitch, int tid, int threads)
 	{
 		constexpr int per = 16 / (int)sizeof(ST);
-		const int ncg = ((W + per - 1) / per + 7) >> 3, steps = 512 / threads;
+		const int ncg = ((W + per - 1) / per + 7) >> 3, steps = (8 * kTile<TB> + threads - 1) / threads;
 #pragma unroll
 		for (int u = 0; u < KN; u++) {
 			const int ur = u / ncg, r = (tid >> 3) + ur * (threads >> 3), c = (tid & 7) + 8 * (u - ur * ncg);
-			k[u] = ur < steps ? piece(x, s0 + r, L, xpitch, per * c, W, xvec) : make_uint4(0, 0, 0, 0);
+			k[u] = r < kTile<TB> ? piece(x, s0 + r, L, xpitch, per * c, W, xvec) : make_uint4(0, 0, 0, 0);
 		}
 		if constexpr (k16<ST>) {
 #pragma unroll
 			for (int u = 0; u < VN; u++) {
-				const int x2 = tid + threads * u, c2 = x2 & 31, ch = x2 >> 5;
+				const int x2 = tid + threads * u, c2 = x2 % (kTile<TB> / 2), ch = x2 / (kTile<TB> / 2);
 				va[u] = piece(y, s0 + row_of(2 * c2), L, ypitch, 8 * ch, Wv, yvec);
 				vb[u] = piece(y, s0 + row_of(2 * c2 + 1), L, ypitch, 8 * ch, Wv, yvec);
 			}
@@ -385,10 +385,10 @@ struct Stream {
 #pragma unroll
 			for (int u = 0; u < VN; u++) {
 				const int ur = u / nvg, r = (tid >> 3) + ur * (threads >> 3), c = (tid & 7) + 8 * (u - ur * nvg);
-				va[u] = ur < steps ? piece(y, s0 + r, L, ypitch, 4 * c, Wv, yvec) : make_uint4(0, 0, 0, 0);
+				va[u] = r < kTile<TB> ? piece(y, s0 + r, L, ypitch, 4 * c, Wv, yvec) : make_uint4(0, 0, 0, 0);
 			}
 		}
-		if (tid < kTile) {
+		if (tid < kTile<TB>) {
 			const bool in = s0 + tid < L;
 			d = doc && in ? doc[s0 + tid] : -1;
 			if (lse) {
@@ -404,11 +404,12 @@ struct Stream {
 	                                      int64_t ypitch, int Wv, bool yvec, int s0, int L, int tid, int threads)
 	{
 		constexpr int per = 16 / (int)sizeof(ST);
-		const int chunks = (W + per - 1) / per, ncg = (chunks + 7) >> 3, steps = 512 / threads, j = tid & 7;
+		const int chunks = (W + per - 1) / per, ncg = (chunks + 7) >> 3, steps = (8 * kTile<TB> + threads - 1) / threads, j = tid & 7;
 		bool bad = false;
 		float out = 0.f;
 		const auto rows = [&](const uint4& bits, int r, int cg) {
 			const int c = j + 8 * cg;
+			if (r >= kTile<TB>) return;  // eight lanes at a time: a row's sum is still formed by all of its lanes
 			if constexpr (!k16<ST>) {
 				if (c < chunks) *reinterpret_cast<uint4*>(str + r * Y.so + 16 * c) = bits;
 			} else {
@@ -437,6 +438,7 @@ struct Stream {
 			const int vchunks = Y.sy >> 4, nvg = ((Wv + 3) / 4 + 7) >> 3;
 			const auto values = [&](const uint4& bits, int r, int cg) {
 				const int c = j + 8 * cg;
+				if (r >= kTile<TB>) return;
 				if (c < vchunks) *reinterpret_cast<uint4*>(ydst + col_of(r) * Y.sy + 16 * c) = bits;
 				const f4 v = __builtin_bit_cast(f4, bits);
 #pragma unroll
@@ -451,9 +453,9 @@ struct Stream {
 			}
 		} else {
 			// two rows next to each other in the order of the products, eight columns: transposed they are eight pairs
-			const int all = 32 * (ydst ? (Wv + 31) / 32 * 4 : (Wv + 15) / 16 * 2), tcols = (Wv + 15) / 16 * 16;
+			const int all = kTile<TB> / 2 * (ydst ? (Wv + 31) / 32 * 4 : (Wv + 15) / 16 * 2), tcols = (Wv + 15) / 16 * 16;
 			const auto pair = [&](const uint4& A, const uint4& B, int x2) {
-				const int c2 = x2 & 31, ch = x2 >> 5;
+				const int c2 = x2 % (kTile<TB> / 2), ch = x2 / (kTile<TB> / 2);
 				if (ydst) {
 					*reinterpret_cast<uint4*>(ydst + 2 * c2 * Y.sy + 16 * ch) = A;
 					*reinterpret_cast<uint4*>(ydst + (2 * c2 + 1) * Y.sy + 16 * ch) = B;
@@ -466,8 +468,8 @@ struct Stream {
 					for (int e = 0; e < 4; e++) {
 						bad |= (a[e] & em) == em || (a[e] >> 16 & em) == em || (b[e] & em) == em || (b[e] >> 16 & em) == em;
 						if (8 * ch < tcols) {
-							*reinterpret_cast<unsigned*>(yt + (8 * ch + 2 * e) * kPitch * 2 + 4 * c2) = (a[e] & 0xffffu) | (b[e] << 16);
-							*reinterpret_cast<unsigned*>(yt + (8 * ch + 2 * e + 1) * kPitch * 2 + 4 * c2) = (a[e] >> 16) | (b[e] & 0xffff0000u);
+							*reinterpret_cast<unsigned*>(yt + (8 * ch + 2 * e) * kPitch(TB) * 2 + 4 * c2) = (a[e] & 0xffffu) | (b[e] << 16);
+							*reinterpret_cast<unsigned*>(yt + (8 * ch + 2 * e + 1) * kPitch(TB) * 2 + 4 * c2) = (a[e] >> 16) | (b[e] & 0xffff0000u);
 						}
 					}
 				}
@@ -476,11 +478,11 @@ struct Stream {
 			for (int u = 0; u < VN; u++)
 				if (tid + threads * u < all) pair(va[u], vb[u], tid + threads * u);
 			for (int x2 = tid + threads * VN; x2 < all; x2 += threads) {
-				const int c2 = x2 & 31, ch = x2 >> 5;
+				const int c2 = x2 % (kTile<TB> / 2), ch = x2 / (kTile<TB> / 2);
 				pair(piece(y, s0 + row_of(2 * c2), L, ypitch, 8 * ch, Wv, yvec), piece(y, s0 + row_of(2 * c2 + 1), L, ypitch, 8 * ch, Wv, yvec), x2);
 			}
 		}
-		if (tid < kTile) {
+		if (tid < kTile<TB>) {
 			docs[tid] = d;
 			if (slse) { slse[tid] = l; sD[tid] = dd; }
 		}
@@ -503,7 +505,7 @@ __device__ __forceinline__ f4 mma16(const uint4& a, const uint4& b, f4 c)
 // product's other factor has).
 // `bad` (values that are not finite in a tile of which some is hidden): a hidden pair's weight of zero must not meet them, which
 // a matrix instruction cannot leave out.
-template <typename ST, int NB>
+template <typename ST, int NB, int TB>
 __device__ __forceinline__ void weigh(f4 (&acc)[2][NB], char* scr, const char* y, const char* yt, int sy, int Wv, const float (&p)[4][4], int half,
                                       int i, int j, int l16, int g, bool bad)
 {
@@ -535,7 +537,7 @@ __device__ __forceinline__ void weigh(f4 (&acc)[2][NB], char* scr, const char* y
 #pragma unroll
 						for (int e = 0; e < 4; e++) {
 							const int col = 16 * wb + 4 * g + e;
-							if (col < Wv) acc[tb][wb][e] += w * to_f(*reinterpret_cast<const ST*>(k16<ST> ? yt + col * kPitch * 2 + 64 * half + 2 * c : y + (32 * half + c) * sy + 4 * col));
+							if (col < Wv) acc[tb][wb][e] += w * to_f(*reinterpret_cast<const ST*>(k16<ST> ? yt + col * kPitch(TB) * 2 + 64 * half + 2 * c : y + (32 * half + c) * sy + 4 * col));
 						}
 			}
 		return;
@@ -566,7 +568,7 @@ __device__ __forceinline__ void weigh(f4 (&acc)[2][NB], char* scr, const char* y
 #pragma unroll
 		for (int wb = 0; wb < NB; wb++) {
 			if (wb >= blocks) break;
-			const uint4 av = *reinterpret_cast<const uint4*>(yt + (16 * wb + l16) * kPitch * 2 + 64 * half + 16 * g);
+			const uint4 av = *reinterpret_cast<const uint4*>(yt + (16 * wb + l16) * kPitch(TB) * 2 + 64 * half + 16 * g);
 #pragma unroll
 			for (int tb = 0; tb < 2; tb++) acc[tb][wb] = mma16<ST>(av, pb[tb], acc[tb][wb]);
 		}
@@ -590,10 +592,11 @@ __device__ __forceinline__ int place_class(const L1MaskedArgs& A, int prefix, in
 }
 
 // the same with documents, by a whole wave; d: the document of stream row `lane` of the tile, -1 where there is none
-__device__ __forceinline__ int doc_class(int c, int d, Span own, bool own_whole)
+template <int TB>
+__device__ __forceinline__ int doc_class(int c, int d, Span own, bool own_whole, int lane)
 {
-	if (!__ballot(d >= 0 && d >= own.lo && d <= own.hi)) return 0;
-	return !own_whole || own.lo != own.hi || __ballot(d != own.lo) ? 2 : c;
+	if (!__ballot(d >= 0 && d >= own.lo && d <= own.hi && lane < kTile<TB>)) return 0;
+	return !own_whole || own.lo != own.hi || __ballot(d != own.lo && lane < kTile<TB>) ? 2 : c;
 }
 
 // where a workgroup's owners lie and what the two sides are
@@ -604,23 +607,43 @@ struct Block {
 };
 
 // classes of the tiles first + step * t, t < n, for the whole workgroup
-template <bool OWNK>
+template <bool OWNK, int TB>
 __device__ __forceinline__ void classify(const L1MaskedArgs& A, const Block& K, const int* doc, int prefix, int own_lo, int own_hi, Span own_docs,
                                          bool own_whole, int first, int step, int n, unsigned char* cls, int tid, int threads)
 {
-	const int lane = tid & 63;
-	for (int t = doc ? tid >> 6 : tid; t < n; t += doc ? threads >> 6 : threads) {
-		const int lo = (first + step * t) * kTile, hi = min(lo + kTile, K.str_rows);
-		int c = place_class<OWNK>(A, prefix, own_lo, own_hi, K.str_place0 + lo, K.str_place0 + hi - 1, hi - lo == kTile);
-		if (doc && c) c = doc_class(c, lo + lane < hi ? doc[K.str_place0 + lo + lane] : -1, own_docs, own_whole);
-		if (!doc || lane == 0) cls[t] = (unsigned char)c;
+	const auto by_place = [&](int t) {
+		const int lo = (first + step * t) * kTile<TB>, hi = min(lo + kTile<TB>, K.str_rows);
+		return place_class<OWNK>(A, prefix, own_lo, own_hi, K.str_place0 + lo, K.str_place0 + hi - 1, hi - lo == kTile<TB>);
+	};
+	if (!doc) {
+		for (int t = tid; t < n; t += threads) cls[t] = (unsigned char)by_place(t);
+		return;
+	}
+	// a wave for each tile, eight tiles' loads at a time: their latency is most of this
+	const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = threads >> 6;
+	for (int t0 = wave; t0 < n; t0 += 8 * waves) {
+		int d[8];
+#pragma unroll
+		for (int u = 0; u < 8; u++) {
+			const int row = (first + step * (t0 + u * waves)) * kTile<TB> + lane;
+			d[u] = -1;
+			if (t0 + u * waves < n && lane < kTile<TB> && row < K.str_rows) d[u] = doc[K.str_place0 + row];
+		}
+#pragma unroll
+		for (int u = 0; u < 8; u++) {
+			const int t = t0 + u * waves;
+			if (t >= n) break;
+			int c = by_place(t);
+			if (c) c = doc_class<TB>(c, d[u], own_docs, own_whole, lane);
+			if (lane == 0) cls[t] = (unsigned char)c;
+		}
 	}
 }
 
 __device__ __forceinline__ int next_tile(const unsigned char* cls, int t, int n)
 {
 	while (t < n && !cls[t]) t++;
-	return t;
+	return __builtin_amdgcn_readfirstlane(t);  // the same in all lanes
 }
 
 // no short cuts: a branch for every pair would cost more than the comparisons
@@ -639,8 +662,8 @@ __device__ __forceinline__ void owner_docs(const int* doc, const Block& K, int r
 		if (d >= 0) lo = hi = d; else none = 1;
 	}
 	lo = wave_min(lo); hi = wave_max(hi); none = wave_max(none);
-	mine = {lo, hi};
-	mine_whole = !none;
+	mine = {__builtin_amdgcn_readfirstlane(lo), __builtin_amdgcn_readfirstlane(hi)};
+	mine_whole = !__builtin_amdgcn_readfirstlane(none);
 	if (lane == 0) { shared[3 * wave] = lo; shared[3 * wave + 1] = hi; shared[3 * wave + 2] = none; }
 	__syncthreads();
 	for (int w = 0; w < waves; w++) { lo = min(lo, shared[3 * w]); hi = max(hi, shared[3 * w + 1]); none = max(none, shared[3 * w + 2]); }
@@ -686,33 +709,33 @@ __device__ __forceinline__ bool owner_grid(const ST* __restrict__ x, const int* 
 
 // A wave's distances of one tile, acc[a][b] >= 0 scaled by 1/sqrt(W), NaN where a value is.  Called by all waves of the
 // workgroup; `active`: this wave needs them.  Without a grid 16-bit rows go through LDS as float32, half of the columns at a time.
-template <typename ST, bool AHEAD>
+template <typename ST, bool AHEAD, int TB>
 __device__ __forceinline__ void tile_distances(char* own, char* str, const float* over, const Layout& Y, int W, float rw, const Grid& G, bool coded,
                                                bool active, const ST* __restrict__ own_x, int own_r0, int own_rows, int64_t own_pitch,
                                                const ST* __restrict__ str_x, int s0, int str_rows, int64_t str_pitch, int i, int j, int tid, int threads,
-                                               float (&x)[4][8])
+                                               float (&x)[4][TB])
 {
 	if constexpr (!k16<ST>) {
 #pragma unroll
 		for (int a = 0; a < 4; a++)
 #pragma unroll
-			for (int b = 0; b < 8; b++) x[a][b] = 0.f;
-		if (active) distances32<AHEAD>(own, str, (W + 3) >> 2, Y.so, i, j, x);
+			for (int b = 0; b < TB; b++) x[a][b] = 0.f;
+		if (active) distances32<AHEAD, TB>(own, str, (W + 3) >> 2, Y.so, i, j, x);
 #pragma unroll
 		for (int a = 0; a < 4; a++)
 #pragma unroll
-			for (int b = 0; b < 8; b++) x[a][b] *= rw;
+			for (int b = 0; b < TB; b++) x[a][b] *= rw;
 	} else if (coded) {
 		if (!active) return;
-		unsigned acc[4][8];
+		unsigned acc[4][TB];
 #pragma unroll
 		for (int a = 0; a < 4; a++)
 #pragma unroll
-			for (int b = 0; b < 8; b++) acc[a][b] = 0;
-		distances16<AHEAD>(own, str, (W + 7) >> 3, Y.so, i, j, acc);
+			for (int b = 0; b < TB; b++) acc[a][b] = 0;
+		distances16<AHEAD, TB>(own, str, (W + 7) >> 3, Y.so, i, j, acc);
 		const float m = G.inv * rw;
 #pragma unroll
-		for (int b = 0; b < 8; b++) {
+		for (int b = 0; b < TB; b++) {
 			const float o = over[j + 8 * b] * rw;
 #pragma unroll
 			for (int a = 0; a < 4; a++) x[a][b] = __builtin_fmaf((float)acc[a][b], m, o);
@@ -721,20 +744,20 @@ __device__ __forceinline__ void tile_distances(char* own, char* str, const float
 #pragma unroll
 		for (int a = 0; a < 4; a++)
 #pragma unroll
-			for (int b = 0; b < 8; b++) x[a][b] = 0.f;
+			for (int b = 0; b < TB; b++) x[a][b] = 0.f;
 		const int part = 4 * (((W + 7) >> 3));  // columns that fit a row of codes
 		for (int w0 = 0; w0 < W; w0 += part) {
 			const int n = min(part, W - w0);
 			__syncthreads();
 			stage32(own, own_x, own_r0, kOwn, own_rows, own_pitch, w0, n, Y.so, false, tid & 63, 64);
-			stage32(str, str_x, s0, kTile, str_rows, str_pitch, w0, n, Y.so, false, tid, threads);
+			stage32(str, str_x, s0, kTile<TB>, str_rows, str_pitch, w0, n, Y.so, false, tid, threads);
 			__syncthreads();
-			if (active) distances32<false>(own, str, (n + 3) >> 2, Y.so, i, j, x);
+			if (active) distances32<false, TB>(own, str, (n + 3) >> 2, Y.so, i, j, x);
 		}
 #pragma unroll
 		for (int a = 0; a < 4; a++)
 #pragma unroll
-			for (int b = 0; b < 8; b++) x[a][b] *= rw;
+			for (int b = 0; b < TB; b++) x[a][b] *= rw;
 	}
 }
 
@@ -771,24 +794,24 @@ __device__ __forceinline__ float weight(float x)
 // NB: 16-column blocks of the value width held by a wave.  Grid: x = batch * head (heads next to each other go to different
 // XCDs and one head's tiles to one), y = owner tiles, the last first: under causality it has the most to do; z = splits: split
 // z takes every gridDim.z-th tile of the stream.  part: NULL, or [splits][B][T][H][Wv + 1] sums to be joined, weights' sum last.
-template <typename ST, bool CAP, int NB, int THREADS>
+template <typename ST, bool CAP, int NB, int TB, int THREADS>
 __global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* __restrict__ q, const ST* __restrict__ k,
                                                       const ST* __restrict__ v, ST* __restrict__ o, float* __restrict__ lse, float* __restrict__ part)
 {
 	constexpr int KN = k16<ST> && NB == 8 ? 4 : 2, VN = k16<ST> && NB < 8 ? 1 : 2;
 	extern __shared__ __align__(16) char lds[];
-	const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 63, wave = tid >> 6, waves = threads >> 6;
+	const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = threads >> 6;
 	const int i = lane & 7, j = lane >> 3, l16 = lane & 15, g = lane >> 4;
 	Block K;
 	K.b = blockIdx.x / A.H; K.h = blockIdx.x % A.H; K.hk = K.h / (A.H / A.Hk);
 	K.nown = waves * kOwn; K.own0 = (gridDim.y - 1 - blockIdx.y) * K.nown;
 	K.own_rows = A.T; K.str_rows = A.S; K.own_place0 = A.S - A.T; K.str_place0 = 0;
 	const int row0 = K.own0 + wave * kOwn;
-	const Layout Y = masked_layout<ST>(A.W, A.Wv, waves, false, true);
+	const Layout Y = masked_layout<ST, TB>(A.W, A.Wv, waves, false, true);
 	char *own = lds + Y.own + wave * kOwn * Y.so, *str = lds + Y.str, *y = lds + Y.y, *yt = lds + Y.yt, *scr = lds + Y.scratch + wave * kScratch;
 	int* docs = reinterpret_cast<int*>(lds + Y.rows);
-	float* over = reinterpret_cast<float*>(lds + Y.rows) + 3 * kTile;
-	float* red = over + kTile;
+	float* over = reinterpret_cast<float*>(lds + Y.rows) + 3 * kTile<TB>;
+	float* red = over + kTile<TB>;
 	unsigned char* cls = reinterpret_cast<unsigned char*>(red + 64);
 	const int* doc = A.doc ? A.doc + (int64_t)K.b * A.S : nullptr;
 	const int prefix = A.prefix ? A.prefix[K.b] : 0;
@@ -821,32 +844,32 @@ __global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* 
 #pragma unroll
 		for (int wb = 0; wb < NB; wb++) out[tb][wb] = (f4)(0.f);
 	const int s_end = A.causal ? min(A.S, max(own_hi + 1, prefix)) : A.S;  // nothing behind is visible
-	const int tiles = (s_end + kTile - 1) / kTile, step = gridDim.z;
+	const int tiles = (s_end + kTile<TB> - 1) / kTile<TB>, step = gridDim.z;
 	for (int t0 = blockIdx.z; t0 < tiles; t0 += step * kClasses) {
 		const int n = min(kClasses, (tiles - t0 + step - 1) / step);
 		__syncthreads();
-		classify<false>(A, K, doc, prefix, own_lo, own_hi, all, all_whole, t0, step, n, cls, tid, threads);
+		classify<false, TB>(A, K, doc, prefix, own_lo, own_hi, all, all_whole, t0, step, n, cls, tid, threads);
 		__syncthreads();
-		Stream<ST, KN, VN> F;
+		Stream<ST, TB, KN, VN> F;
 		int next = next_tile(cls, 0, n);
-		if (next < n) F.fetch(kh, kpitch, A.W, A.vec & 2, vh, vpitch, A.Wv, A.vec & 4, (t0 + step * next) * kTile, A.S, doc, nullptr, nullptr, 0, tid, threads);
+		if (next < n) F.fetch(kh, kpitch, A.W, A.vec & 2, vh, vpitch, A.Wv, A.vec & 4, (t0 + step * next) * kTile<TB>, A.S, doc, nullptr, nullptr, 0, tid, threads);
 		while (next < n) {
-			const int kind = cls[next], s0 = (t0 + step * next) * kTile;
+			const int kind = __builtin_amdgcn_readfirstlane(cls[next]), s0 = (t0 + step * next) * kTile<TB>;
 			const int tid = here(threadIdx.x), lane = tid & 63, i = lane & 7, j = lane >> 3, l16 = lane & 15, g = lane >> 4;
 			__syncthreads();
 			bool bad = F.place(str, nullptr, over, k16<ST> ? nullptr : y, yt, docs, nullptr, nullptr, Y, G, kh, kpitch, A.W, A.vec & 2, vh, vpitch, A.Wv,
 			                   A.vec & 4, s0, A.S, tid, threads);
 			next = next_tile(cls, next + 1, n);
-			if (next < n) F.fetch(kh, kpitch, A.W, A.vec & 2, vh, vpitch, A.Wv, A.vec & 4, (t0 + step * next) * kTile, A.S, doc, nullptr, nullptr, 0, tid, threads);
+			if (next < n) F.fetch(kh, kpitch, A.W, A.vec & 2, vh, vpitch, A.Wv, A.vec & 4, (t0 + step * next) * kTile<TB>, A.S, doc, nullptr, nullptr, 0, tid, threads);
 			bad = __syncthreads_or(bad && kind == 2);
-			// what the tile is to this wave's own rows
 			int mykind = row0 < A.T ? kind : 0;
 			if (mykind == 2) {
-				mykind = place_class<false>(A, prefix, my_lo, my_hi, s0, min(s0 + kTile, A.S) - 1, s0 + kTile <= A.S);
-				if (mykind && doc) mykind = doc_class(mykind, docs[lane], mine, mine_whole);
+				mykind = place_class<false>(A, prefix, my_lo, my_hi, s0, min(s0 + kTile<TB>, A.S) - 1, s0 + kTile<TB> <= A.S);
+				if (mykind && doc) mykind = doc_class<TB>(mykind, docs[lane % kTile<TB>], mine, mine_whole, lane);
 			}
-			float x[4][8];
-			tile_distances<ST, true>(own, str, over, Y, A.W, A.rw, G, coded, mykind, qh, row0, A.T, qpitch, kh, s0, A.S, kpitch, i, j, tid, threads, x);
+			mykind = __builtin_amdgcn_readfirstlane(mykind);  // what the tile is to this wave's own rows
+			float x[4][TB];
+			tile_distances<ST, true, TB>(own, str, over, Y, A.W, A.rw, G, coded, mykind, qh, row0, A.T, qpitch, kh, s0, A.S, kpitch, i, j, tid, threads, x);
 			if (!mykind) continue;
 			// float32: a tile's sum on its own, then to the total: the roundings of either are fewer
 			f4 tile[2][NB];
@@ -856,7 +879,7 @@ __global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* 
 #pragma unroll
 					for (int wb = 0; wb < NB; wb++) tile[tb][wb] = (f4)(0.f);
 #pragma unroll
-			for (int half = 0; half < 2; half++) {
+			for (int half = 0; half < TB / 4; half++) {
 				float p[4][4];
 #pragma unroll
 				for (int bb = 0; bb < 4; bb++) {
@@ -869,6 +892,7 @@ __global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* 
 					}
 				}
 				if (mykind == 2) {
+					asm volatile("");  // a branch: the compiler would rather compare in every tile and select
 #pragma unroll
 					for (int bb = 0; bb < 4; bb++) {
 						const int s = s0 + j + 8 * (4 * half + bb), sd = docs[j + 8 * (4 * half + bb)];
@@ -881,8 +905,8 @@ __global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* 
 				for (int bb = 0; bb < 4; bb++)
 #pragma unroll
 					for (int a = 0; a < 4; a++) den[a] += p[a][bb];
-				if constexpr (k16<ST>) weigh<ST, NB>(out, scr, y, yt, Y.sy, A.Wv, p, half, i, j, l16, g, bad);
-				else weigh<ST, NB>(tile, scr, y, yt, Y.sy, A.Wv, p, half, i, j, l16, g, bad);
+				if constexpr (k16<ST>) weigh<ST, NB, TB>(out, scr, y, yt, Y.sy, A.Wv, p, half, i, j, l16, g, bad);
+				else weigh<ST, NB, TB>(tile, scr, y, yt, Y.sy, A.Wv, p, half, i, j, l16, g, bad);
 			}
 			if constexpr (!k16<ST>)
 #pragma unroll
@@ -1037,14 +1061,14 @@ __device__ __forceinline__ void signs(float (&sum)[WL][32], const float (&ov)[WL
 // Gradients of one side.  OWNK false: owners are queries, dx = dq.  OWNK true: owners are keys, dx = dk and dy = dv, summed
 // over the query heads that share them.  WL: columns w a lane holds in the sign part (W <= 64 * WL).  With g = the gradient of
 // the score: sum g * sign = 2 * sum g * h - sum g.  Grid as in the forward; px, py: NULL, or [splits][rows][W], [splits][rows][Wv].
-template <typename ST, bool OWNK, bool CAP, int WL, int NB, int THREADS>
+template <typename ST, bool OWNK, bool CAP, int WL, int NB, int TB, int THREADS>
 __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* __restrict__ q, const ST* __restrict__ k,
                                                       const ST* __restrict__ v, const ST* __restrict__ dout,
                                                       const float* __restrict__ lse, const float* __restrict__ D,
                                                       ST* __restrict__ dx, ST* __restrict__ dy, float* __restrict__ px, float* __restrict__ py)
 {
 	extern __shared__ __align__(16) char lds[];
-	const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 63, wave = tid >> 6, waves = threads >> 6;
+	const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = threads >> 6;
 	const int i = lane & 7, j = lane >> 3, l16 = lane & 15, g = lane >> 4;
 	constexpr int KN = k16<ST> && NB == 8 ? 4 : 2, VN = k16<ST> && NB < 8 ? 1 : 2;
 	const int group = A.H / A.Hk, heads = OWNK ? A.Hk : A.H;
@@ -1060,12 +1084,12 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 	K.own_place0 = OWNK ? 0 : A.S - A.T;
 	K.str_place0 = OWNK ? A.S - A.T : 0;
 	const int row0 = K.own0 + wave * kOwn;
-	const Layout Y = masked_layout<ST>(A.W, A.Wv, waves, true, OWNK);
+	const Layout Y = masked_layout<ST, TB>(A.W, A.Wv, waves, true, OWNK);
 	char *own = lds + Y.own + wave * kOwn * Y.so, *str = lds + Y.str, *raw = lds + Y.raw, *y = lds + Y.y, *yt = lds + Y.yt;
 	char* scr = lds + Y.scratch + wave * kScratch;
 	float* sc = reinterpret_cast<float*>(scr);
 	int* docs = reinterpret_cast<int*>(lds + Y.rows);
-	float *slse = reinterpret_cast<float*>(docs) + kTile, *sD = slse + kTile, *over = sD + kTile, *red = over + kTile;
+	float *slse = reinterpret_cast<float*>(docs) + kTile<TB>, *sD = slse + kTile<TB>, *over = sD + kTile<TB>, *red = over + kTile<TB>;
 	unsigned char* cls = reinterpret_cast<unsigned char*>(red + 64);
 	const int* doc = A.doc ? A.doc + (int64_t)K.b * A.S : nullptr;
 	const int prefix = A.prefix ? A.prefix[K.b] : 0;
@@ -1135,45 +1159,46 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 			olse[a] = in ? lse[((int64_t)K.b * A.T + t) * A.H + h] : 0.f;
 			oD[a] = in ? D[((int64_t)K.b * A.T + t) * A.H + h] : 0.f;
 		}
-		int first = 0, last = (K.str_rows + kTile - 1) / kTile;
+		int first = 0, last = (K.str_rows + kTile<TB> - 1) / kTile<TB>;
 		if (A.causal) {
-			if (OWNK) { if (own_lo >= prefix) first = max(0, own_lo - K.str_place0) / kTile; }
-			else last = (min(A.S, max(own_hi + 1, prefix)) + kTile - 1) / kTile;
+			if (OWNK) { if (own_lo >= prefix) first = max(0, own_lo - K.str_place0) / kTile<TB>; }
+			else last = (min(A.S, max(own_hi + 1, prefix)) + kTile<TB> - 1) / kTile<TB>;
 		}
 		const int step = gridDim.z;
 		for (int t0 = first + blockIdx.z; t0 < last; t0 += step * kClasses) {
 			const int n = min(kClasses, (last - t0 + step - 1) / step);
 			__syncthreads();
-			classify<OWNK>(A, K, doc, prefix, own_lo, own_hi, all, all_whole, t0, step, n, cls, tid, threads);
+			classify<OWNK, TB>(A, K, doc, prefix, own_lo, own_hi, all, all_whole, t0, step, n, cls, tid, threads);
 			__syncthreads();
-			Stream<ST, KN, VN> F;
+			Stream<ST, TB, KN, VN> F;
 			const ST* str_y = OWNK ? oh : vh;
 			const int64_t y_pitch = OWNK ? opitch : vpitch;
 			const bool y_vec = A.vec & (OWNK ? 8 : 4);
 			const int* str_doc = doc ? doc + K.str_place0 : nullptr;
 			const float *lh = OWNK ? lse + (int64_t)K.b * A.T * A.H + h : nullptr, *Dh = OWNK ? D + (int64_t)K.b * A.T * A.H + h : nullptr;
 			int next = next_tile(cls, 0, n);
-			if (next < n) F.fetch(str_x, str_pitch, A.W, str_vec, str_y, y_pitch, A.Wv, y_vec, (t0 + step * next) * kTile, K.str_rows, str_doc, lh, Dh, A.H, tid, threads);
+			if (next < n) F.fetch(str_x, str_pitch, A.W, str_vec, str_y, y_pitch, A.Wv, y_vec, (t0 + step * next) * kTile<TB>, K.str_rows, str_doc, lh, Dh, A.H, tid, threads);
 			while (next < n) {
-				const int kind = cls[next], s0 = (t0 + step * next) * kTile;
+				const int kind = __builtin_amdgcn_readfirstlane(cls[next]), s0 = (t0 + step * next) * kTile<TB>;
 				const int tid = here(threadIdx.x), lane = tid & 63, i = lane & 7, j = lane >> 3, l16 = lane & 15, g = lane >> 4;
 				__syncthreads();
 				// without a grid the codes come out as nonsense that nobody reads; the ordered integers are wanted all the same
 				bool bad = F.place(str, raw, over, y, k16<ST> && OWNK ? yt : nullptr, docs, OWNK ? slse : nullptr, sD, Y, G, str_x, str_pitch, A.W, str_vec,
 				                   str_y, y_pitch, A.Wv, y_vec, s0, K.str_rows, tid, threads);
 				next = next_tile(cls, next + 1, n);
-				if (next < n) F.fetch(str_x, str_pitch, A.W, str_vec, str_y, y_pitch, A.Wv, y_vec, (t0 + step * next) * kTile, K.str_rows, str_doc, lh, Dh, A.H, tid, threads);
+				if (next < n) F.fetch(str_x, str_pitch, A.W, str_vec, str_y, y_pitch, A.Wv, y_vec, (t0 + step * next) * kTile<TB>, K.str_rows, str_doc, lh, Dh, A.H, tid, threads);
 				bad = __syncthreads_or(bad && kind == 2);
 				int mykind = row0 < K.own_rows ? kind : 0;
 				if (mykind == 2) {
-					mykind = place_class<OWNK>(A, prefix, my_lo, my_hi, K.str_place0 + s0, K.str_place0 + min(s0 + kTile, K.str_rows) - 1, s0 + kTile <= K.str_rows);
-					if (mykind && doc) mykind = doc_class(mykind, docs[lane], mine, mine_whole);
+					mykind = place_class<OWNK>(A, prefix, my_lo, my_hi, K.str_place0 + s0, K.str_place0 + min(s0 + kTile<TB>, K.str_rows) - 1, s0 + kTile<TB> <= K.str_rows);
+					if (mykind && doc) mykind = doc_class<TB>(mykind, docs[lane % kTile<TB>], mine, mine_whole, lane);
 				}
-				float x[4][8];
-				tile_distances<ST, false>(own, str, over, Y, A.W, A.rw, G, coded, mykind, own_x, row0, K.own_rows, own_pitch, str_x, s0, K.str_rows, str_pitch, i, j, tid, threads, x);
+				mykind = __builtin_amdgcn_readfirstlane(mykind);  // what the tile is to this wave's own rows
+				float x[4][TB];
+				tile_distances<ST, true, TB>(own, str, over, Y, A.W, A.rw, G, coded, mykind, own_x, row0, K.own_rows, own_pitch, str_x, s0, K.str_rows, str_pitch, i, j, tid, threads, x);
 				if (!mykind) continue;
 #pragma unroll
-				for (int half = 0; half < 2; half++) {
+				for (int half = 0; half < TB / 4; half++) {
 					const int lane = here(tid & 63), i = lane & 7, j = lane >> 3, l16 = lane & 15, g = lane >> 4;
 					float p[4][4], pf[4][4];  // weights, and the derivative of their argument by the distance's sum
 #pragma unroll
@@ -1189,6 +1214,7 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 						}
 					}
 					if (mykind == 2) {
+						asm volatile("");  // a branch, as in the forward
 #pragma unroll
 						for (int bb = 0; bb < 4; bb++) {
 							const int r = j + 8 * (4 * half + bb), sp = K.str_place0 + s0 + r, sd = docs[r];
@@ -1200,7 +1226,7 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 							}
 						}
 					}
-					if constexpr (OWNK) weigh<ST, NY>(dyv, scr, y, yt, Y.sy, A.Wv, p, half, i, j, l16, g, bad);
+					if constexpr (OWNK) weigh<ST, NY, TB>(dyv, scr, y, yt, Y.sy, A.Wv, p, half, i, j, l16, g, bad);
 					// dp of this half's 32 columns
 					f4 dp[2][2];
 #pragma unroll
@@ -1336,14 +1362,16 @@ int launch(F* f, dim3 grid, int waves, int bytes, hipStream_t st, void** args)
 
 template <typename ST>
 struct MaskedImpl {
+	static constexpr int TF = k16<ST> ? 8 : 4, TBW = 4;  // tiles of the forward and of the backward
+
 	template <bool CAP>
 	static int fwd_cap(L1MaskedArgs& A, const L1MaskedPlan& P, const void* q, const void* k, const void* v, void* o, float* lse, float* part, hipStream_t st)
 	{
 		const dim3 grid((unsigned)(A.B * A.H), (unsigned)l1_cdiv(A.T, kOwn * P.waves), (unsigned)P.splits);
-		const int bytes = masked_layout<ST>(A.W, A.Wv, P.waves, false, true).total;
+		const int bytes = masked_layout<ST, TF>(A.W, A.Wv, P.waves, false, true).total;
 		void* args[] = {&A, &q, &k, &v, &o, &lse, &part};
-		if (A.Wv > 64) return launch(masked_fwd<ST, CAP, 8, 256>, grid, P.waves, bytes, st, args);
-		return launch(masked_fwd<ST, CAP, 4, 512>, grid, P.waves, bytes, st, args);
+		if (A.Wv > 64) return launch(masked_fwd<ST, CAP, 8, TF, 256>, grid, P.waves, bytes, st, args);
+		return launch(masked_fwd<ST, CAP, 4, TF, 512>, grid, P.waves, bytes, st, args);
 	}
 	static int fwd(L1MaskedArgs& A, const L1MaskedPlan& P, const void* q, const void* k, const void* v, void* o, float* lse, float* part, hipStream_t st)
 	{
@@ -1366,11 +1394,11 @@ struct MaskedImpl {
 	{
 		const int64_t heads = (int64_t)A.B * (OWNK ? A.Hk : A.H), n = OWNK ? A.S : A.T;
 		const dim3 grid((unsigned)heads, (unsigned)l1_cdiv(n, kOwn * P.waves), (unsigned)P.splits);
-		const int bytes = masked_layout<ST>(A.W, A.Wv, P.waves, true, OWNK).total;
+		const int bytes = masked_layout<ST, TBW>(A.W, A.Wv, P.waves, true, OWNK).total;
 		void* args[] = {&A, &q, &k, &v, &dout, &lse, &D, &dx, &dy, &px, &py};
-		if (A.W > 64) return launch(masked_bwd<ST, OWNK, CAP, 2, 8, 256>, grid, P.waves, bytes, st, args);
-		if (A.Wv > 64) return launch(masked_bwd<ST, OWNK, CAP, 1, 8, 256>, grid, P.waves, bytes, st, args);
-		return launch(masked_bwd<ST, OWNK, CAP, 1, 4, 512>, grid, P.waves, bytes, st, args);
+		if (A.W > 64) return launch(masked_bwd<ST, OWNK, CAP, 2, 8, TBW, 256>, grid, P.waves, bytes, st, args);
+		if (A.Wv > 64) return launch(masked_bwd<ST, OWNK, CAP, 1, 8, TBW, 256>, grid, P.waves, bytes, st, args);
+		return launch(masked_bwd<ST, OWNK, CAP, 1, 4, TBW, 512>, grid, P.waves, bytes, st, args);
 	}
 	template <bool OWNK>
 	static int side(L1MaskedArgs& A, const L1MaskedPlan& P, const void* q, const void* k, const void* v, const void* dout, const float* lse, const float* D,
@@ -1399,7 +1427,10 @@ struct MaskedImpl {
 	{
 		return side<true>(A, P, q, k, v, dout, lse, D, dk, dv, part, st);
 	}
-	static int lds(int W, int Wv, int waves, bool backward, bool weigh) { return masked_layout<ST>(W, Wv, waves, backward, weigh).total; }
+	static int lds(int W, int Wv, int waves, bool backward, bool weigh)
+	{
+		return backward ? masked_layout<ST, TBW>(W, Wv, waves, true, weigh).total : masked_layout<ST, TF>(W, Wv, waves, false, weigh).total;
+	}
 };
 
 }  // namespace
