@@ -38,6 +38,7 @@ namespace {
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef short short2v __attribute__((ext_vector_type(2)));
 
 constexpr int kOwn = 32;        // owner rows of a wave
 constexpr int kPad = 36;        // floats in a row of the scratch: 9 chunks of 16 bytes, odd, so rows spread over the banks
@@ -52,9 +53,15 @@ template <typename ST> constexpr bool k16 = sizeof(ST) == 2;
 // type, 2^-12 (float16) and 2^-9 (bfloat16) on average
 template <typename ST> constexpr float kRange = 24.f;
 template <> constexpr float kRange<__bf16> = 160.f;
-// what a weight is multiplied by before it is rounded to 16 bits: p <= 1, and float16 has no room below 2^-14
+// what a weight is multiplied by: p <= 1, and is rounded to 16 bits for the products; float16 has no room below 2^-14
 template <typename ST> constexpr float kWeight = 1.f;
 template <> constexpr float kWeight<_Float16> = 16384.f;
+
+// What the weights' exponents are counted in: 16-bit rows take 2^x, so that everything but the distance's factor is multiplied by
+// log2(e) once per row instead of once per pair; and p times kWeight, which is an addition to the exponent.
+template <typename ST> constexpr float kUnit = k16<ST> ? 1.442695041f : 1.f;
+template <typename ST> constexpr float kShift = 0.f;
+template <> constexpr float kShift<_Float16> = 14.f;
 
 // an odd number of 16-byte chunks for n of them: neighbouring rows start in different banks
 __host__ __device__ __forceinline__ int odd_chunks(int n) { return n | 1; }
@@ -112,8 +119,6 @@ __device__ __forceinline__ void unpack(const uint4& r, float (&x)[per])
 	for (int e = 0; e < per; e++) x[e] = to_f(h[e]);
 }
 
-// The bits of a 16-bit float as an integer in the same order: -0 and 0 are 0, and equal values and no others are equal.
-__device__ __forceinline__ int ordered(unsigned bits) { return bits & 0x8000u ? -(int)(bits & 0x7fffu) : (int)bits; }
 
 // stream row r of a tile <-> its place c in the order of the products
 __device__ __forceinline__ int col_of(int r) { return 32 * (r >> 5) + 4 * (r & 7) + ((r >> 3) & 3); }
@@ -302,34 +307,35 @@ __device__ __forceinline__ void stage32(char* dst, const ST* __restrict__ x, int
 }
 
 // the grid of a workgroup's codes
-struct Grid { float lo, hi, sc, inv; };
+// x -> x * sc + b in [0, 1], which is 65535 steps; inv: one step
+struct Grid { float sc, b, inv; };
 
-// eight values as codes, the first n of them; over: plus what lies outside of the range
+// eight values as codes, those behind the first n as zero; over: plus what lies outside of [0, 1]
 template <typename ST>
 __device__ __forceinline__ uint4 codes_of(const uint4& bits, int n, const Grid& G, float& over)
 {
 	float v[8];
-	unsigned code[8];
 	unpack<ST>(bits, v);
+	unsigned w[4];
 #pragma unroll
 	for (int e = 0; e < 8; e++) {
-		const float y = __builtin_amdgcn_fmed3f(v[e], G.lo, G.hi);
-		over += e < n ? __builtin_fabsf(v[e] - y) : 0.f;
-		code[e] = e < n ? (unsigned)__builtin_fmaf(y - G.lo, G.sc, 0.5f) : 0u;
+		v[e] = __builtin_fmaf(v[e], G.sc, G.b);
+		if (n < 8) v[e] = e < n ? v[e] : 0.f;
+		over += __builtin_fabsf(v[e] - __builtin_amdgcn_fmed3f(v[e], 0.f, 1.f));
 	}
-	return make_uint4(code[0] | code[1] << 16, code[2] | code[3] << 16, code[4] | code[5] << 16, code[6] | code[7] << 16);
+#pragma unroll
+	for (int e = 0; e < 4; e++) w[e] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pknorm_u16(v[2 * e], v[2 * e + 1]));
+	return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// the bits of eight 16-bit floats as integers in the same order: -0 and 0 are 0, and equal values and no others are equal
 __device__ __forceinline__ uint4 ordered8(const uint4& bits)
 {
-	unsigned short b[8];
-	short s[8];
-	__builtin_memcpy(b, &bits, 16);
-#pragma unroll
-	for (int e = 0; e < 8; e++) s[e] = (short)ordered(b[e]);
-	uint4 r;
-	__builtin_memcpy(&r, s, 16);
-	return r;
+	const auto two = [](unsigned x) {
+		const short2v m = __builtin_bit_cast(short2v, x) >> 15;
+		return __builtin_bit_cast(unsigned, (__builtin_bit_cast(short2v, x & 0x7fff7fffu) ^ m) - m);
+	};
+	return make_uint4(two(bits.x), two(bits.y), two(bits.z), two(bits.w));
 }
 
 // The owner rows of a wave as codes, and (raw, unless NULL) as ordered integers.
@@ -462,14 +468,18 @@ struct Stream {
 				}
 				if (yt) {
 					const unsigned a[4] = {A.x, A.y, A.z, A.w}, b[4] = {B.x, B.y, B.z, B.w};
-					// not finite: all bits of the exponent
-					constexpr unsigned em = __is_same(ST, _Float16) ? 0x7c00u : 0x7f80u;
+					// not finite: all bits of the exponent, and one more at its end carries into the sign's place
+					constexpr unsigned em = __is_same(ST, _Float16) ? 0x7c007c00u : 0x7f807f80u, one = __is_same(ST, _Float16) ? 0x04000400u : 0x00800080u;
+					unsigned carry = 0;
 #pragma unroll
-					for (int e = 0; e < 4; e++) {
-						bad |= (a[e] & em) == em || (a[e] >> 16 & em) == em || (b[e] & em) == em || (b[e] >> 16 & em) == em;
-						if (8 * ch < tcols) {
-							*reinterpret_cast<unsigned*>(yt + (8 * ch + 2 * e) * kPitch(TB) * 2 + 4 * c2) = (a[e] & 0xffffu) | (b[e] << 16);
-							*reinterpret_cast<unsigned*>(yt + (8 * ch + 2 * e + 1) * kPitch(TB) * 2 + 4 * c2) = (a[e] >> 16) | (b[e] & 0xffff0000u);
+					for (int e = 0; e < 4; e++) carry |= ((a[e] & em) + one) | ((b[e] & em) + one);
+					bad |= (carry & 0x80008000u) != 0;
+					if (8 * ch < tcols) {
+						char* to = yt + 8 * ch * kPitch(TB) * 2 + 4 * c2;
+#pragma unroll
+						for (int e = 0; e < 4; e++) {
+							*reinterpret_cast<unsigned*>(to + 2 * e * kPitch(TB) * 2) = __builtin_amdgcn_perm(b[e], a[e], 0x05040100u);
+							*reinterpret_cast<unsigned*>(to + (2 * e + 1) * kPitch(TB) * 2) = __builtin_amdgcn_perm(b[e], a[e], 0x07060302u);
 						}
 					}
 				}
@@ -484,7 +494,7 @@ struct Stream {
 		}
 		if (tid < kTile<TB>) {
 			docs[tid] = d;
-			if (slse) { slse[tid] = l; sD[tid] = dd; }
+			if (slse) { slse[tid] = l * kUnit<ST> - kShift<ST>; sD[tid] = dd; }
 		}
 		return bad;
 	}
@@ -501,7 +511,7 @@ __device__ __forceinline__ f4 mma16(const uint4& a, const uint4& b, f4 c)
 }
 
 // Weights of half a tile into the wave's scratch, and acc[tb][wb] += sum over its 32 columns c of value[c][16 wb + ..] * p[owner][c].
-// 16 bits: p times kWeight, rounded to the type (a relative error of half a step of the type in each weight, as the
+// 16 bits: rounded to the type (a relative error of half a step of the type in each weight, as the
 // product's other factor has).
 // `bad` (values that are not finite in a tile of which some is hidden): a hidden pair's weight of zero must not meet them, which
 // a matrix instruction cannot leave out.
@@ -516,7 +526,7 @@ __device__ __forceinline__ void weigh(f4 (&acc)[2][NB], char* scr, const char* y
 		if constexpr (k16<ST>) {
 			ST w[4];
 #pragma unroll
-			for (int e = 0; e < 4; e++) w[e] = (ST)(p[a][e] * kWeight<ST>);
+			for (int e = 0; e < 4; e++) w[e] = (ST)p[a][e];
 			uint2 packed;
 			__builtin_memcpy(&packed, w, 8);
 			*reinterpret_cast<uint2*>(scr + (i + 8 * a) * pitch + 8 * j) = packed;
@@ -699,12 +709,15 @@ __device__ __forceinline__ bool owner_grid(const ST* __restrict__ x, const int* 
 	const bool all_finite = !__syncthreads_or(!finite);
 	for (int w = 0; w < waves; w++) { lo = fminf(lo, shared[3 * w]); hi = fmaxf(hi, shared[3 * w + 1]); }
 	if (lo > hi) lo = hi = 0.f;  // no row takes part
-	G.lo = lo;
-	G.hi = hi;
-	G.sc = hi > lo ? 65535.f / (hi - lo) : 0.f;
-	G.inv = (hi - lo) / 65535.f;
-	// a range so narrow that its scale overflows float32 has no use for codes either
-	return all_finite && hi - lo <= kRange<ST> && G.sc <= 1e30f;
+	// a margin of 2^-20 on both sides, or the roundings of x * sc + b would put an owner outside
+	const float span = (hi - lo) * (1.f + 0x1p-19f);
+	lo -= (hi - lo) * 0x1p-20f;
+	G.sc = span > 0.f ? 1.f / span : 0.f;
+	G.b = -lo * G.sc;
+	G.inv = span / 65535.f;
+	// b is rounded by 2^-21 at most up to 8, which the margin covers: values that lie further from zero than that, for their
+	// span, or next to nothing apart, or all the same, go without codes
+	return all_finite && span <= kRange<ST> && span > 0.f && G.sc <= 1e30f && __builtin_fabsf(G.b) <= 8.f;
 }
 
 // A wave's distances of one tile, acc[a][b] >= 0 scaled by 1/sqrt(W), NaN where a value is.  Called by all waves of the
@@ -733,10 +746,10 @@ __device__ __forceinline__ void tile_distances(char* own, char* str, const float
 #pragma unroll
 			for (int b = 0; b < TB; b++) acc[a][b] = 0;
 		distances16<AHEAD, TB>(own, str, (W + 7) >> 3, Y.so, i, j, acc);
-		const float m = G.inv * rw;
+		const float m = G.inv * rw, span = m * 65535.f;
 #pragma unroll
 		for (int b = 0; b < TB; b++) {
-			const float o = over[j + 8 * b] * rw;
+			const float o = over[j + 8 * b] * span;
 #pragma unroll
 			for (int a = 0; a < 4; a++) x[a][b] = __builtin_fmaf((float)acc[a][b], m, o);
 		}
@@ -761,7 +774,7 @@ __device__ __forceinline__ void tile_distances(char* own, char* str, const float
 	}
 }
 
-// capped score and, in fac, its derivative by the score, from the distance over sqrt(W)
+// capped score in those units and, in fac, its derivative by the score, from the distance over sqrt(W) (in those units without a cap)
 template <typename ST, bool CAP>
 __device__ __forceinline__ float score(float dist, float cap, float icap, float& fac)
 {
@@ -778,14 +791,14 @@ __device__ __forceinline__ float score(float dist, float cap, float icap, float&
 			th = tanhf(-dist * icap);
 		}
 		fac = 1.f - th * th;
-		return cap * th;
+		return cap * kUnit<ST> * th;
 	}
 }
 
 template <typename ST>
 __device__ __forceinline__ float weight(float x)
 {
-	if constexpr (k16<ST>) return __builtin_amdgcn_exp2f(x * 1.442695041f);
+	if constexpr (k16<ST>) return __builtin_amdgcn_exp2f(x);
 	else return expf(x);
 }
 
@@ -815,7 +828,7 @@ __global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* 
 	unsigned char* cls = reinterpret_cast<unsigned char*>(red + 64);
 	const int* doc = A.doc ? A.doc + (int64_t)K.b * A.S : nullptr;
 	const int prefix = A.prefix ? A.prefix[K.b] : 0;
-	const float slope = A.has_slopes ? A.slopes[K.h] : 0.f;
+	const float slope = A.has_slopes ? A.slopes[K.h] * kUnit<ST> : 0.f;
 	const int64_t qpitch = (int64_t)A.H * A.W, kpitch = (int64_t)A.Hk * A.W, vpitch = (int64_t)A.Hk * A.Wv;
 	const ST* qh = q + ((int64_t)K.b * A.T * A.H + K.h) * A.W;
 	const ST* kh = k + ((int64_t)K.b * A.S * A.Hk + K.hk) * A.W;
@@ -824,7 +837,7 @@ __global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* 
 	Span mine, all;
 	bool mine_whole, all_whole;
 	owner_docs(doc, K, row0, reinterpret_cast<int*>(red), lane, wave, waves, mine, mine_whole, all, all_whole);
-	Grid G = {0.f, 0.f, 0.f, 0.f};
+	Grid G = {0.f, 0.f, 0.f};
 	bool coded = false;
 	if constexpr (k16<ST>) {
 		coded = owner_grid(qh, doc, K, row0, qpitch, A.W, A.vec & 1, red + 32, lane, wave, waves, G);
@@ -869,7 +882,7 @@ __global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* 
 			}
 			mykind = __builtin_amdgcn_readfirstlane(mykind);  // what the tile is to this wave's own rows
 			float x[4][TB];
-			tile_distances<ST, true, TB>(own, str, over, Y, A.W, A.rw, G, coded, mykind, qh, row0, A.T, qpitch, kh, s0, A.S, kpitch, i, j, tid, threads, x);
+			tile_distances<ST, true, TB>(own, str, over, Y, A.W, CAP ? A.rw : A.rw * kUnit<ST>, G, coded, mykind, qh, row0, A.T, qpitch, kh, s0, A.S, kpitch, i, j, tid, threads, x);
 			if (!mykind) continue;
 			// float32: a tile's sum on its own, then to the total: the roundings of either are fewer
 			f4 tile[2][NB];
@@ -882,15 +895,25 @@ __global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* 
 			for (int half = 0; half < TB / 4; half++) {
 				float p[4][4];
 #pragma unroll
-				for (int bb = 0; bb < 4; bb++) {
-					const int b = 4 * half + bb;
-					const float s = (float)(s0 + j + 8 * b - my_lo - i);
+				for (int bb = 0; bb < 4; bb++)
 #pragma unroll
 					for (int a = 0; a < 4; a++) {
 						float fac;
-						p[a][bb] = weight<ST>(__builtin_fmaf(-slope, __builtin_fabsf(s - 8.f * a), score<ST, CAP>(x[a][b], A.cap, A.icap, fac)));
+						p[a][bb] = score<ST, CAP>(x[a][4 * half + bb], A.cap, A.icap, fac);
+					}
+				if (slope != 0.f) {
+					asm volatile("");  // a branch
+#pragma unroll
+					for (int bb = 0; bb < 4; bb++) {
+						const float s = (float)(s0 + j + 8 * (4 * half + bb) - my_lo - i);
+#pragma unroll
+						for (int a = 0; a < 4; a++) p[a][bb] = __builtin_fmaf(-slope, __builtin_fabsf(s - 8.f * a), p[a][bb]);
 					}
 				}
+#pragma unroll
+				for (int bb = 0; bb < 4; bb++)
+#pragma unroll
+					for (int a = 0; a < 4; a++) p[a][bb] = weight<ST>(p[a][bb] + kShift<ST>);
 				if (mykind == 2) {
 					asm volatile("");  // a branch: the compiler would rather compare in every tile and select
 #pragma unroll
@@ -932,7 +955,7 @@ __global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* 
 #pragma unroll
 	for (int tb = 0; tb < 2; tb++) {
 		const int t = row0 + 16 * tb + l16;
-		const float d = sc[16 * tb + l16];
+		const float d = sc[16 * tb + l16] * (1.f / kWeight<ST>);
 		if (t >= A.T) continue;
 		const int64_t row = ((int64_t)K.b * A.T + t) * A.H + K.h;
 		float* to = part ? part + (blockIdx.z * rows + row) * (A.Wv + 1) : nullptr;
@@ -1104,7 +1127,7 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 	Span mine, all;
 	bool mine_whole, all_whole;
 	owner_docs(doc, K, row0, reinterpret_cast<int*>(red), lane, wave, waves, mine, mine_whole, all, all_whole);
-	Grid G = {0.f, 0.f, 0.f, 0.f};
+	Grid G = {0.f, 0.f, 0.f};
 	bool coded = false;
 	if constexpr (k16<ST>) {
 		coded = owner_grid(own_x, doc, K, row0, own_pitch, A.W, own_vec, red + 32, lane, wave, waves, G);
@@ -1123,6 +1146,7 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 #pragma unroll
 	for (int a = 0; a < 4; a++) od4[a] = doc && row0 + i + 8 * a < K.own_rows ? doc[my_lo + i + 8 * a] : -1;
 	float gsum[4] = {0.f, 0.f, 0.f, 0.f};
+	const float grw = A.rw * (1.f / kWeight<ST>);
 	constexpr int NY = OWNK ? NB : 1;
 	f4 dyv[2][NY];
 #pragma unroll
@@ -1134,7 +1158,7 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 
 	for (int hg = 0; hg < (OWNK ? group : 1); hg++) {
 		const int h = OWNK ? K.hk * group + hg : K.h;
-		const float slope = A.has_slopes ? A.slopes[h] : 0.f;
+		const float slope = A.has_slopes ? A.slopes[h] * kUnit<ST> : 0.f;
 		const ST* qh = q + ((int64_t)K.b * A.T * A.H + h) * A.W;
 		const ST* oh = dout + ((int64_t)K.b * A.T * A.H + h) * A.Wv;
 		const ST* str_x = OWNK ? qh : kh;
@@ -1156,7 +1180,7 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 		for (int a = 0; a < 4; a++) {
 			const int t = row0 + i + 8 * a;
 			const bool in = !OWNK && t < A.T;
-			olse[a] = in ? lse[((int64_t)K.b * A.T + t) * A.H + h] : 0.f;
+			olse[a] = in ? lse[((int64_t)K.b * A.T + t) * A.H + h] * kUnit<ST> - kShift<ST> : 0.f;
 			oD[a] = in ? D[((int64_t)K.b * A.T + t) * A.H + h] : 0.f;
 		}
 		int first = 0, last = (K.str_rows + kTile<TB> - 1) / kTile<TB>;
@@ -1195,7 +1219,7 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 				}
 				mykind = __builtin_amdgcn_readfirstlane(mykind);  // what the tile is to this wave's own rows
 				float x[4][TB];
-				tile_distances<ST, true, TB>(own, str, over, Y, A.W, A.rw, G, coded, mykind, own_x, row0, K.own_rows, own_pitch, str_x, s0, K.str_rows, str_pitch, i, j, tid, threads, x);
+				tile_distances<ST, true, TB>(own, str, over, Y, A.W, CAP ? A.rw : A.rw * kUnit<ST>, G, coded, mykind, own_x, row0, K.own_rows, own_pitch, str_x, s0, K.str_rows, str_pitch, i, j, tid, threads, x);
 				if (!mykind) continue;
 #pragma unroll
 				for (int half = 0; half < TB / 4; half++) {
@@ -1204,15 +1228,27 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 #pragma unroll
 					for (int bb = 0; bb < 4; bb++) {
 						const int b = 4 * half + bb, r = j + 8 * b;
-						const float s = (float)(K.str_place0 + s0 + r - my_lo - i), sl = OWNK ? slse[r] : 0.f;
+						const float sl = OWNK ? slse[r] : 0.f;
 #pragma unroll
 						for (int a = 0; a < 4; a++) {
 							float fac;
-							const float c = score<ST, CAP>(x[a][b], A.cap, A.icap, fac);
-							p[a][bb] = weight<ST>(__builtin_fmaf(-slope, __builtin_fabsf(s - 8.f * a), c) - (OWNK ? sl : olse[a]));
-							pf[a][bb] = CAP ? fac * A.rw : A.rw;
+							p[a][bb] = score<ST, CAP>(x[a][b], A.cap, A.icap, fac) - (OWNK ? sl : olse[a]);
+							pf[a][bb] = (CAP ? fac : 1.f) * grw;
 						}
 					}
+					if (slope != 0.f) {
+						asm volatile("");  // a branch
+#pragma unroll
+						for (int bb = 0; bb < 4; bb++) {
+							const float s = (float)(K.str_place0 + s0 + j + 8 * (4 * half + bb) - my_lo - i);
+#pragma unroll
+							for (int a = 0; a < 4; a++) p[a][bb] = __builtin_fmaf(-slope, __builtin_fabsf(s - 8.f * a), p[a][bb]);
+						}
+					}
+#pragma unroll
+					for (int bb = 0; bb < 4; bb++)
+#pragma unroll
+						for (int a = 0; a < 4; a++) p[a][bb] = weight<ST>(p[a][bb]);
 					if (mykind == 2) {
 						asm volatile("");  // a branch, as in the forward
 #pragma unroll
