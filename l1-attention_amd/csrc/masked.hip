@@ -46,33 +46,35 @@ L1MaskedArgs args_of(const l1attn_masked_desc* d, const void* q, const void* k, 
 
 const L1MaskedTable& table_of(int dtype) { return dtype == 0 ? l1_masked_f32() : dtype == 1 ? l1_masked_f16() : l1_masked_bf16(); }
 
-// Workgroups of up to eight waves share what they stage; a compute unit has 160 KB of LDS, and 256 of them want work.  So: the
-// largest workgroup that fits LDS and still gives each compute unit one, then as many splits of the other side as fill
-// two for each, none of them with fewer than two tiles.
-L1MaskedPlan plan_of(const L1MaskedTable& t, int64_t owners, int64_t stream, int64_t heads, int W, int Wv, bool backward, bool weigh)
+// Waves of a workgroup share what they stage; a compute unit has 160 KB of LDS, and 256 of them want work.  16-bit rows: four
+// waves, of which two workgroups fit a compute unit and work while the other one waits (eight in one: 263 instead of 218 us for
+// the forward of B1 T4096 H16 W64 with documents); float32: eight where they leave no unit idle, since one workgroup fits either way.
+// Then as many splits of the other side's tiles as make 1024 workgroups, which also evens out what masks leave to do (the two
+// backward kernels of the same shape: 1.90 ms with 512, 1.28 with 1024, 1.21 with 2048, where shorter ones lose more than that:
+// the forward of B2 T1024 S2048 H16/4 W64 takes 168, 156 and 171 us), none of them with fewer than two tiles of 64.
+L1MaskedPlan plan_of(const L1MaskedTable& t, int64_t owners, int64_t stream, int64_t heads, const l1attn_masked_desc* d, bool backward, bool weigh)
 {
 	L1MaskedPlan p;
-	const bool wide = W > 64 || Wv > 64;
-	p.waves = wide || t.lds(64, 64, 1, false, false) < 26000 ? 4 : 8;
+	const int W = (int)d->W, Wv = (int)d->Wv;
+	p.waves = d->dtype == 0 && W <= 64 && Wv <= 64 ? 8 : 4;
 	while (p.waves > 2 && (t.lds(W, Wv, p.waves, backward, weigh) > 160 * 1024 || heads * l1_cdiv(owners, 32 * p.waves) < 256)) p.waves >>= 1;
-	const int64_t groups = heads * l1_cdiv(owners, 32 * p.waves), tiles = l1_cdiv(stream, 64);
-	int64_t s = l1_cdiv(1024, groups);
-	if (s > tiles / 2) s = tiles / 2;
+	int64_t s = l1_cdiv(1024, heads * l1_cdiv(owners, 32 * p.waves));
+	if (s > l1_cdiv(stream, 64) / 2) s = l1_cdiv(stream, 64) / 2;
 	p.splits = (int)(s < 1 ? 1 : s > 16 ? 16 : s);
 	return p;
 }
 
 L1MaskedPlan plan_fwd(const l1attn_masked_desc* d)
 {
-	return plan_of(table_of(d->dtype), d->T, d->S, d->B * d->H, (int)d->W, (int)d->Wv, false, true);
+	return plan_of(table_of(d->dtype), d->T, d->S, d->B * d->H, d, false, true);
 }
 L1MaskedPlan plan_q(const l1attn_masked_desc* d)
 {
-	return plan_of(table_of(d->dtype), d->T, d->S, d->B * d->H, (int)d->W, (int)d->Wv, true, false);
+	return plan_of(table_of(d->dtype), d->T, d->S, d->B * d->H, d, true, false);
 }
 L1MaskedPlan plan_k(const l1attn_masked_desc* d)
 {
-	return plan_of(table_of(d->dtype), d->S, d->T, d->B * d->Hk, (int)d->W, (int)d->Wv, true, true);
+	return plan_of(table_of(d->dtype), d->S, d->T, d->B * d->Hk, d, true, true);
 }
 
 }  // namespace
@@ -83,7 +85,7 @@ size_t l1attn_masked_fwd_workspace_bytes(const l1attn_masked_desc* desc)
 {
 	if (check_desc(desc)) return 0;
 	const L1MaskedPlan p = plan_fwd(desc);
-	return p.splits > 1 ? (size_t)p.splits * desc->B * desc->T * desc->H * (desc->Wv + 1) * sizeof(float) : 0;
+	return p.splits > 1 ? (size_t)p.splits * desc->B * desc->T * desc->H * ((desc->Wv + 3) / 4 * 4 + 1) * sizeof(float) : 0;
 }
 
 int l1attn_masked_fwd(const l1attn_masked_desc* desc, const void* q, const void* k, const void* v, void* o, float* lse, void* workspace,

@@ -806,7 +806,8 @@ __device__ __forceinline__ float weight(float x)
 
 // NB: 16-column blocks of the value width held by a wave.  Grid: x = batch * head (heads next to each other go to different
 // XCDs and one head's tiles to one), y = owner tiles, the last first: under causality it has the most to do; z = splits: split
-// z takes every gridDim.z-th tile of the stream.  part: NULL, or [splits][B][T][H][Wv + 1] sums to be joined, weights' sum last.
+// z takes every gridDim.z-th tile of the stream.  part: NULL, or [splits][B][T][H][Wv up to a multiple of 4] sums to be
+// joined, and behind them the weights' sums [splits][B][T][H].
 template <typename ST, bool CAP, int NB, int TB, int THREADS>
 __global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* __restrict__ q, const ST* __restrict__ k,
                                                       const ST* __restrict__ v, ST* __restrict__ o, float* __restrict__ lse, float* __restrict__ part)
@@ -958,16 +959,19 @@ __global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* 
 		const float d = sc[16 * tb + l16] * (1.f / kWeight<ST>);
 		if (t >= A.T) continue;
 		const int64_t row = ((int64_t)K.b * A.T + t) * A.H + K.h;
-		float* to = part ? part + (blockIdx.z * rows + row) * (A.Wv + 1) : nullptr;
+		const int wp = (A.Wv + 3) & ~3;
+		float* to = part ? part + (blockIdx.z * rows + row) * wp : nullptr;
 		const float r = (part ? 1.f : 1.f / (1.f + d)) * (1.f / kWeight<ST>);
 		if (g == 0) {
-			if (part) to[A.Wv] = d;
+			if (part) part[gridDim.z * rows * wp + blockIdx.z * rows + row] = d;
 			else if (lse) lse[row] = log1pf(d);
 		}
 #pragma unroll
 		for (int wb = 0; wb < NB; wb++) {
 			const int w = 16 * wb + 4 * g;
-			if (!part && k16<ST> && A.vec & 8 && w + 4 <= A.Wv) {
+			if (part) {
+				if (w < wp) *reinterpret_cast<f4*>(to + w) = out[tb][wb] * r;
+			} else if (k16<ST> && A.vec & 8 && w + 4 <= A.Wv) {
 				ST h[4];
 #pragma unroll
 				for (int e = 0; e < 4; e++) h[e] = (ST)(out[tb][wb][e] * r);
@@ -977,10 +981,7 @@ __global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* 
 			} else {
 #pragma unroll
 				for (int e = 0; e < 4; e++)
-					if (w + e < A.Wv) {
-						if (part) to[w + e] = out[tb][wb][e] * r;
-						else o[row * A.Wv + w + e] = (ST)(out[tb][wb][e] * r);
-					}
+					if (w + e < A.Wv) o[row * A.Wv + w + e] = (ST)(out[tb][wb][e] * r);
 			}
 		}
 	}
@@ -991,11 +992,11 @@ __global__ void __launch_bounds__(256) masked_fwd_join(const float* __restrict__
 {
 	const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
 	if (row >= rows) return;
-	const int lane = threadIdx.x & 63;
+	const int lane = threadIdx.x & 63, wp = (Wv + 3) & ~3;
 	float d = 0.f, y0 = 0.f, y1 = 0.f;
 	for (int z = 0; z < splits; z++) {
-		const float* p = part + (z * rows + row) * (Wv + 1);
-		d += p[Wv];
+		const float* p = part + (z * rows + row) * wp;
+		d += part[splits * rows * wp + z * rows + row];
 		if (lane < Wv) y0 += p[lane];
 		if (lane + 64 < Wv) y1 += p[lane + 64];
 	}
