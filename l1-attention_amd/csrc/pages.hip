@@ -11,6 +11,7 @@ namespace {
 
 constexpr int kRows = 1024;   // rows of a call: one workgroup looks at all of them
 constexpr int kChunk = 4096;  // pages that a workgroup of the scans looks at
+constexpr int kOne = 4;       // chunks that one workgroup looks at by itself
 
 // inclusive sum over the workgroup's threads (`total`: of all of them); tmp: one int for each wave
 __device__ __forceinline__ int block_scan(int x, int* tmp, int& total)
@@ -33,15 +34,28 @@ __device__ __forceinline__ int block_scan(int x, int* tmp, int& total)
 	return x + before;
 }
 
+// Whether x is among ids[0, b).  Sixteen of them a step, the same ones for all threads: one after the other, each read's latency
+// counts.
+__device__ __forceinline__ bool named_before(const int* ids, int b, int x)
+{
+	bool found = false;
+	for (int c = 0; c < b && !found; c += 16) {
+#pragma unroll
+		for (int u = 0; u < 16; u += 4) {
+			const int4 y = *reinterpret_cast<const int4*>(ids + c + u);
+			found |= (c + u < b && y.x == x) | (c + u + 1 < b && y.y == x) | (c + u + 2 < b && y.z == x) | (c + u + 3 < b && y.w == x);
+		}
+	}
+	return found;
+}
+
 // The row that entry b of a call names, or -1: out of range, or named before.  ids: one int for each row, filled here.
 __device__ __forceinline__ int named_once(const int32_t* seqs, int b, int B, int rows, int* ids)
 {
 	const int s = b < B ? (seqs ? seqs[b] : b) : -1;
-	if (b < kRows) ids[b] = s;
+	ids[b] = s;
 	__syncthreads();
-	bool ok = b < B && s >= 0 && s < rows;
-	for (int c = 0; ok && c < b; c++) ok = ids[c] != s;
-	return ok ? s : -1;
+	return b < B && s >= 0 && s < rows && !(seqs && named_before(ids, b, s)) ? s : -1;
 }
 
 // What an append() takes, by one workgroup, a thread for each of its rows: where each row's tokens go and which pages they get.
@@ -50,7 +64,7 @@ __device__ __forceinline__ int named_once(const int32_t* seqs, int b, int B, int
 __global__ void __launch_bounds__(kRows) cache_take(L1Cache C, const int32_t* __restrict__ seqs, const int32_t* __restrict__ counts, int B, int n,
                                                     int J, uint8_t* __restrict__ served, int4* __restrict__ plan, int32_t* __restrict__ take)
 {
-	__shared__ int ids[kRows], first[kRows], held[kRows], fresh_page[kRows];
+	__shared__ __align__(16) int ids[kRows], first[kRows], held[kRows], fresh_page[kRows];
 	__shared__ int tmp[16];
 	const int b = threadIdx.x;
 	const int s = named_once(seqs, b, B, C.rows, ids);
@@ -105,7 +119,7 @@ __global__ void __launch_bounds__(kRows) cache_take(L1Cache C, const int32_t* __
 	first[b] = share ? last : -1;
 	__syncthreads();
 	bool freed = share && __hip_atomic_load(&C.refs[last], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0;
-	for (int c = 0; freed && c < b; c++) freed = first[c] != last;
+	freed = freed && !named_before(first, b, last);
 	held[b] = freed ? last : -1;
 	__syncthreads();
 	int gone;
@@ -122,7 +136,7 @@ __global__ void __launch_bounds__(kRows) cache_take(L1Cache C, const int32_t* __
 __global__ void __launch_bounds__(kRows) cache_fork(L1Cache C, const int32_t* __restrict__ parents, const int32_t* __restrict__ children, int B,
                                                     uint8_t* __restrict__ served, int32_t* __restrict__ held)
 {
-	__shared__ int ids[kRows];
+	__shared__ __align__(16) int ids[kRows];
 	const int b = threadIdx.x;
 	const int child = named_once(children, b, B, C.rows, ids);
 	const int parent = b < B ? parents[b] : -1;
@@ -223,11 +237,38 @@ __global__ void __launch_bounds__(kRows) cache_push(L1Cache C, const int32_t* __
 	if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) *top_after = min(top + before + total, C.N);
 }
 
+// The same by one workgroup, chunk after chunk, instead of three launches, for pools of up to kOne chunks.
+__global__ void __launch_bounds__(kRows) cache_push_one(L1Cache C, int chunks)
+{
+	__shared__ int tmp[16];
+	int top = min(max(*C.n_free, 0), C.N);
+	for (int chunk = 0; chunk < chunks; chunk++) {
+		const int p0 = chunk * kChunk + threadIdx.x * (kChunk / kRows);
+		int flag[kChunk / kRows], n = 0, total;
+#pragma unroll
+		for (int u = 0; u < kChunk / kRows; u++) {
+			flag[u] = p0 + u < C.N && C.refs[p0 + u] == -1;
+			n += flag[u];
+		}
+		int at = top + block_scan(n, tmp, total) - n;
+#pragma unroll
+		for (int u = 0; u < kChunk / kRows; u++)
+			if (flag[u]) {
+				C.refs[p0 + u] = 0;
+				if (at < C.N) C.free[at] = p0 + u;
+				at++;
+			}
+		top = min(top + total, C.N);
+	}
+	__syncthreads();
+	if (threadIdx.x == 0) *C.n_free = top;
+}
+
 __global__ void cache_copy_int(int32_t* to, const int32_t* from) { *to = *from; }
 
 // compact(), first part: the pages in use in ascending order (live), the holes before n_live, and the free stack that is left.
 __global__ void __launch_bounds__(kRows) cache_order(L1Cache C, const int32_t* __restrict__ counts, int chunks, int32_t* __restrict__ live,
-                                                     int32_t* __restrict__ holes, int32_t* __restrict__ map, int32_t* __restrict__ sums)
+                                                     int32_t* __restrict__ holes, int32_t* __restrict__ map, int32_t* __restrict__ sums, int32_t* __restrict__ how_many)
 {
 	__shared__ int tmp[16];
 	const int before = sum_before(counts, blockIdx.x, tmp), n_live = sum_before(counts, chunks, tmp);
@@ -251,6 +292,7 @@ __global__ void __launch_bounds__(kRows) cache_order(L1Cache C, const int32_t* _
 	}
 	if (blockIdx.x == 0 && threadIdx.x == 0) {
 		sums[0] = n_live;
+		*how_many = n_live;
 		if (n_live == C.N) sums[1] = 0;
 		*C.n_free = C.N - n_live;
 	}
@@ -296,7 +338,7 @@ template <typename ST> __device__ __forceinline__ float value(ST x) { return (fl
 // Tokens into pages: a workgroup for each page of each row and head, keys (z 0) and values (z 1).  The page's scale becomes
 // the larger of what it was (if it held tokens) and the new tokens' largest magnitude over 127; if it grew, or the page is a
 // copy of a shared one, the codes that were there are written again.  A value that is not finite does not count for the
-// scale: infinities are coded as +-127, NaN as 0.  G: elements a thread holds side by side (4 where the width allows it).
+// scale: infinities are coded as +-127, NaN as 0.  G: elements a thread holds side by side.
 template <typename ST, int G>
 __global__ void __launch_bounds__(256) cache_write(L1Cache C, const ST* __restrict__ kx, const ST* __restrict__ vx, int n, int J,
                                                    const int4* __restrict__ plan, const int32_t* __restrict__ take)
@@ -329,11 +371,16 @@ __global__ void __launch_bounds__(256) cache_write(L1Cache C, const ST* __restri
 		const int t = at / groups, w = (at % groups) * G, place = base + t;
 		if (place < start || place >= end) continue;
 		const ST* row = x + (((int64_t)r * n + place - start) * C.Hk + h) * W;
+		ST in[G];
+		if (w < W) {
+			if constexpr (G > 1) __builtin_memcpy(in, __builtin_assume_aligned(row + w, 16), sizeof(in));
+			else in[0] = row[w];
+		}
 #pragma unroll
 		for (int e = 0; e < G; e++) {
-			val[u][e] = w + e < W ? value(row[w + e]) : 0.f;
+			val[u][e] = w < W ? value(in[e]) : 0.f;
 			const float m = __builtin_fabsf(val[u][e]);
-			if (m <= 3.402823466e38f) top = fmaxf(top, m);
+			top = m <= 3.402823466e38f ? fmaxf(top, m) : top;
 		}
 	}
 #pragma unroll
@@ -371,9 +418,10 @@ __global__ void __launch_bounds__(256) cache_write(L1Cache C, const ST* __restri
 template <typename ST>
 int write_tokens(const L1Cache& C, const void* k, const void* v, int B, int n, int J, const int4* plan, const int32_t* take, hipStream_t st)
 {
-	// four elements side by side wherever both widths are whole fours (rows of the inputs then start on whole fours too)
+	// eight elements side by side, whole vectors, where both widths are whole eights and the inputs start on 16 bytes
 	const dim3 grid((unsigned)(B * J), (unsigned)C.Hk, 2);
-	if (C.W % 4 == 0 && C.Wv % 4 == 0) hipLaunchKernelGGL((cache_write<ST, 4>), grid, dim3(256), 0, st, C, (const ST*)k, (const ST*)v, n, J, plan, take);
+	if (C.W % 8 == 0 && C.Wv % 8 == 0 && !(((uintptr_t)k | (uintptr_t)v) & 15))
+		hipLaunchKernelGGL((cache_write<ST, 8>), grid, dim3(256), 0, st, C, (const ST*)k, (const ST*)v, n, J, plan, take);
 	else hipLaunchKernelGGL((cache_write<ST, 1>), grid, dim3(256), 0, st, C, (const ST*)k, (const ST*)v, n, J, plan, take);
 	L1_LAUNCH_CHECK();
 	return L1ATTN_OK;
@@ -456,6 +504,11 @@ int l1attn_cache_free(const l1attn_cache* cache, const int32_t* seqs, const int3
 	int32_t* counts = (int32_t*)workspace;
 	hipLaunchKernelGGL(cache_drop, dim3((unsigned)B), dim3(256), 0, st, C, seqs, keep, (int)B);
 	L1_LAUNCH_CHECK();
+	if (chunks <= kOne) {
+		hipLaunchKernelGGL(cache_push_one, dim3(1), dim3(kRows), 0, st, C, (int)chunks);
+		L1_LAUNCH_CHECK();
+		return L1ATTN_OK;
+	}
 	hipLaunchKernelGGL(cache_count<true>, dim3(chunks), dim3(kRows), 0, st, C, counts);
 	L1_LAUNCH_CHECK();
 	hipLaunchKernelGGL(cache_push, dim3(chunks), dim3(kRows), 0, st, C, counts, C.n_free, counts + chunks);
@@ -488,7 +541,7 @@ int l1attn_cache_compact(const l1attn_cache* cache, int32_t* live, void* workspa
 	if (C.N == 0) return L1ATTN_ERR_ARG;
 	hipLaunchKernelGGL(cache_count<false>, dim3(chunks), dim3(kRows), 0, st, C, counts);
 	L1_LAUNCH_CHECK();
-	hipLaunchKernelGGL(cache_order, dim3(chunks), dim3(kRows), 0, st, C, counts, (int)chunks, order, holes, map, sums);
+	hipLaunchKernelGGL(cache_order, dim3(chunks), dim3(kRows), 0, st, C, counts, (int)chunks, order, holes, map, sums, live);
 	L1_LAUNCH_CHECK();
 	hipLaunchKernelGGL(cache_move, dim3(2048), dim3(256), 0, st, C, order, holes, map, sums);
 	L1_LAUNCH_CHECK();
@@ -496,8 +549,6 @@ int l1attn_cache_compact(const l1attn_cache* cache, int32_t* live, void* workspa
 		hipLaunchKernelGGL(cache_rename, dim3((unsigned)l1_cdiv((int64_t)C.rows * C.M, 256)), dim3(256), 0, st, C, map);
 		L1_LAUNCH_CHECK();
 	}
-	hipLaunchKernelGGL(cache_copy_int, dim3(1), dim3(1), 0, st, live, sums);
-	L1_LAUNCH_CHECK();
 	return L1ATTN_OK;
 }
 
