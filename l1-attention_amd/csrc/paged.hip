@@ -8,187 +8,376 @@
 // order.  A workgroup takes 256 tokens at a time: a lane holds one token's key row and forms the distances of all rows
 // (the rows' values are broadcast LDS reads); then a lane holds 16 value columns of every 16th token and adds p * v.
 // The bytes of the cache are read once and are what bounds it for few rows; with many rows it is the vector ALU.
+// paged_attend: up to 4 rows, and float32; paged_attend_rows: more rows of 16 bits.
 #include "paged.h"
 #include <math.h>
+#include <type_traits>
 
 namespace {
 
-constexpr int kTok = 256;  // tokens of a step, one for each thread
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+
+constexpr int kTok = 512;  // least tokens of a split
 
 struct AttendArgs {
 	L1Cache C;
-	int B, n, H, G, splits;
+	int B, n, H, G, splits, chunk, parts;
 	float cap, icap, rw;
 	int has_slopes;
 	float slopes[256];
 };
 
-// the tokens [lo, hi) of a split: whole steps, spread evenly; the same in the join
-__device__ __forceinline__ int split_tokens(int len, int splits)
+// Tokens of a split, the same in the join: the sequence in A.parts, whole kTok of them, at most the call's chunk.
+__device__ __forceinline__ int split_tokens(const AttendArgs& A, int len)
 {
-	const int per = (len + splits - 1) / splits;
-	return (per + kTok - 1) / kTok * kTok;
+	const int per = ((len + A.parts - 1) / A.parts + kTok - 1) / kTok * kTok;
+	return min(max(per, kTok), A.chunk);
 }
-
-template <typename ST> __device__ __forceinline__ float value(ST x) { return (float)x; }
 
 // length of entry b's sequence, 0 where it names none
 __device__ __forceinline__ int seq_of(const AttendArgs& A, const int32_t* seqs, int b, int& s)
 {
 	s = seqs ? seqs[b] : b;
-	if (s < 0 || s >= A.C.rows) return 0;
+	if (s < 0 || s >= A.C.rows || A.C.N < 1) return 0;
 	return min(max(A.C.lens[s], 0), A.C.M * A.C.P);
 }
 
-// RB: rows of a workgroup.  Grid: splits, batch * key heads, blocks of rows.
-// part: [splits][B][n][H][Wv + 1] (the last: the weights' sum), or NULL with one split, which writes o itself.
-template <typename ST, int RB>
-__global__ void __launch_bounds__(256) paged_attend(AttendArgs A, const ST* __restrict__ q, const int32_t* __restrict__ seqs,
-                                                    const int32_t* __restrict__ counts, ST* __restrict__ o, float* __restrict__ part)
+// One 16-byte piece of codes as float32.
+__device__ __forceinline__ void codes4(int word, float (&x)[4])
 {
-	constexpr int RP = RB < 4 ? RB : RB + 4;  // floats between two tokens' weights
+	x[0] = (float)(int8_t)word;
+	x[1] = (float)(int8_t)(word >> 8);
+	x[2] = (float)(int8_t)(word >> 16);
+	x[3] = (float)(word >> 24);
+}
+
+// One 16-bit or float32 logit's weight exp(c(a) - slope * dist), a <= 0.
+template <typename ST> __device__ __forceinline__ float weight(const AttendArgs& A, float a, float slope, float dist)
+{
+	if constexpr (sizeof(ST) == 4) {
+		if (A.cap > 0.f) a = A.cap * tanhf(a * A.icap);
+		return expf(a - slope * dist);
+	} else {
+		if (A.cap > 0.f) {
+			const float e = __builtin_amdgcn_exp2f(a * (2.885390082f * A.icap));
+			a = A.cap * (e - 1.f) * __builtin_amdgcn_rcpf(e + 1.f);
+		}
+		return __builtin_amdgcn_exp2f(1.442695041f * (a - slope * dist));
+	}
+}
+
+// RB rows of a workgroup.  Grid: splits, batch * key heads, blocks of rows.  part: [splits][B][n][H][Wv + 1] (the last: the
+// weights' sum), or NULL with one split, which writes o itself.
+// Each of the four waves takes 64 U tokens of its own at a time and waits for no other: a lane holds U tokens against all rows,
+// whose values are broadcast LDS reads; the weights pass through the wave's own piece of LDS into the layout of the matrix
+// instructions, which add up weight * value.  A step's loads are on their way together: the next step's pages, keys, values.
+template <typename ST, int RB, int NC, int MINW>
+__global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST* __restrict__ q, const int32_t* __restrict__ seqs,
+                                                          const int32_t* __restrict__ counts, ST* __restrict__ o, float* __restrict__ part)
+{
+	constexpr bool F32 = sizeof(ST) == 4, CODED = !F32 && RB >= 8;
+	constexpr int U = RB <= 2 ? 1 : 2, VG = NC / 4, KB = RB >= 8 ? 2 : 4;  // KB: pieces of 16 bytes of a key row under way
+	constexpr int pitch = 64 * U + (F32 ? 4 : 8);                          // between two rows' weights: an odd number of 16-byte pieces
+	using PT = std::conditional_t<F32, float, _Float16>;
+	constexpr int pool = 4 * RB * pitch * (int)sizeof(PT), join = 2 * RB * 128 * 4;
 	__shared__ __align__(16) float qs[RB * 128];
-	__shared__ __align__(16) float ps[kTok * RP];
-	__shared__ float vscale[kTok];
-	__shared__ int vpage[kTok];
+	__shared__ __align__(16) unsigned qc[CODED ? RB * 64 : 1];
+	__shared__ __align__(16) char shared_pool[pool > join ? pool : join];
+	__shared__ float red[8], dens[4 * RB];
 	const L1Cache& C = A.C;
-	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g = lane >> 4;
 	const int b = blockIdx.y / C.Hk, hk = blockIdx.y % C.Hk, r0 = blockIdx.z * RB, R = A.n * A.G;
 	int s;
 	const int len = seq_of(A, seqs, b, s);
 	const int cnt = counts ? min(max(counts[b], 0), A.n) : A.n;
-	const int per = split_tokens(len, A.splits), lo = blockIdx.x * per, hi = min(lo + per, len);
+	const int per = split_tokens(A, len), lo = min((int64_t)blockIdx.x * per, (int64_t)len), hi = min(lo + per, len);
 	if (lo >= hi && part) return;  // the join knows which splits there are
-	// the rows' values, zero behind the width: the cache's rows are zero there as well
-	for (int x = tid; x < RB * C.pk; x += 256) {
-		const int r = r0 + x / C.pk, w = x % C.pk;
-		const int t = r / A.G, h = hk * A.G + r % A.G;
-		qs[(x / C.pk) * 128 + w] = r < R && w < C.W ? value(q[(((int64_t)b * A.n + t) * A.H + h) * C.W + w]) : 0.f;
-	}
-	float slope[RB];
-	int place[RB];
-#pragma unroll
-	for (int r = 0; r < RB; r++) {
-		const int t = (r0 + r) / A.G;
-		slope[r] = A.has_slopes && r0 + r < R ? A.slopes[hk * A.G + (r0 + r) % A.G] : 0.f;
-		place[r] = r0 + r < R && t < cnt ? len - cnt + t : -1;  // sees nothing
-	}
-	const int vchunks = C.pv / 16;           // lanes of a value row
-	const int vtok = 64 / vchunks;           // tokens that a wave reads at once
-	const int vc = lane % vchunks, vt = lane / vchunks;
-	const bool vlane = vt < vtok;
-	float acc[RB][16], den[RB];
-#pragma unroll
-	for (int r = 0; r < RB; r++) {
-		den[r] = 0.f;
-#pragma unroll
-		for (int e = 0; e < 16; e++) acc[r][e] = 0.f;
-	}
 	const int32_t* table = C.table + (int64_t)s * C.M;
-	for (int t0 = lo; t0 < hi; t0 += kTok) {
-		__syncthreads();
-		const int t = t0 + tid;
-		const int page = t < hi ? table[t / C.P] : -1;
-		const bool there = page >= 0 && page < C.N;
-		const int64_t at = there ? ((int64_t)page * C.Hk + hk) : 0;
-		float dist[RB];
+	const int psh = C.P == 16 ? 4 : C.P == 32 ? 5 : 6;  // a page's tokens are 16, 32 or 64
+	int page[U];
+	const int first = lo + 64 * U * wave + lane;
 #pragma unroll
-		for (int r = 0; r < RB; r++) dist[r] = 0.f;
-		const float ks = there ? C.ks[at] : 0.f;
-		vscale[tid] = there ? C.vs[at] : 0.f;
-		vpage[tid] = there ? page : -1;
-		if (there) {
-			const int8_t* row = C.k + (at * C.P + t % C.P) * C.pk;
-			for (int w = 0; w < C.pk; w += 16) {
-				const uint4 raw = *reinterpret_cast<const uint4*>(row + w);
-				const int word[4] = {(int)raw.x, (int)raw.y, (int)raw.z, (int)raw.w};
+	for (int u = 0; u < U; u++) page[u] = first + 64 * u < hi ? table[(first + 64 * u) >> psh] : -1;
+	// the rows' values, zero behind the width: the cache's rows are zero there as well
+	float least = 0.f, most = 0.f;
+	bool finite = true;
+	for (int x = tid; x < RB * C.pk; x += 256) {
+		const int rr = x / C.pk, r = r0 + rr, w = x - rr * C.pk;
+		const int t = r / A.G, h = hk * A.G + r - t * A.G;
+		const float y = r < R && w < C.W ? (float)q[(((int64_t)b * A.n + t) * A.H + h) * C.W + w] : 0.f;
+		qs[rr * 128 + w] = y;
+		finite &= __builtin_fabsf(y) <= 3.402823466e38f;
+		least = fminf(least, y);
+		most = fmaxf(most, y);
+	}
+	bool coded = false;
+	float sc = 0.f, off = 0.f, m = A.rw;
+	if constexpr (CODED) {
+		// the grid: over the rows' values and over what the pages' scales allow
+		float kmax = 0.f;
+		for (int j = (lo >> psh) + tid; j << psh < hi; j += 256) {
+			const int pg = table[j];
+			if (pg < 0 || pg >= C.N) continue;
+			const float y = C.ks[(int64_t)pg * C.Hk + hk];
+			finite &= __builtin_fabsf(y) <= 3.402823466e38f;
+			kmax = fmaxf(kmax, __builtin_fabsf(y));
+		}
+		least = fminf(least, -127.f * kmax);
+		most = fmaxf(most, 127.f * kmax);
 #pragma unroll
-				for (int d = 0; d < 4; d++) {
-					const float k0 = (float)(int8_t)word[d], k1 = (float)(int8_t)(word[d] >> 8), k2 = (float)(int8_t)(word[d] >> 16), k3 = (float)(word[d] >> 24);
+		for (int k = 32; k; k >>= 1) {
+			least = fminf(least, __shfl_xor(least, k));
+			most = fmaxf(most, __shfl_xor(most, k));
+		}
+		if (lane == 0) { red[2 * wave] = least; red[2 * wave + 1] = most; }
+		finite = !__syncthreads_or(!finite);
 #pragma unroll
-					for (int r = 0; r < RB; r++) {
-						const float4 qv = *reinterpret_cast<const float4*>(qs + r * 128 + w + 4 * d);
-						dist[r] += __builtin_fabsf(__builtin_fmaf(-k0, ks, qv.x));
-						dist[r] += __builtin_fabsf(__builtin_fmaf(-k1, ks, qv.y));
-						dist[r] += __builtin_fabsf(__builtin_fmaf(-k2, ks, qv.z));
-						dist[r] += __builtin_fabsf(__builtin_fmaf(-k3, ks, qv.w));
+		for (int w = 0; w < 4; w++) { least = fminf(least, red[2 * w]); most = fmaxf(most, red[2 * w + 1]); }
+		const float span = (most - least) * (1.f + 0x1p-19f);
+		coded = finite && span > 1e-30f && span <= (std::is_same_v<ST, _Float16> ? 24.f : 160.f);
+		sc = coded ? 1.f / span : 0.f;
+		off = coded ? -(least - (most - least) * 0x1p-20f) * sc : 0.f;
+		if (coded) {
+			m = span * (1.f / 65535.f) * A.rw;
+			for (int x = tid; x < RB * (C.pk / 2); x += 256) {
+				const int rr = x / (C.pk / 2), w = x - rr * (C.pk / 2);
+				qc[rr * 64 + w] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pknorm_u16(__builtin_fmaf(qs[rr * 128 + 2 * w], sc, off),
+				                                                                             __builtin_fmaf(qs[rr * 128 + 2 * w + 1], sc, off)));
+			}
+		}
+	}
+	__syncthreads();
+	PT* ps = reinterpret_cast<PT*>(shared_pool) + wave * RB * pitch;
+	const int kchunks = C.pk / 16;
+	float den[RB];
+	f4 acc[VG][4];
+#pragma unroll
+	for (int r = 0; r < RB; r++) den[r] = 0.f;
+#pragma unroll
+	for (int wg = 0; wg < VG; wg++)
+#pragma unroll
+		for (int e = 0; e < 4; e++) acc[wg][e] = (f4)(0.f);
+	for (int t0 = lo + 64 * U * wave; t0 < hi; t0 += 256 * U) {
+		float ks[U], vs[U];
+		bool there[U];
+		const int8_t* krow[U];
+		int pg[U];
+		uint4 kr[U][KB];
+#pragma unroll
+		for (int u = 0; u < U; u++) {
+			const int t = t0 + 64 * u + lane;
+			there[u] = page[u] >= 0 && page[u] < C.N;
+			pg[u] = there[u] ? page[u] : 0;
+			const int64_t at = (int64_t)pg[u] * C.Hk + hk;
+			krow[u] = C.k + ((at << psh) + (t & (C.P - 1))) * C.pk;
+#pragma unroll
+			for (int c = 0; c < KB; c++) kr[u][c] = *reinterpret_cast<const uint4*>(krow[u] + 16 * min(c, kchunks - 1));
+			ks[u] = there[u] ? C.ks[at] : 0.f;
+			vs[u] = there[u] ? C.vs[at] : 0.f;
+			page[u] = t + 256 * U < hi ? table[(t + 256 * U) >> psh] : -1;
+		}
+		// the values: for 16 bits eight tokens in a row of every 32, for float32 four of every 16, four columns each
+		constexpr int VT = F32 ? 4 : 8;
+		unsigned vr[16 * U / VT][VG][VT];
+#pragma unroll
+		for (int kc = 0; kc < 16 * U / VT; kc++) {
+			const int tok = 4 * VT * kc + VT * g;
+			const int vp = __shfl(pg[kc * 4 * VT / 64], tok & 63);
+			const int8_t* row = C.v + ((((int64_t)vp * C.Hk + hk) << psh) + ((t0 + tok) & (C.P - 1))) * C.pv;
+#pragma unroll
+			for (int wg = 0; wg < VG; wg++)
+#pragma unroll
+				for (int e = 0; e < VT; e++)
+					vr[kc][wg][e] = *reinterpret_cast<const unsigned*>(row + e * C.pv + min(64 * wg + 4 * l16, C.pv - 4));
+		}
+		float dist[U][RB];
+		if (coded) {
+			unsigned sum[U][RB];
+#pragma unroll
+			for (int u = 0; u < U; u++)
+#pragma unroll
+				for (int r = 0; r < RB; r++) sum[u][r] = 0;
+#pragma unroll 1
+			for (int c0 = 0; c0 < kchunks; c0 += KB) {
+#pragma unroll
+				for (int i = 0; i < KB; i++) {
+					const int c = c0 + i;
+					unsigned kc[U][8];
+#pragma unroll
+					for (int u = 0; u < U; u++) {
+						const uint4 raw = kr[u][i];
+						kr[u][i] = *reinterpret_cast<const uint4*>(krow[u] + 16 * min(c + KB, kchunks - 1));
+						const int word[4] = {(int)raw.x, (int)raw.y, (int)raw.z, (int)raw.w};
+						const float f = ks[u] * sc;
+#pragma unroll
+						for (int d = 0; d < 4; d++) {
+							float x[4];
+							codes4(word[d], x);
+							kc[u][2 * d] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pknorm_u16(__builtin_fmaf(x[0], f, off), __builtin_fmaf(x[1], f, off)));
+							kc[u][2 * d + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pknorm_u16(__builtin_fmaf(x[2], f, off), __builtin_fmaf(x[3], f, off)));
+						}
 					}
+					if (c < kchunks)
+#pragma unroll
+						for (int r = 0; r < RB; r++)
+#pragma unroll
+							for (int h = 0; h < 2; h++) {
+								const uint4 y = *reinterpret_cast<const uint4*>(qc + r * 64 + 8 * c + 4 * h);
+#pragma unroll
+								for (int u = 0; u < U; u++) {
+									unsigned z = sum[u][r];
+									z = __builtin_amdgcn_sad_u16(kc[u][4 * h], y.x, z);
+									z = __builtin_amdgcn_sad_u16(kc[u][4 * h + 1], y.y, z);
+									z = __builtin_amdgcn_sad_u16(kc[u][4 * h + 2], y.z, z);
+									z = __builtin_amdgcn_sad_u16(kc[u][4 * h + 3], y.w, z);
+									sum[u][r] = z;
+								}
+							}
 				}
 			}
+#pragma unroll
+			for (int u = 0; u < U; u++)
+#pragma unroll
+				for (int r = 0; r < RB; r++) dist[u][r] = (float)sum[u][r];
+		} else {
+#pragma unroll
+			for (int u = 0; u < U; u++)
+#pragma unroll
+				for (int r = 0; r < RB; r++) dist[u][r] = 0.f;
+#pragma unroll 1
+			for (int c0 = 0; c0 < kchunks; c0 += KB) {
+#pragma unroll
+				for (int i = 0; i < KB; i++) {
+					const int c = c0 + i;
+					uint4 raw[U];
+#pragma unroll
+					for (int u = 0; u < U; u++) {
+						raw[u] = kr[u][i];
+						kr[u][i] = *reinterpret_cast<const uint4*>(krow[u] + 16 * min(c + KB, kchunks - 1));
+					}
+					if (c < kchunks)
+#pragma unroll
+						for (int d = 0; d < 4; d++) {
+							float k[U][4];
+#pragma unroll
+							for (int u = 0; u < U; u++) {
+								codes4((int)(d == 0 ? raw[u].x : d == 1 ? raw[u].y : d == 2 ? raw[u].z : raw[u].w), k[u]);
+							}
+#pragma unroll
+							for (int r = 0; r < RB; r++) {
+								const float4 y = *reinterpret_cast<const float4*>(qs + r * 128 + 16 * c + 4 * d);
+#pragma unroll
+								for (int u = 0; u < U; u++) {
+									const float d0 = __builtin_fmaf(-k[u][0], ks[u], y.x), d1 = __builtin_fmaf(-k[u][1], ks[u], y.y);
+									const float d2 = __builtin_fmaf(-k[u][2], ks[u], y.z), d3 = __builtin_fmaf(-k[u][3], ks[u], y.w);
+									dist[u][r] += (__builtin_fabsf(d0) + __builtin_fabsf(d1)) + (__builtin_fabsf(d2) + __builtin_fabsf(d3));
+								}
+							}
+						}
+				}
+			}
+		}
+		// float16 weights: 2^14 over the power of two above the largest scale of the step's values, and back
+		float up = 1.f, down = 1.f;
+		if constexpr (!F32) {
+			float most = __builtin_fabsf(vs[0]);
+			if constexpr (U == 2) most = fmaxf(most, __builtin_fabsf(vs[1]));
+#pragma unroll
+			for (int k = 32; k; k >>= 1) most = fmaxf(most, __shfl_xor(most, k));
+			const int ve = most > 0.f ? max(__builtin_amdgcn_frexp_expf(most), -100) : 0;
+			up = __builtin_amdgcn_ldexpf(1.f, 14 - ve);
+			down = __builtin_amdgcn_ldexpf(1.f, ve - 14);
 		}
 #pragma unroll
 		for (int r = 0; r < RB; r++) {
-			float c = -dist[r] * A.rw;
-			if (A.cap > 0.f) c = A.cap * tanhf(c * A.icap);
-			const float p = there && t <= place[r] ? expf(c - slope[r] * (float)(place[r] - t)) : 0.f;
-			den[r] += p;
-			ps[tid * RP + r] = p;
+			const int row = r0 + r, tq = row / A.G, place = row < R && tq < cnt ? len - cnt + tq : -1;  // -1: sees nothing
+			const float slope = A.has_slopes && row < R ? A.slopes[hk * A.G + row - tq * A.G] : 0.f;
+#pragma unroll
+			for (int u = 0; u < U; u++) {
+				const int t = t0 + 64 * u + lane;
+				const float w = weight<ST>(A, -dist[u][r] * m, slope, (float)(place - t));
+				const float p = there[u] && t < hi && t <= place ? w : 0.f;
+				den[r] += p;
+				ps[r * pitch + 64 * u + lane] = (PT)(p != 0.f ? p * (vs[u] * up) : 0.f);  // the scale of a hidden token has no influence
+			}
 		}
-		__syncthreads();
-		// values: wave `wave` takes every fourth group of vtok tokens
-		if (vlane)
-			for (int u = wave * vtok + vt; u < min(kTok, hi - t0); u += 4 * vtok) {
-				const int pg = vpage[u];
-				if (pg < 0) continue;
-				const float vs = vscale[u];
-				const int8_t* row = C.v + (((int64_t)pg * C.Hk + hk) * C.P + (t0 + u) % C.P) * C.pv + 16 * vc;
-				const uint4 raw = *reinterpret_cast<const uint4*>(row);
-				const int word[4] = {(int)raw.x, (int)raw.y, (int)raw.z, (int)raw.w};
-				float x[16];
+		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+		__builtin_amdgcn_wave_barrier();
 #pragma unroll
-				for (int d = 0; d < 4; d++) {
-					x[4 * d] = (float)(int8_t)word[d];
-					x[4 * d + 1] = (float)(int8_t)(word[d] >> 8);
-					x[4 * d + 2] = (float)(int8_t)(word[d] >> 16);
-					x[4 * d + 3] = (float)(word[d] >> 24);
-				}
+		for (int wg = 0; wg < VG; wg++) {
+			f4 y[4];
 #pragma unroll
-				for (int r = 0; r < RB; r++) {
-					const float p = ps[u * RP + r];
-					const float pv = p != 0.f ? p * vs : 0.f;  // the scale of a hidden token has no influence
+			for (int e = 0; e < 4; e++) y[e] = F32 ? acc[wg][e] : (f4)(0.f);
 #pragma unroll
-					for (int e = 0; e < 16; e++) acc[r][e] = __builtin_fmaf(pv, x[e], acc[r][e]);
+			for (int kc = 0; kc < 16 * U / VT; kc++) {
+				const uint4 pa = *reinterpret_cast<const uint4*>(ps + l16 % RB * pitch + 4 * VT * kc + VT * g);
+				if constexpr (F32) {
+					const float a[4] = {__builtin_bit_cast(float, pa.x), __builtin_bit_cast(float, pa.y), __builtin_bit_cast(float, pa.z), __builtin_bit_cast(float, pa.w)};
+#pragma unroll
+					for (int d = 0; d < 4; d++) {
+						float x[4];
+						codes4((int)vr[kc][wg][d], x);
+#pragma unroll
+						for (int e = 0; e < 4; e++) y[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[d], x[e], y[e], 0, 0, 0);
+					}
+				} else {
+#pragma unroll
+					for (int e = 0; e < 4; e++) {
+						unsigned x[4];
+#pragma unroll
+						for (int d = 0; d < 4; d++) {
+							// byte e of two tokens, plus 128, behind the bits of 1024: then without the 1152
+							const unsigned two = __builtin_amdgcn_perm(vr[kc][wg][2 * d + 1] ^ 0x80808080u, vr[kc][wg][2 * d] ^ 0x80808080u, 0x0c040c00u + 0x00010001u * e) | 0x64006400u;
+							const h2 v = __builtin_bit_cast(h2, two) - (h2){(_Float16)1152.f, (_Float16)1152.f};
+							x[d] = __builtin_bit_cast(unsigned, v);
+						}
+						y[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, pa), __builtin_bit_cast(h8, make_uint4(x[0], x[1], x[2], x[3])), y[e], 0, 0, 0);
+					}
 				}
 			}
+#pragma unroll
+			for (int e = 0; e < 4; e++) acc[wg][e] = F32 ? y[e] : acc[wg][e] + y[e] * down;
+		}
+		__builtin_amdgcn_wave_barrier();
 	}
-	// sums over the lanes and waves, in a fixed order, row by row through LDS
+	// rows 4 g + i (a row again every RB), columns 64 wg + 4 l16 + e; over the waves through LDS, where the weights lay
+#pragma unroll
+	for (int r = 0; r < RB; r++) {
+#pragma unroll
+		for (int k = 32; k; k >>= 1) den[r] += __shfl_xor(den[r], k);
+		if (lane == 0) dens[wave * RB + r] = den[r];
+	}
 	__syncthreads();
-	__shared__ float red[4 * 128 + 4];  // a row's columns of each wave, and the sums of its weights
-	for (int r = 0; r < RB; r++) {
+	float* sums = reinterpret_cast<float*>(shared_pool);  // [2 waves][RB][128], in two turns
+	for (int turn = 0; turn < 2; turn++) {
+		if ((wave >> 1) == turn)
 #pragma unroll
-		for (int m = 32; m; m >>= 1) den[r] += __shfl_xor(den[r], m);
+			for (int wg = 0; wg < VG; wg++)
+#pragma unroll
+				for (int i = 0; i < 4; i++) {
+					if (4 * g + i >= RB) continue;
+					float* at = sums + ((wave & 1) * RB + 4 * g + i) * 128 + 64 * wg + 4 * l16;
+					f4 y = {acc[wg][0][i], acc[wg][1][i], acc[wg][2][i], acc[wg][3][i]};
+					if (turn) y += *reinterpret_cast<const f4*>(at);
+					*reinterpret_cast<f4*>(at) = y;
+				}
+		__syncthreads();
 	}
-#pragma unroll
-	for (int r = 0; r < RB; r++) {
-		// each wave's own columns: over its tokens vt
-		float sum[16];
-#pragma unroll
-		for (int e = 0; e < 16; e++) sum[e] = acc[r][e];
-		__syncthreads();
-		for (int step = vtok; step > 1;) {
-			const int half = (step + 1) / 2;
-#pragma unroll
-			for (int e = 0; e < 16; e++) {
-				const float y = __shfl(sum[e], min(lane + half * vchunks, 63));
-				if (vt + half < step) sum[e] += y;
-			}
-			step = half;
-		}
-		if (vlane && vt == 0)
-#pragma unroll
-			for (int e = 0; e < 16; e++) red[wave * 128 + 16 * vc + e] = sum[e];
-		if (lane == 0) red[512 + wave] = den[r];
-		__syncthreads();
-		const int row = r0 + r;
-		if (row < R) {
-			const int64_t out = ((int64_t)b * A.n + row / A.G) * A.H + hk * A.G + row % A.G;
-			const float d = red[512] + red[513] + red[514] + red[515];
-			for (int w = tid; w < C.Wv; w += 256) {
-				const float y = red[w] + red[128 + w] + red[256 + w] + red[384 + w];
-				if (part) part[((int64_t)blockIdx.x * A.B * A.n * A.H + out) * (C.Wv + 1) + w] = y;
-				else o[out * C.Wv + w] = (ST)(y / (1.f + d));
-			}
-			if (part && tid == 0) part[((int64_t)blockIdx.x * A.B * A.n * A.H + out) * (C.Wv + 1) + C.Wv] = d;
+	for (int x = tid; x < RB * C.Wv; x += 256) {
+		const int r = x / C.Wv, w = x - r * C.Wv, row = r0 + r;
+		if (row >= R) continue;
+		const int t = row / A.G;
+		const int64_t out = ((int64_t)b * A.n + t) * A.H + hk * A.G + row - t * A.G;
+		const float d = dens[r] + dens[RB + r] + dens[2 * RB + r] + dens[3 * RB + r];
+		const float y = sums[r * 128 + w] + sums[(RB + r) * 128 + w];
+		if (part) {
+			float* to = part + ((int64_t)blockIdx.x * A.B * A.n * A.H + out) * (C.Wv + 1);
+			to[w] = y;
+			if (w == 0) to[C.Wv] = d;
+		} else {
+			o[out * C.Wv + w] = (ST)(y / (1.f + d));
 		}
 	}
 }
@@ -201,8 +390,9 @@ __global__ void __launch_bounds__(128) paged_join(AttendArgs A, const float* __r
 	const int b = (int)(row / ((int64_t)A.n * A.H));
 	int s;
 	const int len = seq_of(A, seqs, b, s);
-	const int per = split_tokens(len, A.splits), m = len ? (len + per - 1) / per : 0, Wv = A.C.Wv;
+	const int per = split_tokens(A, len), m = len ? (len + per - 1) / per : 0, Wv = A.C.Wv;
 	float d = 1.f, y = 0.f;
+#pragma unroll 8
 	for (int u = 0; u < m; u++) {
 		const float* p = part + ((int64_t)u * rows + row) * (Wv + 1);
 		d += p[Wv];
@@ -211,37 +401,45 @@ __global__ void __launch_bounds__(128) paged_join(AttendArgs A, const float* __r
 	if ((int)threadIdx.x < Wv) o[row * Wv + threadIdx.x] = (ST)(y / d);
 }
 
-// workgroups that a call is split into over the tokens: about four for each of the 256 compute units in all
-int splits_for(const L1Cache& C, int64_t groups)
+// rows of a workgroup
+int row_block(int64_t R) { return R <= 1 ? 1 : R <= 2 ? 2 : R <= 4 ? 4 : R <= 8 ? 8 : 16; }
+
+// Splits of the longest sequence that the table can hold: about 2048 workgroups in all, of 512 tokens at least, and eight where
+// the sequences may be much shorter than that.
+void splits_for(const L1Cache& C, int64_t groups, AttendArgs* A)
 {
-	const int64_t most = l1_cdiv((int64_t)C.M * C.P, kTok), want = l1_cdiv(1024, groups);
-	return (int)(want < 1 ? 1 : want > most ? (most < 1 ? 1 : most) : want);
+	const int64_t tokens = (int64_t)C.M * C.P, most = l1_cdiv(tokens, kTok), want = l1_cdiv(2048, groups);
+	A->chunk = (int)(l1_cdiv(l1_cdiv(tokens, want), kTok) * kTok);
+	if (A->chunk < kTok) A->chunk = kTok;
+	int64_t parts = l1_cdiv(4096, groups);
+	parts = parts > 8 ? 8 : parts;
+	A->parts = (int)(parts > most ? (most < 1 ? 1 : most) : parts);
+	const int64_t n = l1_cdiv(tokens, A->chunk);
+	A->splits = (int)(n > A->parts ? n : A->parts);
 }
 
-int row_block(int64_t R) { return R <= 1 ? 1 : R <= 2 ? 2 : R <= 4 ? 4 : 8; }
-
-template <typename ST, int RB>
-int attend(const AttendArgs& A, const void* q, const int32_t* seqs, const int32_t* counts, void* o, float* part, hipStream_t st)
+template <typename ST>
+int attend(const AttendArgs& A, const void* q, const int32_t* seqs, const int32_t* counts, void* o, float* ws, hipStream_t st)
 {
-	const dim3 grid((unsigned)A.splits, (unsigned)(A.B * A.C.Hk), (unsigned)l1_cdiv((int64_t)A.n * A.G, RB));
-	hipLaunchKernelGGL((paged_attend<ST, RB>), grid, dim3(256), 0, st, A, (const ST*)q, seqs, counts, (ST*)o, A.splits > 1 ? part : nullptr);
+	const int rb = row_block((int64_t)A.n * A.G);
+	const dim3 grid((unsigned)A.splits, (unsigned)(A.B * A.C.Hk), (unsigned)l1_cdiv((int64_t)A.n * A.G, rb));
+	float* part = A.splits > 1 ? ws : nullptr;
+	const bool wide = A.C.pk > 64 || A.C.pv > 64;
+#define L1_ATTEND(RB, MINW)                                                                                                              \
+	if (wide) hipLaunchKernelGGL((paged_attend<ST, RB, 8, 2>), grid, dim3(256), 0, st, A, (const ST*)q, seqs, counts, (ST*)o, part);     \
+	else hipLaunchKernelGGL((paged_attend<ST, RB, 4, MINW>), grid, dim3(256), 0, st, A, (const ST*)q, seqs, counts, (ST*)o, part)
+	if (rb == 1) { L1_ATTEND(1, 4); }
+	else if (rb == 2) { L1_ATTEND(2, 4); }
+	else if (rb == 4) { L1_ATTEND(4, 2); }
+	else if (rb == 8) { L1_ATTEND(8, 2); }
+	else { L1_ATTEND(16, 2); }
+#undef L1_ATTEND
 	L1_LAUNCH_CHECK();
-	if (A.splits > 1) {
+	if (part) {
 		hipLaunchKernelGGL(paged_join<ST>, dim3((unsigned)(A.B * A.n * A.H)), dim3(128), 0, st, A, part, seqs, (ST*)o);
 		L1_LAUNCH_CHECK();
 	}
 	return L1ATTN_OK;
-}
-
-template <typename ST>
-int attend_rows(const AttendArgs& A, const void* q, const int32_t* seqs, const int32_t* counts, void* o, float* part, hipStream_t st)
-{
-	switch (row_block((int64_t)A.n * A.G)) {
-	case 1: return attend<ST, 1>(A, q, seqs, counts, o, part, st);
-	case 2: return attend<ST, 2>(A, q, seqs, counts, o, part, st);
-	case 4: return attend<ST, 4>(A, q, seqs, counts, o, part, st);
-	default: return attend<ST, 8>(A, q, seqs, counts, o, part, st);
-	}
 }
 
 // 0, an error, or 1 for a call with nothing to do
@@ -263,7 +461,7 @@ int check_attend(const l1attn_cache* cache, const l1attn_attend_desc* d, AttendA
 	for (int h = 0; h < 256; h++) A->slopes[h] = d->slopes && h < d->H ? d->slopes[h] : 0.f;
 	if (d->B == 0 || d->n == 0) return 1;
 	const int64_t groups = d->B * A->C.Hk * l1_cdiv(d->n * A->G, row_block(d->n * A->G));
-	A->splits = splits_for(A->C, groups);
+	splits_for(A->C, groups, A);
 	return L1ATTN_OK;
 }
 
@@ -288,9 +486,9 @@ int l1attn_cache_attend(const l1attn_cache* cache, const l1attn_attend_desc* des
 	const size_t need = l1attn_cache_attend_workspace_bytes(cache, desc);
 	if (need && (!workspace || workspace_bytes < need)) return L1ATTN_ERR_WORKSPACE;
 	hipStream_t st = (hipStream_t)stream;
-	if (desc->dtype == 0) return attend_rows<float>(A, q, seqs, counts, o, (float*)workspace, st);
-	if (desc->dtype == 1) return attend_rows<_Float16>(A, q, seqs, counts, o, (float*)workspace, st);
-	return attend_rows<__bf16>(A, q, seqs, counts, o, (float*)workspace, st);
+	if (desc->dtype == 0) return attend<float>(A, q, seqs, counts, o, (float*)workspace, st);
+	if (desc->dtype == 1) return attend<_Float16>(A, q, seqs, counts, o, (float*)workspace, st);
+	return attend<__bf16>(A, q, seqs, counts, o, (float*)workspace, st);
 }
 
 }  // extern "C"
