@@ -19,21 +19,17 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
-constexpr int kTok = 512;  // least tokens of a split
-
 struct AttendArgs {
 	L1Cache C;
-	int B, n, H, G, splits, chunk, parts;
+	int B, n, H, G, splits, step;
 	float cap, icap, rw;
-	int has_slopes;
 	float slopes[256];
 };
 
-// Tokens of a split, the same in the join: the sequence in A.parts, whole kTok of them, at most the call's chunk.
+// Tokens of a split, the same in the join: the sequence's share, whole steps of a workgroup.
 __device__ __forceinline__ int split_tokens(const AttendArgs& A, int len)
 {
-	const int per = ((len + A.parts - 1) / A.parts + kTok - 1) / kTok * kTok;
-	return min(max(per, kTok), A.chunk);
+	return max((len + A.splits - 1) / A.splits + A.step - 1, 1) / A.step * A.step;
 }
 
 // length of entry b's sequence, 0 where it names none
@@ -53,34 +49,40 @@ __device__ __forceinline__ void codes4(int word, float (&x)[4])
 	x[3] = (float)(word >> 24);
 }
 
-// One 16-bit or float32 logit's weight exp(c(a) - slope * dist), a <= 0.
-template <typename ST> __device__ __forceinline__ float weight(const AttendArgs& A, float a, float slope, float dist)
+// c(a) = cap tanh(a / cap) of a logit a <= 0, and exp(a)
+template <typename ST> __device__ __forceinline__ float capped(float a, float cap, float icap)
 {
-	if constexpr (sizeof(ST) == 4) {
-		if (A.cap > 0.f) a = A.cap * tanhf(a * A.icap);
-		return expf(a - slope * dist);
-	} else {
-		if (A.cap > 0.f) {
-			const float e = __builtin_amdgcn_exp2f(a * (2.885390082f * A.icap));
-			a = A.cap * (e - 1.f) * __builtin_amdgcn_rcpf(e + 1.f);
-		}
-		return __builtin_amdgcn_exp2f(1.442695041f * (a - slope * dist));
-	}
+	if constexpr (sizeof(ST) == 4) return cap * tanhf(a * icap);
+	const float e = __builtin_amdgcn_exp2f(a * (2.885390082f * icap));
+	return cap * (e - 1.f) * __builtin_amdgcn_rcpf(e + 1.f);
+}
+template <typename ST> __device__ __forceinline__ float exponential(float a)
+{
+	if constexpr (sizeof(ST) == 4) return expf(a);
+	return __builtin_amdgcn_exp2f(1.442695041f * a);
 }
 
-// RB rows of a workgroup.  Grid: splits, batch * key heads, blocks of rows.  part: [splits][B][n][H][Wv + 1] (the last: the
+// page * stride bytes behind a pool's base
+template <typename T> __device__ __forceinline__ const T* page_at(const T* base, int page, unsigned stride)
+{
+	return reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + (uint64_t)(uint32_t)page * stride);
+}
+
+// RB rows of a workgroup.  Grid: batch * key heads, splits, blocks of rows: the splits behind a short sequence's end
+// have nothing to do; the pairs are turned so that every group's splits are spread over the eight dies.  part: [splits][B][n][H][Wv + 1] (the last: the
 // weights' sum), or NULL with one split, which writes o itself.
 // Each of the four waves takes 64 U tokens of its own at a time and waits for no other: a lane holds U tokens against all rows,
 // whose values are broadcast LDS reads; the weights pass through the wave's own piece of LDS into the layout of the matrix
 // instructions, which add up weight * value.  A step's loads are on their way together: the next step's pages, keys, values.
-template <typename ST, int RB, int NC, int MINW>
+template <typename ST, int RB, int NC, bool FULL, int MINW>
 __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST* __restrict__ q, const int32_t* __restrict__ seqs,
                                                           const int32_t* __restrict__ counts, ST* __restrict__ o, float* __restrict__ part)
 {
-	constexpr bool F32 = sizeof(ST) == 4, CODED = !F32 && RB >= 8;
-	constexpr int U = RB <= 2 ? 1 : 2, VG = NC / 4, KB = RB >= 8 ? 2 : 4;  // KB: pieces of 16 bytes of a key row under way
+	constexpr bool F32 = sizeof(ST) == 4, CODED = !F32 && RB >= 8, LATE = RB >= 8;  // LATE: values are asked for behind the distances, for want of registers
+	constexpr int U = RB <= 4 ? 1 : 2, VG = NC / 4, KB = RB >= 8 ? 2 : 4;  // KB: pieces of 16 bytes of a key row under way
 	constexpr int pitch = 64 * U + (F32 ? 4 : 8);                          // between two rows' weights: an odd number of 16-byte pieces
 	using PT = std::conditional_t<F32, float, _Float16>;
+	constexpr int TR = 256 / RB;  // threads of a row before and behind the loop
 	constexpr int pool = 4 * RB * pitch * (int)sizeof(PT), join = 2 * RB * 128 * 4;
 	__shared__ __align__(16) float qs[RB * 128];
 	__shared__ __align__(16) unsigned qc[CODED ? RB * 64 : 1];
@@ -88,29 +90,45 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 	__shared__ float red[8], dens[4 * RB];
 	const L1Cache& C = A.C;
 	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g = lane >> 4;
-	const int b = blockIdx.y / C.Hk, hk = blockIdx.y % C.Hk, r0 = blockIdx.z * RB, R = A.n * A.G;
+	const int group = (blockIdx.x + blockIdx.y) % gridDim.x, b = group / C.Hk, hk = group % C.Hk, r0 = blockIdx.z * RB, R = A.n * A.G;
 	int s;
 	const int len = seq_of(A, seqs, b, s);
 	const int cnt = counts ? min(max(counts[b], 0), A.n) : A.n;
-	const int per = split_tokens(A, len), lo = min((int64_t)blockIdx.x * per, (int64_t)len), hi = min(lo + per, len);
+	const int per = split_tokens(A, len), lo = min((int64_t)blockIdx.y * per, (int64_t)len), hi = min(lo + per, len);
 	if (lo >= hi && part) return;  // the join knows which splits there are
 	const int32_t* table = C.table + (int64_t)s * C.M;
 	const int psh = C.P == 16 ? 4 : C.P == 32 ? 5 : 6;  // a page's tokens are 16, 32 or 64
+	const int pk = FULL ? 16 * NC : C.pk, pv = FULL ? 16 * NC : C.pv;
+	int after[U];  // page of the lane's tokens in the step behind the coming one
+	const int first = lo + 64 * U * wave;
+	auto page_of = [&](int t) { return t < hi ? table[t >> psh] : -1; };
 	int page[U];
-	const int first = lo + 64 * U * wave + lane;
 #pragma unroll
-	for (int u = 0; u < U; u++) page[u] = first + 64 * u < hi ? table[(first + 64 * u) >> psh] : -1;
+	for (int u = 0; u < U; u++) {
+		page[u] = page_of(first + 64 * u + lane);
+		after[u] = page_of(first + 64 * u + lane + 256 * U);
+	}
 	// the rows' values, zero behind the width: the cache's rows are zero there as well
+	const int my = tid / TR, my0 = tid % TR, myt = (r0 + my) / A.G;
+	const int64_t myrow = r0 + my < R ? ((int64_t)b * A.n + myt) * A.H + hk * A.G + (r0 + my - myt * A.G) : -1;
 	float least = 0.f, most = 0.f;
 	bool finite = true;
-	for (int x = tid; x < RB * C.pk; x += 256) {
-		const int rr = x / C.pk, r = r0 + rr, w = x - rr * C.pk;
-		const int t = r / A.G, h = hk * A.G + r - t * A.G;
-		const float y = r < R && w < C.W ? (float)q[(((int64_t)b * A.n + t) * A.H + h) * C.W + w] : 0.f;
-		qs[rr * 128 + w] = y;
+	for (int w = my0; w < pk; w += TR) {
+		const float y = myrow >= 0 && w < C.W ? (float)q[myrow * C.W + w] : 0.f;
+		qs[my * 128 + w] = y;
 		finite &= __builtin_fabsf(y) <= 3.402823466e38f;
 		least = fminf(least, y);
 		most = fmaxf(most, y);
+	}
+	// what a row sees, -1 for nothing, and its slope
+	int place[RB];
+	float slope[RB];
+	int rt = r0 / A.G, rx = r0 - rt * A.G;
+#pragma unroll
+	for (int r = 0; r < RB; r++) {
+		place[r] = __builtin_amdgcn_readfirstlane(r0 + r < R && rt < cnt ? len - cnt + rt : -1);
+		slope[r] = A.slopes[hk * A.G + rx];
+		if (++rx == A.G) { rx = 0; rt++; }
 	}
 	bool coded = false;
 	float sc = 0.f, off = 0.f, m = A.rw;
@@ -141,16 +159,14 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 		off = coded ? -(least - (most - least) * 0x1p-20f) * sc : 0.f;
 		if (coded) {
 			m = span * (1.f / 65535.f) * A.rw;
-			for (int x = tid; x < RB * (C.pk / 2); x += 256) {
-				const int rr = x / (C.pk / 2), w = x - rr * (C.pk / 2);
-				qc[rr * 64 + w] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pknorm_u16(__builtin_fmaf(qs[rr * 128 + 2 * w], sc, off),
-				                                                                             __builtin_fmaf(qs[rr * 128 + 2 * w + 1], sc, off)));
-			}
+			for (int w = my0; w < pk / 2; w += TR)
+				qc[my * 64 + w] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pknorm_u16(__builtin_fmaf(qs[my * 128 + 2 * w], sc, off),
+				                                                                             __builtin_fmaf(qs[my * 128 + 2 * w + 1], sc, off)));
 		}
 	}
 	__syncthreads();
 	PT* ps = reinterpret_cast<PT*>(shared_pool) + wave * RB * pitch;
-	const int kchunks = C.pk / 16;
+	const int kchunks = FULL ? NC : pk / 16;
 	float den[RB];
 	f4 acc[VG][4];
 #pragma unroll
@@ -159,39 +175,63 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 	for (int wg = 0; wg < VG; wg++)
 #pragma unroll
 		for (int e = 0; e < 4; e++) acc[wg][e] = (f4)(0.f);
-	for (int t0 = lo + 64 * U * wave; t0 < hi; t0 += 256 * U) {
-		float ks[U], vs[U];
-		bool there[U];
-		const int8_t* krow[U];
-		int pg[U];
-		uint4 kr[U][KB];
+	const int kend = (kchunks + KB - 1) / KB * KB;
+	float ks[U], vs[U];
+	int pg[U];
+	const int8_t* krow[U];
+	uint4 kr[U][KB];
+	// A step begins at a multiple of 64, so a lane's place in its page is always the same.
+	const unsigned kstride = (unsigned)C.Hk * C.P * pk, vstride = (unsigned)C.Hk * C.P * pv;
+	const int8_t *kbase = C.k + (int64_t)hk * C.P * pk, *vbase = C.v + (int64_t)hk * C.P * pv;
+	const int kin = (lane & (C.P - 1)) * pk;
+	// where tokens are: no page, page 0 and scales 0 if nowhere
+	auto locate = [&](int at, int& to, const int8_t*& row, float& a, float& c) {
+		const bool there = at >= 0 && at < C.N;
+		to = there ? at : -1;
+		const int p0 = there ? at : 0;
+		row = page_at(kbase, p0, kstride) + kin;
+		const float x = *page_at(C.ks + hk, p0, 4u * C.Hk), y = *page_at(C.vs + hk, p0, 4u * C.Hk);
+		a = there ? x : 0.f;
+		c = there ? y : 0.f;
+	};
+#pragma unroll
+	for (int u = 0; u < U; u++) {
+		locate(page[u], pg[u], krow[u], ks[u], vs[u]);
+#pragma unroll
+		for (int c = 0; c < KB; c++) kr[u][c] = *reinterpret_cast<const uint4*>(krow[u] + 16 * (FULL ? c : min(c, kchunks - 1)));
+	}
+	for (int t0 = first; t0 < hi; t0 += 256 * U) {
+		float nks[U], nvs[U];
+		int npg[U];
+		const int8_t* nrow[U];
 #pragma unroll
 		for (int u = 0; u < U; u++) {
-			const int t = t0 + 64 * u + lane;
-			there[u] = page[u] >= 0 && page[u] < C.N;
-			pg[u] = there[u] ? page[u] : 0;
-			const int64_t at = (int64_t)pg[u] * C.Hk + hk;
-			krow[u] = C.k + ((at << psh) + (t & (C.P - 1))) * C.pk;
-#pragma unroll
-			for (int c = 0; c < KB; c++) kr[u][c] = *reinterpret_cast<const uint4*>(krow[u] + 16 * min(c, kchunks - 1));
-			ks[u] = there[u] ? C.ks[at] : 0.f;
-			vs[u] = there[u] ? C.vs[at] : 0.f;
-			page[u] = t + 256 * U < hi ? table[(t + 256 * U) >> psh] : -1;
+			locate(after[u], npg[u], nrow[u], nks[u], nvs[u]);
+			after[u] = page_of(t0 + 64 * u + lane + 512 * U);
 		}
+		// piece c of the key rows: of this step's, then the first ones of the next step's
+		auto piece = [&](int u, int c) {
+			const int8_t* row = c < kend ? krow[u] : nrow[u];
+			c -= c < kend ? 0 : kend;
+			return *reinterpret_cast<const uint4*>(row + 16 * (FULL ? c : min(c, kchunks - 1)));
+		};
 		// the values: for 16 bits eight tokens in a row of every 32, for float32 four of every 16, four columns each
 		constexpr int VT = F32 ? 4 : 8;
 		unsigned vr[16 * U / VT][VG][VT];
+		auto load_values = [&]() {
 #pragma unroll
-		for (int kc = 0; kc < 16 * U / VT; kc++) {
-			const int tok = 4 * VT * kc + VT * g;
-			const int vp = __shfl(pg[kc * 4 * VT / 64], tok & 63);
-			const int8_t* row = C.v + ((((int64_t)vp * C.Hk + hk) << psh) + ((t0 + tok) & (C.P - 1))) * C.pv;
+			for (int kc = 0; kc < 16 * U / VT; kc++) {
+				const int tok = 4 * VT * kc + VT * g;
+				const int vp = max(__shfl(pg[kc * 4 * VT / 64], tok & 63), 0);
+				const int8_t* row = page_at(vbase, vp, vstride) + (tok & (C.P - 1)) * pv + (FULL ? 4 * l16 : 0);
 #pragma unroll
-			for (int wg = 0; wg < VG; wg++)
+				for (int wg = 0; wg < VG; wg++)
 #pragma unroll
-				for (int e = 0; e < VT; e++)
-					vr[kc][wg][e] = *reinterpret_cast<const unsigned*>(row + e * C.pv + min(64 * wg + 4 * l16, C.pv - 4));
-		}
+					for (int e = 0; e < VT; e++)
+						vr[kc][wg][e] = *reinterpret_cast<const unsigned*>(row + e * pv + (FULL ? 64 * wg : min(64 * wg + 4 * l16, pv - 4)));
+			}
+		};
+		if constexpr (!LATE) load_values();
 		float dist[U][RB];
 		if (coded) {
 			unsigned sum[U][RB];
@@ -208,7 +248,7 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 #pragma unroll
 					for (int u = 0; u < U; u++) {
 						const uint4 raw = kr[u][i];
-						kr[u][i] = *reinterpret_cast<const uint4*>(krow[u] + 16 * min(c + KB, kchunks - 1));
+						kr[u][i] = piece(u, c + KB);
 						const int word[4] = {(int)raw.x, (int)raw.y, (int)raw.z, (int)raw.w};
 						const float f = ks[u] * sc;
 #pragma unroll
@@ -219,12 +259,17 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 							kc[u][2 * d + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pknorm_u16(__builtin_fmaf(x[2], f, off), __builtin_fmaf(x[3], f, off)));
 						}
 					}
-					if (c < kchunks)
+					if (FULL || c < kchunks)
+						{
+							// the rows' codes are read four pieces ahead of their use
+							const unsigned* from = qc + 8 * c;
+							uint4 ring[4];
 #pragma unroll
-						for (int r = 0; r < RB; r++)
+							for (int j = 0; j < 4; j++) ring[j] = *reinterpret_cast<const uint4*>(from + (j >> 1) * 64 + 4 * (j & 1));
 #pragma unroll
-							for (int h = 0; h < 2; h++) {
-								const uint4 y = *reinterpret_cast<const uint4*>(qc + r * 64 + 8 * c + 4 * h);
+							for (int j = 0; j < 2 * RB; j++) {
+								const int r = j >> 1, h = j & 1;
+								const uint4 y = ring[j & 3];
 #pragma unroll
 								for (int u = 0; u < U; u++) {
 									unsigned z = sum[u][r];
@@ -234,7 +279,10 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 									z = __builtin_amdgcn_sad_u16(kc[u][4 * h + 3], y.w, z);
 									sum[u][r] = z;
 								}
+								if (j + 4 < 2 * RB) ring[j & 3] = *reinterpret_cast<const uint4*>(from + ((j + 4) >> 1) * 64 + 4 * (j & 1));
+								__builtin_amdgcn_sched_barrier(0);
 							}
+						}
 				}
 			}
 #pragma unroll
@@ -255,30 +303,36 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 #pragma unroll
 					for (int u = 0; u < U; u++) {
 						raw[u] = kr[u][i];
-						kr[u][i] = *reinterpret_cast<const uint4*>(krow[u] + 16 * min(c + KB, kchunks - 1));
+						kr[u][i] = piece(u, c + KB);
 					}
-					if (c < kchunks)
+					if (FULL || c < kchunks) {
+						const float* from = qs + 16 * c;
+						constexpr int AHEAD = 4 * RB < 4 ? 4 * RB : 4;
+						float4 ring[AHEAD];
+						float k[U][4];
 #pragma unroll
-						for (int d = 0; d < 4; d++) {
-							float k[U][4];
+						for (int j = 0; j < AHEAD; j++) ring[j] = *reinterpret_cast<const float4*>(from + j % RB * 128 + 4 * (j / RB));
+#pragma unroll
+						for (int j = 0; j < 4 * RB; j++) {
+							const int d = j / RB, r = j % RB;
+							if (r == 0)
+#pragma unroll
+								for (int u = 0; u < U; u++) codes4((int)(d == 0 ? raw[u].x : d == 1 ? raw[u].y : d == 2 ? raw[u].z : raw[u].w), k[u]);
+							const float4 y = ring[j % AHEAD];
 #pragma unroll
 							for (int u = 0; u < U; u++) {
-								codes4((int)(d == 0 ? raw[u].x : d == 1 ? raw[u].y : d == 2 ? raw[u].z : raw[u].w), k[u]);
+								const float d0 = __builtin_fmaf(-k[u][0], ks[u], y.x), d1 = __builtin_fmaf(-k[u][1], ks[u], y.y);
+								const float d2 = __builtin_fmaf(-k[u][2], ks[u], y.z), d3 = __builtin_fmaf(-k[u][3], ks[u], y.w);
+								dist[u][r] += (__builtin_fabsf(d0) + __builtin_fabsf(d1)) + (__builtin_fabsf(d2) + __builtin_fabsf(d3));
 							}
-#pragma unroll
-							for (int r = 0; r < RB; r++) {
-								const float4 y = *reinterpret_cast<const float4*>(qs + r * 128 + 16 * c + 4 * d);
-#pragma unroll
-								for (int u = 0; u < U; u++) {
-									const float d0 = __builtin_fmaf(-k[u][0], ks[u], y.x), d1 = __builtin_fmaf(-k[u][1], ks[u], y.y);
-									const float d2 = __builtin_fmaf(-k[u][2], ks[u], y.z), d3 = __builtin_fmaf(-k[u][3], ks[u], y.w);
-									dist[u][r] += (__builtin_fabsf(d0) + __builtin_fabsf(d1)) + (__builtin_fabsf(d2) + __builtin_fabsf(d3));
-								}
-							}
+							if (j + AHEAD < 4 * RB) ring[j % AHEAD] = *reinterpret_cast<const float4*>(from + (j + AHEAD) % RB * 128 + 4 * ((j + AHEAD) / RB));
+							__builtin_amdgcn_sched_barrier(0);
 						}
+					}
 				}
 			}
 		}
+		if constexpr (LATE) load_values();
 		// float16 weights: 2^14 over the power of two above the largest scale of the step's values, and back
 		float up = 1.f, down = 1.f;
 		if constexpr (!F32) {
@@ -291,16 +345,24 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 			down = __builtin_amdgcn_ldexpf(1.f, ve - 14);
 		}
 #pragma unroll
-		for (int r = 0; r < RB; r++) {
-			const int row = r0 + r, tq = row / A.G, place = row < R && tq < cnt ? len - cnt + tq : -1;  // -1: sees nothing
-			const float slope = A.has_slopes && row < R ? A.slopes[hk * A.G + row - tq * A.G] : 0.f;
+		for (int u = 0; u < U; u++)
 #pragma unroll
-			for (int u = 0; u < U; u++) {
-				const int t = t0 + 64 * u + lane;
-				const float w = weight<ST>(A, -dist[u][r] * m, slope, (float)(place - t));
-				const float p = there[u] && t < hi && t <= place ? w : 0.f;
+			for (int r = 0; r < RB; r++) dist[u][r] *= -m;
+		if (A.cap > 0.f)
+#pragma unroll
+			for (int u = 0; u < U; u++)
+#pragma unroll
+				for (int r = 0; r < RB; r++) dist[u][r] = capped<ST>(dist[u][r], A.cap, A.icap);
+#pragma unroll
+		for (int u = 0; u < U; u++) {
+			const int t = t0 + 64 * u + lane, sees = pg[u] >= 0 ? t : 0x7fffffff;
+			const float scale = vs[u] * up;
+#pragma unroll
+			for (int r = 0; r < RB; r++) {
+				const float w = exponential<ST>(__builtin_fmaf(-slope[r], (float)(place[r] - t), dist[u][r]));
+				const float p = sees <= place[r] ? w : 0.f;
 				den[r] += p;
-				ps[r * pitch + 64 * u + lane] = (PT)(p != 0.f ? p * (vs[u] * up) : 0.f);  // the scale of a hidden token has no influence
+				ps[r * pitch + 64 * u + lane] = (PT)(p != 0.f ? p * scale : 0.f);  // the scale of a hidden token has no influence
 			}
 		}
 		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -340,7 +402,10 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 #pragma unroll
 			for (int e = 0; e < 4; e++) acc[wg][e] = F32 ? y[e] : acc[wg][e] + y[e] * down;
 		}
+		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 		__builtin_amdgcn_wave_barrier();
+#pragma unroll
+		for (int u = 0; u < U; u++) { pg[u] = npg[u]; krow[u] = nrow[u]; ks[u] = nks[u]; vs[u] = nvs[u]; }
 	}
 	// rows 4 g + i (a row again every RB), columns 64 wg + 4 l16 + e; over the waves through LDS, where the weights lay
 #pragma unroll
@@ -365,20 +430,14 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 				}
 		__syncthreads();
 	}
-	for (int x = tid; x < RB * C.Wv; x += 256) {
-		const int r = x / C.Wv, w = x - r * C.Wv, row = r0 + r;
-		if (row >= R) continue;
-		const int t = row / A.G;
-		const int64_t out = ((int64_t)b * A.n + t) * A.H + hk * A.G + row - t * A.G;
-		const float d = dens[r] + dens[RB + r] + dens[2 * RB + r] + dens[3 * RB + r];
-		const float y = sums[r * 128 + w] + sums[(RB + r) * 128 + w];
-		if (part) {
-			float* to = part + ((int64_t)blockIdx.x * A.B * A.n * A.H + out) * (C.Wv + 1);
-			to[w] = y;
-			if (w == 0) to[C.Wv] = d;
-		} else {
-			o[out * C.Wv + w] = (ST)(y / (1.f + d));
-		}
+	if (myrow < 0) return;
+	const float d = dens[my] + dens[RB + my] + dens[2 * RB + my] + dens[3 * RB + my];
+	float* to = part + ((int64_t)blockIdx.y * A.B * A.n * A.H + myrow) * (C.Wv + 1);
+	if (part && my0 == 0) to[C.Wv] = d;
+	for (int w = my0; w < C.Wv; w += TR) {
+		const float y = sums[my * 128 + w] + sums[(RB + my) * 128 + w];
+		if (part) to[w] = y;
+		else o[myrow * C.Wv + w] = (ST)(y / (1.f + d));
 	}
 }
 
@@ -404,33 +463,32 @@ __global__ void __launch_bounds__(128) paged_join(AttendArgs A, const float* __r
 // rows of a workgroup
 int row_block(int64_t R) { return R <= 1 ? 1 : R <= 2 ? 2 : R <= 4 ? 4 : R <= 8 ? 8 : 16; }
 
-// Splits of the longest sequence that the table can hold: about 2048 workgroups in all, of 512 tokens at least, and eight where
-// the sequences may be much shorter than that.
-void splits_for(const L1Cache& C, int64_t groups, AttendArgs* A)
+// Splits of a sequence: as many as fill the 256 compute units with workgroups once (two of 8 or 16 rows, four of fewer rows).
+// For 32 sequences of about 2050 tokens, 4 rows, W 64, twice or four times as many take 19.5 and 19.7 us instead of 19.0; for 16 of
+// about 20480, 16 rows, W 128, 175 and 167 instead of 164, and the sums to join grow.  A table of 512 tokens at most
+// is not split:
+// 12 us for one sequence of 300 tokens, 16.6 with the kernel that joins.
+int splits_for(const L1Cache& C, int rows, int64_t groups)
 {
-	const int64_t tokens = (int64_t)C.M * C.P, most = l1_cdiv(tokens, kTok), want = l1_cdiv(2048, groups);
-	A->chunk = (int)(l1_cdiv(l1_cdiv(tokens, want), kTok) * kTok);
-	if (A->chunk < kTok) A->chunk = kTok;
-	int64_t parts = l1_cdiv(4096, groups);
-	parts = parts > 8 ? 8 : parts;
-	A->parts = (int)(parts > most ? (most < 1 ? 1 : most) : parts);
-	const int64_t n = l1_cdiv(tokens, A->chunk);
-	A->splits = (int)(n > A->parts ? n : A->parts);
+	const int64_t tokens = (int64_t)C.M * C.P, most = tokens <= 512 ? 1 : l1_cdiv(tokens, rows <= 4 ? 256 : 512);
+	const int64_t want = l1_cdiv(rows <= 4 ? 1024 : 512, groups);
+	return (int)(want > most ? most : want < 1 ? 1 : want);
 }
 
 template <typename ST>
 int attend(const AttendArgs& A, const void* q, const int32_t* seqs, const int32_t* counts, void* o, float* ws, hipStream_t st)
 {
 	const int rb = row_block((int64_t)A.n * A.G);
-	const dim3 grid((unsigned)A.splits, (unsigned)(A.B * A.C.Hk), (unsigned)l1_cdiv((int64_t)A.n * A.G, rb));
+	const dim3 grid((unsigned)(A.B * A.C.Hk), (unsigned)A.splits, (unsigned)l1_cdiv((int64_t)A.n * A.G, rb));
 	float* part = A.splits > 1 ? ws : nullptr;
-	const bool wide = A.C.pk > 64 || A.C.pv > 64;
-#define L1_ATTEND(RB, MINW)                                                                                                              \
-	if (wide) hipLaunchKernelGGL((paged_attend<ST, RB, 8, 2>), grid, dim3(256), 0, st, A, (const ST*)q, seqs, counts, (ST*)o, part);     \
-	else hipLaunchKernelGGL((paged_attend<ST, RB, 4, MINW>), grid, dim3(256), 0, st, A, (const ST*)q, seqs, counts, (ST*)o, part)
+	const int full = A.C.pk == A.C.pv ? A.C.pk : 0;  // rows of 64 or 128 bytes: addresses and loops are known to the compiler
+#define L1_ATTEND(RB, MINW)                                                                                                                          \
+	if (full == 64) hipLaunchKernelGGL((paged_attend<ST, RB, 4, true, MINW>), grid, dim3(256), 0, st, A, (const ST*)q, seqs, counts, (ST*)o, part);  \
+	else if (full == 128) hipLaunchKernelGGL((paged_attend<ST, RB, 8, true, 2>), grid, dim3(256), 0, st, A, (const ST*)q, seqs, counts, (ST*)o, part); \
+	else hipLaunchKernelGGL((paged_attend<ST, RB, 8, false, 2>), grid, dim3(256), 0, st, A, (const ST*)q, seqs, counts, (ST*)o, part)
 	if (rb == 1) { L1_ATTEND(1, 4); }
 	else if (rb == 2) { L1_ATTEND(2, 4); }
-	else if (rb == 4) { L1_ATTEND(4, 2); }
+	else if (rb == 4) { L1_ATTEND(4, 4); }
 	else if (rb == 8) { L1_ATTEND(8, 2); }
 	else { L1_ATTEND(16, 2); }
 #undef L1_ATTEND
@@ -457,11 +515,11 @@ int check_attend(const l1attn_cache* cache, const l1attn_attend_desc* d, AttendA
 	if (l1_cdiv(d->n * A->G, 8) > 65535) return L1ATTN_ERR_RANGE;
 	A->cap = d->softcap; A->icap = d->softcap > 0.f ? 1.f / d->softcap : 0.f;
 	A->rw = (float)(1.0 / sqrt((double)A->C.W));
-	A->has_slopes = d->slopes != nullptr;
 	for (int h = 0; h < 256; h++) A->slopes[h] = d->slopes && h < d->H ? d->slopes[h] : 0.f;
 	if (d->B == 0 || d->n == 0) return 1;
 	const int64_t groups = d->B * A->C.Hk * l1_cdiv(d->n * A->G, row_block(d->n * A->G));
-	splits_for(A->C, groups, A);
+	A->step = row_block(d->n * A->G) <= 4 ? 256 : 512;
+	A->splits = splits_for(A->C, row_block(d->n * A->G), groups);
 	return L1ATTN_OK;
 }
 
