@@ -112,8 +112,6 @@ def _masked_desc(q, k, v, doc, prefix, causal, softcap, slopes):
         raise RuntimeError("n_heads must be a multiple of n_key_heads, got %d and %d" % (H, Hk))
     if not (1 <= W <= 128 and 1 <= Wv <= 128):
         raise RuntimeError("widths of masked attention are 1 to 128, got %d and %d" % (W, Wv))
-    if prefix is not None and not causal:
-        raise ValueError("prefix is an exception to the causal mask: it has no meaning without causal=True")
     _check_rule(H, softcap, slopes)
     return MaskedDesc(B, T, S, H, Hk, W, Wv, DTYPES[q.dtype], int(bool(causal)), softcap,
                       None if slopes is None else ctypes.addressof(_slopes_array(slopes)),

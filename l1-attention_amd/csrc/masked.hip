@@ -20,7 +20,6 @@ int check_desc(const l1attn_masked_desc* d)
 	if (d->B < 0 || d->T < 0 || d->S < d->T || d->H < 1 || d->Hk < 1 || d->H % d->Hk || d->W < 1 || d->Wv < 1) return L1ATTN_ERR_ARG;
 	if (d->dtype < 0 || d->dtype > 2 || (d->causal != 0 && d->causal != 1)) return L1ATTN_ERR_ARG;
 	if (!(d->softcap >= 0.f) || !(d->softcap <= 3e38f)) return L1ATTN_ERR_ARG;
-	if (!d->causal && d->prefix) return L1ATTN_ERR_ARG;
 	// 65535 rows of the grid at two waves of 32 rows; batch * heads is the grid's other side
 	if (d->W > 128 || d->Wv > 128 || d->H > L1_MASKED_HEADS || !fits(d->S, 64 * 65535) || !fits(d->B, 1 << 22) || !fits(d->B * d->H, 1 << 30))
 		return L1ATTN_ERR_RANGE;
@@ -36,7 +35,7 @@ L1MaskedArgs args_of(const l1attn_masked_desc* d, const void* q, const void* k, 
 	A.B = (int)d->B; A.T = (int)d->T; A.S = (int)d->S; A.H = (int)d->H; A.Hk = (int)d->Hk; A.W = (int)d->W; A.Wv = (int)d->Wv;
 	A.causal = d->causal; A.cap = d->softcap; A.icap = d->softcap > 0.f ? 1.f / d->softcap : 0.f;
 	A.rw = (float)(1.0 / sqrt((double)d->W));
-	A.doc = d->doc; A.prefix = d->prefix; A.has_slopes = d->slopes != nullptr;
+	A.doc = d->doc; A.prefix = d->causal ? d->prefix : nullptr; A.has_slopes = d->slopes != nullptr;
 	for (int h = 0; h < L1_MASKED_HEADS; h++) A.slopes[h] = d->slopes && h < d->H ? d->slopes[h] : 0.f;
 	const int per = d->dtype == 0 ? 4 : 8;
 	A.vec = (d->W % per == 0 && !((uintptr_t)q & 15) ? 1 : 0) | (d->W % per == 0 && !((uintptr_t)k & 15) ? 2 : 0) |

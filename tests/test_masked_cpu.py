@@ -29,7 +29,7 @@ def test_host_tensors_and_strides_are_refused():
     (dict(k=_q(1, 4, 2, 8).half()), "dtype"), (dict(q=_q(1, 4, 2, 8).double(), k=_q(1, 4, 2, 8).double(), v=_q(1, 4, 2, 8).double()), "float32, float16"),
     (dict(v=_q(1, 4, 2, 129)), "1 to 128"), (dict(v=_q(1, 4, 2, 0)), "1 to 128"),
     (dict(doc=torch.zeros(1, 3, dtype=torch.int32)), "doc"), (dict(doc=torch.zeros(1, 4, dtype=torch.int64)), "doc"),
-    (dict(prefix=torch.zeros(2, dtype=torch.int32)), "prefix"), (dict(prefix=torch.zeros(1, dtype=torch.int32), causal=False), "prefix"),
+    (dict(prefix=torch.zeros(2, dtype=torch.int32)), "prefix"),
     (dict(softcap=-1.0), "softcap"), (dict(softcap=float("nan")), "softcap"), (dict(slopes=(1.0,)), "slopes")])
 def test_refusals(no_gpu, what, match):
     a = dict(q=_q(1, 4, 2, 8), k=_q(1, 4, 2, 8), v=_q(1, 4, 2, 8))
@@ -61,7 +61,7 @@ def test_c_entry_codes():
     assert L.l1attn_masked_fwd(None, one, one, one, one, None, None, 0, None) == -1
     assert fwd(q=None) == -1 and fwd(o=None) == -1
     for kw in (dict(T=5), dict(T=-1), dict(B=-1), dict(H=3), dict(Hk=0), dict(W=0), dict(dtype=3), dict(causal=2), dict(softcap=-1.0),
-               dict(softcap=float("nan")), dict(causal=0, prefix=16), dict(slope_values=(0.5, -1.0)), dict(slope_values=(0.5, float("nan")))):
+               dict(softcap=float("nan")), dict(slope_values=(0.5, -1.0)), dict(slope_values=(0.5, float("nan")))):
         assert fwd(**kw) == -1, kw
     for kw in (dict(W=129), dict(Wv=129), dict(H=512), dict(S=1 << 23)):
         assert fwd(**kw) == -3, kw

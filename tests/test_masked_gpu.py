@@ -120,6 +120,71 @@ def test_small_and_large_inputs(scale, dtype):
     _check(*_inputs(1, 120, 120, 2, 2, 64, 64, dtype, 11, scale))
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("shift,W,Wv", [(0.0, 64, 64), (300.0, 64, 64), (0.0, 100, 128)])
+def test_a_few_far_values(shift, W, Wv, dtype):
+    # one owner row and one streamed row far off the others, and all of them far from zero (exact in 16 bits: quarters)
+    q, k, v, do = _inputs(1, 90, 90, 2, 1, W, Wv, dtype, 31)
+    q, k = (((x.float() * 2).round() / 4 + shift).to(dtype) for x in (q, k))
+    q[0, 40], k[0, 7, :, 3] = 500.0, -500.0
+    _check(q, k, v, do)
+
+
+def test_a_prefix_changes_nothing_without_causal():
+    q, k, v, do = _inputs(2, 70, 70, 2, 1, 33, 40, BF16, 32)
+    prefix = torch.tensor([30, 0], dtype=torch.int32).cuda()
+    for a, b in zip(_run(q, k, v, do, causal=False, prefix=prefix), _run(q, k, v, do, causal=False)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_one_tensor_for_all_and_broadcast_keys(dtype):
+    x, _, _, do = _inputs(2, 65, 65, 2, 2, 48, 48, dtype, 33)
+    parts = _run(x, x, x, do)
+    y = x.detach().requires_grad_()
+    got, = torch.autograd.grad(_op()(y, y, y), y, do)
+    total = sum(p.double() for p in parts[1:])
+    # autograd adds the three in the tensor's type: two roundings, of sums no larger than the parts' magnitudes
+    room = 2 * torch.finfo(dtype).eps * sum(p.double().abs() for p in parts[1:]) + 1e-30
+    assert ((got.double() - total).abs() <= room).all()
+    one = x[:1].detach().requires_grad_()
+    g, = torch.autograd.grad(_op()(x, one.expand(2, -1, -1, -1), x), one, do)
+    dk = _run(x, x[:1].repeat(2, 1, 1, 1), x, do)[2].double()
+    assert ((g.double() - dk.sum(0, keepdim=True)).abs() <= torch.finfo(dtype).eps * dk.abs().sum(0, keepdim=True) + 1e-30).all()
+
+
+def test_a_captured_training_step_and_two_calls_at_once():
+    q, k, v, do = _inputs(2, 130, 130, 4, 2, 64, 64, BF16, 34)
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    op = _op(softcap=8.0)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):  # as a captured step needs it: the first pass on a stream of its own, nothing of it kept
+        torch.autograd.grad(op(*leaves), leaves, do)
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grads = torch.autograd.grad(op(*leaves), leaves, do)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for seed in range(3):
+        fresh = _inputs(2, 130, 130, 4, 2, 64, 64, BF16, 40 + seed)
+        with torch.no_grad():
+            for a, b in zip(leaves, fresh):
+                a.copy_(b)
+        want = _run(*fresh[:3], do, cap=8.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(grads, want[1:]))
+        got = []
+        for t in streams:
+            t.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(t):
+                got.append(_run(*fresh[:3], do, cap=8.0))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for x in got for a, b in zip(x, want))
+
+
 def test_ties_have_no_sign():
     # integers: many pairs are equal in a column, and sign(0) = 0
     g = torch.Generator().manual_seed(2)
