@@ -17,6 +17,7 @@ namespace {
 
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
 struct AttendArgs {
@@ -78,10 +79,10 @@ template <typename ST, int RB, int NC, bool FULL, int MINW>
 __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST* __restrict__ q, const int32_t* __restrict__ seqs,
                                                           const int32_t* __restrict__ counts, ST* __restrict__ o, float* __restrict__ part)
 {
-	constexpr bool F32 = sizeof(ST) == 4, CODED = !F32 && RB >= 8, LATE = RB >= 8;  // LATE: values are asked for behind the distances, for want of registers
+	constexpr bool F32 = sizeof(ST) == 4, HALF = std::is_same_v<ST, _Float16>, CODED = !F32 && RB >= 8, LATE = RB >= 8;  // LATE: values are asked for behind the distances, for want of registers
 	constexpr int U = RB <= 4 ? 1 : 2, VG = NC / 4, KB = RB >= 8 ? 2 : 4;  // KB: pieces of 16 bytes of a key row under way
 	constexpr int pitch = 64 * U + (F32 ? 4 : 8);                          // between two rows' weights: an odd number of 16-byte pieces
-	using PT = std::conditional_t<F32, float, _Float16>;
+	using PT = ST;  // weights are rounded to the type of the rows
 	constexpr int TR = 256 / RB;  // threads of a row before and behind the loop
 	constexpr int pool = 4 * RB * pitch * (int)sizeof(PT), join = 2 * RB * 128 * 4;
 	__shared__ __align__(16) float qs[RB * 128];
@@ -333,9 +334,10 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 			}
 		}
 		if constexpr (LATE) load_values();
-		// float16 weights: 2^14 over the power of two above the largest scale of the step's values, and back
+		// float16 weights: times 2^14 over the power of two above the largest scale of the step's values, and back; the other types'
+		// exponents reach as far as float32's
 		float up = 1.f, down = 1.f;
-		if constexpr (!F32) {
+		if constexpr (HALF) {
 			float most = __builtin_fabsf(vs[0]);
 			if constexpr (U == 2) most = fmaxf(most, __builtin_fabsf(vs[1]));
 #pragma unroll
@@ -371,7 +373,7 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 		for (int wg = 0; wg < VG; wg++) {
 			f4 y[4];
 #pragma unroll
-			for (int e = 0; e < 4; e++) y[e] = F32 ? acc[wg][e] : (f4)(0.f);
+			for (int e = 0; e < 4; e++) y[e] = HALF ? (f4)(0.f) : acc[wg][e];
 #pragma unroll
 			for (int kc = 0; kc < 16 * U / VT; kc++) {
 				const uint4 pa = *reinterpret_cast<const uint4*>(ps + l16 % RB * pitch + 4 * VT * kc + VT * g);
@@ -390,17 +392,25 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 						unsigned x[4];
 #pragma unroll
 						for (int d = 0; d < 4; d++) {
-							// byte e of two tokens, plus 128, behind the bits of 1024: then without the 1152
-							const unsigned two = __builtin_amdgcn_perm(vr[kc][wg][2 * d + 1] ^ 0x80808080u, vr[kc][wg][2 * d] ^ 0x80808080u, 0x0c040c00u + 0x00010001u * e) | 0x64006400u;
-							const h2 v = __builtin_bit_cast(h2, two) - (h2){(_Float16)1152.f, (_Float16)1152.f};
-							x[d] = __builtin_bit_cast(unsigned, v);
+							const unsigned v0 = vr[kc][wg][2 * d], v1 = vr[kc][wg][2 * d + 1];
+							if constexpr (HALF) {
+								// byte e of two tokens, plus 128, behind the bits of 1024: then without the 1152
+								const unsigned two = __builtin_amdgcn_perm(v1 ^ 0x80808080u, v0 ^ 0x80808080u, 0x0c040c00u + 0x00010001u * e) | 0x64006400u;
+								x[d] = __builtin_bit_cast(unsigned, __builtin_bit_cast(h2, two) - (h2){(_Float16)1152.f, (_Float16)1152.f});
+							} else {
+								// a code's float32 ends in 16 zero bits
+								const float a = (float)(int8_t)(v0 >> 8 * e), c = (float)(int8_t)(v1 >> 8 * e);
+								x[d] = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, c), __builtin_bit_cast(unsigned, a), 0x07060302u);
+							}
 						}
-						y[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, pa), __builtin_bit_cast(h8, make_uint4(x[0], x[1], x[2], x[3])), y[e], 0, 0, 0);
+						const uint4 pb = make_uint4(x[0], x[1], x[2], x[3]);
+						if constexpr (HALF) y[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, pa), __builtin_bit_cast(h8, pb), y[e], 0, 0, 0);
+						else y[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, pa), __builtin_bit_cast(b8, pb), y[e], 0, 0, 0);
 					}
 				}
 			}
 #pragma unroll
-			for (int e = 0; e < 4; e++) acc[wg][e] = F32 ? y[e] : acc[wg][e] + y[e] * down;
+			for (int e = 0; e < 4; e++) acc[wg][e] = HALF ? acc[wg][e] + y[e] * down : y[e];
 		}
 		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 		__builtin_amdgcn_wave_barrier();

@@ -62,9 +62,9 @@ class Pair:
         for a, b in ((g.k_pages, p.pages[0]), (g.v_pages, p.pages[1])):
             assert torch.equal(a.cpu(), b)
 
-    def attend(self, B, n, H, seqs=None, counts=None, cap=0.0, slopes=None, dtype=None):
+    def attend(self, B, n, H, seqs=None, counts=None, cap=0.0, slopes=None, dtype=None, q=None):
         p, dtype = self.plain, dtype or self.dtype
-        q = torch.randn(B, n, H, p.W, generator=self.g).to(dtype)
+        q = (torch.randn(B, n, H, p.W, generator=self.g) if q is None else q).to(dtype)
         print("case attend", B, n, H, p.Hk, p.W, p.Wv, p.P, dtype, seqs, counts, cap, flush=True)
         o = self.m.l1attn_paged(q.cuda(), self.gpu, seqs=self.ints(seqs), counts=self.ints(counts), softcap=cap, slopes=slopes)
         ref, terms = p.attend(q, seqs, counts, cap, slopes)
@@ -177,6 +177,50 @@ def test_attention(Hk, H, n, W, Wv, P, dtype):
     slopes = tuple(2.0 ** (-8 * (h + 1) / H) for h in range(H))
     c.attend(4, n, H, seqs=[2, 0, 0, 77], cap=5.0, slopes=slopes)
     c.attend(3, n, H, seqs=[4, 1, 2], counts=[n, 0, max(0, n - 1)], slopes=slopes)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("scale", [1e-3, 4.0, 30.0])
+@pytest.mark.parametrize("H,n,W", [(2, 1, 64), (8, 2, 64), (16, 3, 112)])
+def test_small_and_large_inputs(H, n, W, scale, dtype):
+    # queries near cached tokens, so that weights are there at every scale; the largest ranges leave the 16-bit codes
+    c = Pair(N=60, P=32, Hk=2, W=W, Wv=W, rows=3, M=25, dtype=dtype, seed=n)
+    k, v = c.data(3, 700, scale)
+    c.append(3, 700, counts=[700, 33, 1], data=(k, v))
+    near = k[:, :n].float().repeat_interleave(H // 2, 2)
+    c.attend(3, n, H, q=near + 0.1 * scale * torch.randn(near.shape, generator=c.g))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("H", [2, 20])
+def test_scales_of_hidden_tokens_have_no_influence(H, dtype):
+    # a page behind the queries' place, and one that only the padding rows would see, with scales that are not finite
+    c = Pair(N=40, P=16, Hk=2, W=64, Wv=64, rows=2, M=8, dtype=dtype)
+    c.append(2, 100, counts=[100, 90])
+    q = torch.randn(1, 40, H, 64, generator=c.g).to(dtype).cuda()
+    want = c.m.l1attn_paged(q, c.gpu)
+    last = int(c.gpu.table[0, 6])  # tokens 96 to 99: the last four query tokens see them
+    c.gpu.k_scale[last], c.gpu.v_scale[last] = float("nan"), float("inf")
+    got = c.m.l1attn_paged(q, c.gpu)
+    tol = 2 * (torch.finfo(dtype).eps + 2.0 ** -24 * (3 * 64 + 64)) * 4.5  # both within the bound of lm_forms, of values up to 4.5
+    assert (got[:, :36].float() - want[:, :36].float()).abs().max() <= tol
+
+
+@pytest.mark.parametrize("H", [2, 12])
+def test_two_calls_at_once(H):
+    c = Pair(N=80, P=32, Hk=2, W=64, Wv=64, rows=4, M=40, seed=4)
+    c.append(4, 600, counts=[600, 550, 3, 0])
+    qs = [torch.randn(4, 2, H, 64, generator=c.g).to(BF16).cuda() for _ in range(2)]
+    want = [c.m.l1attn_paged(q, c.gpu) for q in qs]
+    streams = [torch.cuda.Stream() for _ in qs]
+    for _ in range(4):
+        got = []
+        for q, s in zip(qs, streams):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(c.m.l1attn_paged(q, c.gpu))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 def test_pages_that_are_not_there_give_no_tokens():
