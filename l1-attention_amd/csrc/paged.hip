@@ -5,10 +5,18 @@
 //
 // The rows r of a workgroup are the query tokens and query heads that read one key head.  Every logit is <= 0 and the no-op
 // logit is 0, so partial sums over pieces of a sequence simply add up: no running maximum, and the pieces join in a fixed
-// order.  A workgroup takes 256 tokens at a time: a lane holds one token's key row and forms the distances of all rows
-// (the rows' values are broadcast LDS reads); then a lane holds 16 value columns of every 16th token and adds p * v.
-// The bytes of the cache are read once and are what bounds it for few rows; with many rows it is the vector ALU.
-// paged_attend: up to 4 rows, and float32; paged_attend_rows: more rows of 16 bits.
+// order.  Every byte of the cache is read once for up to 16 rows.
+// Distances.  Up to 4 rows, and float32: float32, two instructions an element and row.  From 5 rows of 16 bits on: sums of
+// |difference| of 16-bit codes (v_sad_u16, two elements an instruction) on one grid over the rows' values and over what the
+// scales of the workgroup's pages allow (127 times the largest); a code is off by half a step at most, which moves a logit by
+// 0.41 steps on average.  Past a range of 24 (float16; 160 bfloat16), where that would reach the type's own rounding, or where a
+// row or scale is not finite, float32.
+// Sums.  Weight times scale is rounded to the rows' type (float16 at 2^14 over the power of two above the step's largest scale),
+// a code is exact in it, and matrix instructions add them in float32; float32 has its own matrix instruction.
+// What bounds it: for few rows latency and the reads (32 sequences of about 2050 tokens, 4 rows, W 64, bfloat16: 34 MB in 17 us),
+// for many the vector ALU (16 of about 20480, 16 rows, W 128, float16: 137 us at 2.4 TB/s; 43 of 100 vector instructions are
+// v_sad_u16, which issue in about 4.2 cycles each; the rest makes codes and float16 of the cache's bytes, and weights).  With
+// one token a lane instead of two at 16 rows a row's codes would be read from LDS twice as often.
 #include "paged.h"
 #include <math.h>
 #include <type_traits>
@@ -22,16 +30,10 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
 struct AttendArgs {
 	L1Cache C;
-	int B, n, H, G, splits, step;
+	int B, n, H, G, slots, step;
 	float cap, icap, rw;
 	float slopes[256];
 };
-
-// Tokens of a split, the same in the join: the sequence's share, whole steps of a workgroup.
-__device__ __forceinline__ int split_tokens(const AttendArgs& A, int len)
-{
-	return max((len + A.splits - 1) / A.splits + A.step - 1, 1) / A.step * A.step;
-}
 
 // length of entry b's sequence, 0 where it names none
 __device__ __forceinline__ int seq_of(const AttendArgs& A, const int32_t* seqs, int b, int& s)
@@ -39,6 +41,54 @@ __device__ __forceinline__ int seq_of(const AttendArgs& A, const int32_t* seqs, 
 	s = seqs ? seqs[b] : b;
 	if (s < 0 || s >= A.C.rows || A.C.N < 1) return 0;
 	return min(max(A.C.lens[s], 0), A.C.M * A.C.P);
+}
+
+// How the tokens of all entries are dealt out to A.slots workgroups of each key head and block of rows.  An entry's tokens are whole steps; each workgroup takes up to `per` of them, of one entry, with per =
+// ceil(steps of all entries / (slots - entries)): the sum of ceil(steps / per) is then at most `slots`.  So a batch of uneven
+// lengths ends everywhere at about the same time.  Found by a sum and a scan over the entries' lengths in every workgroup
+// (256 threads; at most 512 entries).  Whose is `slot`?  `spans`, if not NULL, takes each entry's first slot and how many it has.
+struct Share {
+	int entry, first, per;  // -1 for nobody; first slot of the entry; tokens of a slot
+};
+__device__ __forceinline__ Share share_of(const AttendArgs& A, const int32_t* seqs, int slot, int* lds, int2* spans)
+{
+	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+	int steps[2];
+#pragma unroll
+	for (int i = 0; i < 2; i++) {
+		int s;
+		const int b = 2 * tid + i;
+		steps[i] = b < A.B ? (seq_of(A, seqs, b, s) + A.step - 1) / A.step : 0;
+	}
+	unsigned total = steps[0] + steps[1];
+#pragma unroll
+	for (int m = 32; m; m >>= 1) total += __shfl_xor(total, m);
+	if (lane == 0) lds[wave] = total;
+	if (tid == 0) lds[8] = -1;
+	__syncthreads();
+	total = (unsigned)lds[0] + lds[1] + lds[2] + lds[3];
+	const unsigned room = A.slots - A.B;
+	const int per = max((int)(total / room + (total % room != 0)), 1);
+	const int n0 = (steps[0] + per - 1) / per, n1 = (steps[1] + per - 1) / per;
+	int before = n0 + n1;  // a scan over the threads
+#pragma unroll
+	for (int m = 1; m < 64; m <<= 1) {
+		const int y = __shfl_up(before, m);
+		before += lane >= m ? y : 0;
+	}
+	if (lane == 63) lds[4 + wave] = before;
+	__syncthreads();
+	before -= n0 + n1;
+	for (int w = 0; w < wave; w++) before += lds[4 + w];
+#pragma unroll
+	for (int i = 0; i < 2; i++) {
+		const int b = 2 * tid + i, first = i ? before + n0 : before, n = i ? n1 : n0;
+		if (slot >= first && slot < first + n) { lds[8] = b; lds[9] = first; }
+		if (spans && b < A.B) spans[b] = make_int2(first, n);
+	}
+	__syncthreads();
+	const Share S = {__builtin_amdgcn_readfirstlane(lds[8]), __builtin_amdgcn_readfirstlane(lds[9]), __builtin_amdgcn_readfirstlane(per * A.step)};
+	return S;
 }
 
 // One 16-byte piece of codes as float32.
@@ -69,17 +119,17 @@ template <typename T> __device__ __forceinline__ const T* page_at(const T* base,
 	return reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + (uint64_t)(uint32_t)page * stride);
 }
 
-// RB rows of a workgroup.  Grid: batch * key heads, splits, blocks of rows: the splits behind a short sequence's end
-// have nothing to do; the pairs are turned so that every group's splits are spread over the eight dies.  part: [splits][B][n][H][Wv + 1] (the last: the
-// weights' sum), or NULL with one split, which writes o itself.
+// RB rows of a workgroup.  Grid: slots * key heads, blocks of rows.  part: [slots][n][H][Wv + 1] (the last: the weights' sum); if
+// NULL, a slot is an entry, and the workgroup writes o itself.
 // Each of the four waves takes 64 U tokens of its own at a time and waits for no other: a lane holds U tokens against all rows,
 // whose values are broadcast LDS reads; the weights pass through the wave's own piece of LDS into the layout of the matrix
 // instructions, which add up weight * value.  A step's loads are on their way together: the next step's pages, keys, values.
 template <typename ST, int RB, int NC, bool FULL, int MINW>
 __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST* __restrict__ q, const int32_t* __restrict__ seqs,
-                                                          const int32_t* __restrict__ counts, ST* __restrict__ o, float* __restrict__ part)
+                                                          const int32_t* __restrict__ counts, ST* __restrict__ o, float* __restrict__ part, int2* __restrict__ spans)
 {
-	constexpr bool F32 = sizeof(ST) == 4, HALF = std::is_same_v<ST, _Float16>, CODED = !F32 && RB >= 8, LATE = RB >= 8;  // LATE: values are asked for behind the distances, for want of registers
+	constexpr bool F32 = sizeof(ST) == 4, HALF = std::is_same_v<ST, _Float16>, CODED = !F32 && RB >= 8;
+	constexpr bool LATE = RB >= 8;  // values are asked for behind the distances: registers hold the rows' codes read ahead (183 -> 164 us)
 	constexpr int U = RB <= 4 ? 1 : 2, VG = NC / 4, KB = RB >= 8 ? 2 : 4;  // KB: pieces of 16 bytes of a key row under way
 	constexpr int pitch = 64 * U + (F32 ? 4 : 8);                          // between two rows' weights: an odd number of 16-byte pieces
 	using PT = ST;  // weights are rounded to the type of the rows
@@ -91,12 +141,19 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 	__shared__ float red[8], dens[4 * RB];
 	const L1Cache& C = A.C;
 	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g = lane >> 4;
-	const int group = (blockIdx.x + blockIdx.y) % gridDim.x, b = group / C.Hk, hk = group % C.Hk, r0 = blockIdx.z * RB, R = A.n * A.G;
+	const int slot = blockIdx.x / C.Hk, hk = blockIdx.x % C.Hk, r0 = blockIdx.y * RB, R = A.n * A.G;
+	int b = slot, lo = 0, per = 0x40000000;
+	if (part) {
+		__shared__ int lds[10];
+		const Share S = share_of(A, seqs, slot, lds, blockIdx.x + blockIdx.y ? nullptr : spans);
+		if (S.entry < 0) return;
+		b = S.entry;
+		lo = (slot - S.first) * S.per;
+		per = S.per;
+	}
 	int s;
-	const int len = seq_of(A, seqs, b, s);
+	const int len = seq_of(A, seqs, b, s), hi = min(lo + per, len);
 	const int cnt = counts ? min(max(counts[b], 0), A.n) : A.n;
-	const int per = split_tokens(A, len), lo = min((int64_t)blockIdx.y * per, (int64_t)len), hi = min(lo + per, len);
-	if (lo >= hi && part) return;  // the join knows which splits there are
 	const int32_t* table = C.table + (int64_t)s * C.M;
 	const int psh = C.P == 16 ? 4 : C.P == 32 ? 5 : 6;  // a page's tokens are 16, 32 or 64
 	const int pk = FULL ? 16 * NC : C.pk, pv = FULL ? 16 * NC : C.pv;
@@ -442,7 +499,7 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 	}
 	if (myrow < 0) return;
 	const float d = dens[my] + dens[RB + my] + dens[2 * RB + my] + dens[3 * RB + my];
-	float* to = part + ((int64_t)blockIdx.y * A.B * A.n * A.H + myrow) * (C.Wv + 1);
+	float* to = part + ((int64_t)(slot - b) * A.n * A.H + myrow) * (C.Wv + 1);  // [slot][n][H]
 	if (part && my0 == 0) to[C.Wv] = d;
 	for (int w = my0; w < C.Wv; w += TR) {
 		const float y = sums[my * 128 + w] + sums[(RB + my) * 128 + w];
@@ -451,51 +508,51 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 	}
 }
 
-// the splits of each row, in their order
+// The sums of each entry's slots, in their order, two heads of a workgroup.  Grid: n, B, heads.
 template <typename ST>
-__global__ void __launch_bounds__(128) paged_join(AttendArgs A, const float* __restrict__ part, const int32_t* __restrict__ seqs, ST* __restrict__ o)
+__global__ void __launch_bounds__(256) paged_join(AttendArgs A, const float* __restrict__ part, const int2* __restrict__ spans, ST* __restrict__ o)
 {
-	const int64_t row = blockIdx.x, rows = (int64_t)A.B * A.n * A.H;
-	const int b = (int)(row / ((int64_t)A.n * A.H));
-	int s;
-	const int len = seq_of(A, seqs, b, s);
-	const int per = split_tokens(A, len), m = len ? (len + per - 1) / per : 0, Wv = A.C.Wv;
+	const int2 S = spans[blockIdx.y];
+	const int Wv = A.C.Wv, w = threadIdx.x & 127, h = 2 * blockIdx.z + (threadIdx.x >> 7);
+	if (w >= Wv || h >= A.H) return;
+	const float* p = part + (((int64_t)S.x * A.n + blockIdx.x) * A.H + h) * (Wv + 1);
+	const int64_t pitch = (int64_t)A.n * A.H * (Wv + 1);
 	float d = 1.f, y = 0.f;
 #pragma unroll 8
-	for (int u = 0; u < m; u++) {
-		const float* p = part + ((int64_t)u * rows + row) * (Wv + 1);
+	for (int u = 0; u < S.y; u++, p += pitch) {
 		d += p[Wv];
-		if ((int)threadIdx.x < Wv) y += p[threadIdx.x];
+		y += p[w];
 	}
-	if ((int)threadIdx.x < Wv) o[row * Wv + threadIdx.x] = (ST)(y / d);
+	o[(((int64_t)blockIdx.y * A.n + blockIdx.x) * A.H + h) * Wv + w] = (ST)(y / d);
 }
 
 // rows of a workgroup
 int row_block(int64_t R) { return R <= 1 ? 1 : R <= 2 ? 2 : R <= 4 ? 4 : R <= 8 ? 8 : 16; }
 
-// Splits of a sequence: as many as fill the 256 compute units with workgroups once (two of 8 or 16 rows, four of fewer rows).
-// For 32 sequences of about 2050 tokens, 4 rows, W 64, twice or four times as many take 19.5 and 19.7 us instead of 19.0; for 16 of
-// about 20480, 16 rows, W 128, 175 and 167 instead of 164, and the sums to join grow.  A table of 512 tokens at most
-// is not split:
-// 12 us for one sequence of 300 tokens, 16.6 with the kernel that joins.
-int splits_for(const L1Cache& C, int rows, int64_t groups)
+// Workgroups of each key head and block of rows: as many as fill the 256 compute units once (two of 8 or 16 rows, four of fewer
+// rows), at least two for each entry.  0: each entry has one, which writes the result itself: 12 us for one sequence of 300
+// tokens, 16.6 with a kernel that joins; and where the entries alone are many.  Dealing out the steps of all entries instead of
+// an equal number of splits for each: 169 -> 140 us for 16 sequences of 8192 to 32768 tokens.
+int slots_for(const L1Cache& C, int64_t B, int rows, int64_t others)
 {
-	const int64_t tokens = (int64_t)C.M * C.P, most = tokens <= 512 ? 1 : l1_cdiv(tokens, rows <= 4 ? 256 : 512);
-	const int64_t want = l1_cdiv(rows <= 4 ? 1024 : 512, groups);
-	return (int)(want > most ? most : want < 1 ? 1 : want);
+	if (B > 512 || (int64_t)C.M * C.P <= 512) return 0;
+	const int64_t want = l1_cdiv(rows <= 4 ? 1024 : 512, others), most = B * l1_cdiv((int64_t)C.M * C.P, rows <= 4 ? 256 : 512);
+	const int64_t n = want > 2 * B ? want : 2 * B;
+	return (int)(n < most + B ? n : most + B);
 }
 
 template <typename ST>
-int attend(const AttendArgs& A, const void* q, const int32_t* seqs, const int32_t* counts, void* o, float* ws, hipStream_t st)
+int attend(const AttendArgs& A, const void* q, const int32_t* seqs, const int32_t* counts, void* o, int2* ws, hipStream_t st)
 {
 	const int rb = row_block((int64_t)A.n * A.G);
-	const dim3 grid((unsigned)(A.B * A.C.Hk), (unsigned)A.splits, (unsigned)l1_cdiv((int64_t)A.n * A.G, rb));
-	float* part = A.splits > 1 ? ws : nullptr;
+	const dim3 grid((unsigned)((A.slots ? A.slots : A.B) * A.C.Hk), (unsigned)l1_cdiv((int64_t)A.n * A.G, rb));
+	int2* spans = A.slots ? ws : nullptr;  // of each entry; behind them the sums
+	float* part = spans ? reinterpret_cast<float*>(ws + A.B) : nullptr;
 	const int full = A.C.pk == A.C.pv ? A.C.pk : 0;  // rows of 64 or 128 bytes: addresses and loops are known to the compiler
 #define L1_ATTEND(RB, MINW)                                                                                                                          \
-	if (full == 64) hipLaunchKernelGGL((paged_attend<ST, RB, 4, true, MINW>), grid, dim3(256), 0, st, A, (const ST*)q, seqs, counts, (ST*)o, part);  \
-	else if (full == 128) hipLaunchKernelGGL((paged_attend<ST, RB, 8, true, 2>), grid, dim3(256), 0, st, A, (const ST*)q, seqs, counts, (ST*)o, part); \
-	else hipLaunchKernelGGL((paged_attend<ST, RB, 8, false, 2>), grid, dim3(256), 0, st, A, (const ST*)q, seqs, counts, (ST*)o, part)
+	if (full == 64) hipLaunchKernelGGL((paged_attend<ST, RB, 4, true, MINW>), grid, dim3(256), 0, st, A, (const ST*)q, seqs, counts, (ST*)o, part, spans);  \
+	else if (full == 128) hipLaunchKernelGGL((paged_attend<ST, RB, 8, true, 2>), grid, dim3(256), 0, st, A, (const ST*)q, seqs, counts, (ST*)o, part, spans); \
+	else hipLaunchKernelGGL((paged_attend<ST, RB, 8, false, 2>), grid, dim3(256), 0, st, A, (const ST*)q, seqs, counts, (ST*)o, part, spans)
 	if (rb == 1) { L1_ATTEND(1, 4); }
 	else if (rb == 2) { L1_ATTEND(2, 4); }
 	else if (rb == 4) { L1_ATTEND(4, 4); }
@@ -504,7 +561,7 @@ int attend(const AttendArgs& A, const void* q, const int32_t* seqs, const int32_
 #undef L1_ATTEND
 	L1_LAUNCH_CHECK();
 	if (part) {
-		hipLaunchKernelGGL(paged_join<ST>, dim3((unsigned)(A.B * A.n * A.H)), dim3(128), 0, st, A, part, seqs, (ST*)o);
+		hipLaunchKernelGGL(paged_join<ST>, dim3((unsigned)A.n, (unsigned)A.B, (unsigned)((A.H + 1) / 2)), dim3(256), 0, st, A, part, spans, (ST*)o);
 		L1_LAUNCH_CHECK();
 	}
 	return L1ATTN_OK;
@@ -527,9 +584,9 @@ int check_attend(const l1attn_cache* cache, const l1attn_attend_desc* d, AttendA
 	A->rw = (float)(1.0 / sqrt((double)A->C.W));
 	for (int h = 0; h < 256; h++) A->slopes[h] = d->slopes && h < d->H ? d->slopes[h] : 0.f;
 	if (d->B == 0 || d->n == 0) return 1;
-	const int64_t groups = d->B * A->C.Hk * l1_cdiv(d->n * A->G, row_block(d->n * A->G));
-	A->step = row_block(d->n * A->G) <= 4 ? 256 : 512;
-	A->splits = splits_for(A->C, row_block(d->n * A->G), groups);
+	const int rb = row_block(d->n * A->G);
+	A->step = rb <= 4 ? 256 : 512;
+	A->slots = slots_for(A->C, d->B, rb, A->C.Hk * l1_cdiv(d->n * A->G, rb));
 	return L1ATTN_OK;
 }
 
@@ -540,8 +597,8 @@ extern "C" {
 size_t l1attn_cache_attend_workspace_bytes(const l1attn_cache* cache, const l1attn_attend_desc* desc)
 {
 	AttendArgs A;
-	if (check_attend(cache, desc, &A) || A.splits == 1) return 0;
-	return (size_t)A.splits * A.B * A.n * A.H * (A.C.Wv + 1) * sizeof(float);
+	if (check_attend(cache, desc, &A) || !A.slots) return 0;
+	return A.B * sizeof(int2) + (size_t)A.slots * A.n * A.H * (A.C.Wv + 1) * sizeof(float);
 }
 
 int l1attn_cache_attend(const l1attn_cache* cache, const l1attn_attend_desc* desc, const void* q, const int32_t* seqs, const int32_t* counts,
@@ -552,11 +609,11 @@ int l1attn_cache_attend(const l1attn_cache* cache, const l1attn_attend_desc* des
 	if (rc) return rc == 1 ? L1ATTN_OK : rc;
 	if (!q || !o) return L1ATTN_ERR_ARG;
 	const size_t need = l1attn_cache_attend_workspace_bytes(cache, desc);
-	if (need && (!workspace || workspace_bytes < need)) return L1ATTN_ERR_WORKSPACE;
+	if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 8)) return L1ATTN_ERR_WORKSPACE;
 	hipStream_t st = (hipStream_t)stream;
-	if (desc->dtype == 0) return attend<float>(A, q, seqs, counts, o, (float*)workspace, st);
-	if (desc->dtype == 1) return attend<_Float16>(A, q, seqs, counts, o, (float*)workspace, st);
-	return attend<__bf16>(A, q, seqs, counts, o, (float*)workspace, st);
+	if (desc->dtype == 0) return attend<float>(A, q, seqs, counts, o, (int2*)workspace, st);
+	if (desc->dtype == 1) return attend<_Float16>(A, q, seqs, counts, o, (int2*)workspace, st);
+	return attend<__bf16>(A, q, seqs, counts, o, (int2*)workspace, st);
 }
 
 }  // extern "C"

@@ -58,7 +58,7 @@ __device__ __forceinline__ int named_once(const int32_t* seqs, int b, int B, int
 	return b < B && s >= 0 && s < rows && !(seqs && named_before(ids, b, s)) ? s : -1;
 }
 
-// What an append() takes, by one workgroup, a thread for each of its rows: where each row's tokens go and which pages they get.
+// (8.9 us for 64 rows: a chain of dependent reads and scans, one workgroup.)  What an append() takes, by one workgroup, a thread for each of its rows: where each row's tokens go and which pages they get.
 // plan[b] = {sequence or -1, first place, tokens, the page to copy from or -1}; take[b][j]: the page that holds the j-th page
 // of the row's new tokens.
 __global__ void __launch_bounds__(kRows) cache_take(L1Cache C, const int32_t* __restrict__ seqs, const int32_t* __restrict__ counts, int B, int n,
@@ -298,7 +298,8 @@ __global__ void __launch_bounds__(kRows) cache_order(L1Cache C, const int32_t* _
 	}
 }
 
-// second part: page r of those behind n_live moves into the r-th hole
+// second part: page r of those behind n_live moves into the r-th hole; bound by the copy (54 us for 205 MB read and written, 43 at a
+// large copy's rate)
 __global__ void __launch_bounds__(256) cache_move(L1Cache C, const int32_t* __restrict__ live, const int32_t* __restrict__ holes,
                                                   int32_t* __restrict__ map, const int32_t* __restrict__ sums)
 {
@@ -335,7 +336,9 @@ __global__ void __launch_bounds__(256) cache_rename(L1Cache C, const int32_t* __
 
 template <typename ST> __device__ __forceinline__ float value(ST x) { return (float)x; }
 
-// Tokens into pages: a workgroup for each page of each row and head, keys (z 0) and values (z 1).  The page's scale becomes
+// Tokens into pages: a workgroup for each page of each row and head, keys (z 0) and values (z 1): the values are read twice, for
+// the scale and for the codes, the second time from the caches (29 us for 8 rows of up to 2000 tokens, 8 heads, W 128, bfloat16:
+// 48 MB read, 24 MB written; 4.6 us for one token of 64 rows).  The page's scale becomes
 // the larger of what it was (if it held tokens) and the new tokens' largest magnitude over 127; if it grew, or the page is a
 // copy of a shared one, the codes that were there are written again.  A value that is not finite does not count for the
 // scale: infinities are coded as +-127, NaN as 0.  G: elements a thread holds side by side.

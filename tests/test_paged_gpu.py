@@ -191,6 +191,21 @@ def test_small_and_large_inputs(H, n, W, scale, dtype):
     c.attend(3, n, H, q=near + 0.1 * scale * torch.randn(near.shape, generator=c.g))
 
 
+@pytest.mark.parametrize("B,H,n", [(300, 2, 1), (300, 4, 5), (513, 2, 2)])
+def test_many_entries(B, H, n):
+    # every row of the table many times, in no order, some that are not there; uneven lengths over several steps
+    c = Pair(N=200, P=32, Hk=1, W=64, Wv=64, rows=7, M=40, seed=9)
+    c.append(7, 1200, counts=[1200, 0, 1, 513, 256, 800, 40])
+    seqs = torch.randint(-1, 8, (B,), generator=c.g).tolist()
+    q = torch.randn(7, n, H, 64, generator=c.g).to(BF16)
+    each = c.attend(7, n, H, q=q)
+    o = c.m.l1attn_paged(torch.stack([q[s % 7] for s in seqs]).cuda(), c.gpu, seqs=c.ints(seqs))
+    ref, terms = c.plain.attend(q)
+    none = torch.zeros_like(ref[0])
+    lf.check([o], [torch.stack([ref[s] if 0 <= s < 7 else none for s in seqs])], [torch.stack([terms[s] if 0 <= s < 7 else none for s in seqs])], BF16, 64, names=("o",))
+    assert each.shape == q.shape
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("H", [2, 20])
 def test_scales_of_hidden_tokens_have_no_influence(H, dtype):
