@@ -8,7 +8,7 @@
 // order.  Every byte of the cache is read once for up to 16 rows.
 // Distances.  Up to 4 rows, and float32: float32, two instructions an element and row.  From 5 rows of 16 bits on: sums of
 // |difference| of 16-bit codes (v_sad_u16, two elements an instruction) on one grid over the rows' values and over what the
-// scales of the workgroup's pages allow (127 times the largest); a code is off by half a step at most, which moves a logit by
+// scales of the workgroup's pages allow (128 times the largest); a code is off by half a step at most, which moves a logit by
 // 0.41 steps on average.  Past a range of 24 (float16; 160 bfloat16), where that would reach the type's own rounding, or where a
 // row or scale is not finite, float32.
 // Sums.  Weight times scale is rounded to the rows' type (float16 at 2^14 over the power of two above the step's largest scale),
@@ -200,8 +200,8 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 			finite &= __builtin_fabsf(y) <= 3.402823466e38f;
 			kmax = fmaxf(kmax, __builtin_fabsf(y));
 		}
-		least = fminf(least, -127.f * kmax);
-		most = fmaxf(most, 127.f * kmax);
+		least = fminf(least, -128.f * kmax);
+		most = fmaxf(most, 128.f * kmax);  // a negative scale as well, and the code -128: from a pool that the caller filled
 #pragma unroll
 		for (int k = 32; k; k >>= 1) {
 			least = fminf(least, __shfl_xor(least, k));

@@ -58,7 +58,8 @@ __device__ __forceinline__ int named_once(const int32_t* seqs, int b, int B, int
 	return b < B && s >= 0 && s < rows && !(seqs && named_before(ids, b, s)) ? s : -1;
 }
 
-// (8.9 us for 64 rows: a chain of dependent reads and scans, one workgroup.)  What an append() takes, by one workgroup, a thread for each of its rows: where each row's tokens go and which pages they get.
+// What an append() takes, by one workgroup, a thread for each of its rows: where each row's tokens go and which pages they get.
+// A chain of dependent reads and scans: @TAKE us for 64 rows.
 // plan[b] = {sequence or -1, first place, tokens, the page to copy from or -1}; take[b][j]: the page that holds the j-th page
 // of the row's new tokens.
 __global__ void __launch_bounds__(kRows) cache_take(L1Cache C, const int32_t* __restrict__ seqs, const int32_t* __restrict__ counts, int B, int n,
@@ -98,7 +99,7 @@ __global__ void __launch_bounds__(kRows) cache_take(L1Cache C, const int32_t* __
 	held[b] = cnt > 0 ? (start + cnt + C.P - 1) / C.P - start / C.P : 0;
 	ids[b] = last;
 	__syncthreads();
-	for (int64_t x = b; x < (int64_t)B * J; x += kRows) {
+	for (int64_t x = b; x < (int64_t)B * J; x += blockDim.x) {
 		const int r = (int)(x / J), j = (int)(x % J);
 		int page = -1;
 		if (j < held[r]) {
@@ -112,14 +113,12 @@ __global__ void __launch_bounds__(kRows) cache_take(L1Cache C, const int32_t* __
 		take[x] = page;
 	}
 	if (ok) C.lens[s] = start + cnt;
-	__syncthreads();
+	if (!__syncthreads_or(share)) {
+		if (b == 0) *C.n_free = top - total;
+		return;
+	}
 	// the shared pages that were written to lose a holder; those that lose the last one are free again, in ascending order
-	if (share) atomicSub(&C.refs[last], 1);
-	__threadfence();
-	first[b] = share ? last : -1;
-	__syncthreads();
-	bool freed = share && __hip_atomic_load(&C.refs[last], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0;
-	freed = freed && !named_before(first, b, last);
+	const bool freed = share && atomicSub(&C.refs[last], 1) == 1;
 	held[b] = freed ? last : -1;
 	__syncthreads();
 	int gone;
@@ -459,7 +458,7 @@ int l1attn_cache_append(const l1attn_cache* cache, int dtype, const void* k, con
 	hipStream_t st = (hipStream_t)stream;
 	int4* plan = (int4*)workspace;
 	int32_t* take = (int32_t*)(plan + B);
-	hipLaunchKernelGGL(cache_take, dim3(1), dim3(kRows), 0, st, C, seqs, counts, (int)B, (int)n, J, served, plan, take);
+	hipLaunchKernelGGL(cache_take, dim3(1), dim3((unsigned)l1_align_up((size_t)B, 64)), 0, st, C, seqs, counts, (int)B, (int)n, J, served, plan, take);
 	L1_LAUNCH_CHECK();
 	if (n == 0) return L1ATTN_OK;
 	if (dtype == 0) return write_tokens<float>(C, k, v, (int)B, (int)n, J, plan, take, st);
@@ -479,7 +478,7 @@ int l1attn_cache_fork(const l1attn_cache* cache, const int32_t* parents, const i
 	if (!parents || !children || !served) return L1ATTN_ERR_ARG;
 	if (!workspace || workspace_bytes < (size_t)B * sizeof(int32_t)) return L1ATTN_ERR_WORKSPACE;
 	hipStream_t st = (hipStream_t)stream;
-	hipLaunchKernelGGL(cache_fork, dim3(1), dim3(kRows), 0, st, C, parents, children, (int)B, served, (int32_t*)workspace);
+	hipLaunchKernelGGL(cache_fork, dim3(1), dim3((unsigned)l1_align_up((size_t)B, 64)), 0, st, C, parents, children, (int)B, served, (int32_t*)workspace);
 	L1_LAUNCH_CHECK();
 	hipLaunchKernelGGL(cache_fork_rows, dim3((unsigned)B, (unsigned)min((int64_t)64, l1_cdiv(C.M + 1, 1024))), dim3(256), 0, st, C, parents, children, served, (const int32_t*)workspace);
 	L1_LAUNCH_CHECK();

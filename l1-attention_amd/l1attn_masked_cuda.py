@@ -10,12 +10,12 @@ No counterpart in the reference, whose model code composes an unmasked form from
 
 q [B,T,H,W], k [B,S,Hk,W], v [B,S,Hk,Wv] of one type (float32, float16, bfloat16), T <= S, H a multiple of Hk, widths up to
 128: the queries are the last T of the S tokens (T < S: a prompt worked off in chunks).  Token s is visible to token i where
-causal is off, or s <= i, or s < prefix[b] (int32 [B]: a prefix that sees all of itself), and, with doc (int32 [B,S]), where
-both are of one document: equal numbers >= 0; a negative number is padding, which sees nothing and is seen by nothing.  A row
-that sees nothing is zero, as are its gradients.  The 1 in the denominator is the framework's no-op logit.
+causal is off, or s <= i, or s < prefix[b] (int32 [B]: a prefix that sees all of itself; without causal it changes nothing),
+and, with doc (int32 [B,S]), where both are of one document: equal numbers >= 0; a negative number is padding, which sees
+nothing and is seen by nothing.  A row that sees nothing is zero, as are its gradients.  The 1 in the denominator is the framework's no-op logit.
 
 slopes: H numbers >= 0 (constants, no gradient).  softcap >= 0, 0 for none.  Calls on several streams and in graph capture
-are fine: a call keeps nothing.
+are fine: a call keeps nothing.  As with any operator, a backward pass is captured with no eager graph of the same leaves alive.
 """
 from torch import nn
 from torch.autograd import Function

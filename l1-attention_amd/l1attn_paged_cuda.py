@@ -29,7 +29,7 @@ def _round16(n):
 
 
 class L1PagedCache(object):
-    """The state, as tensors that the caller may keep, copy and load:
+    """The state, as tensors that the caller may keep, copy and load (in place):
 
     k_pages [N,Hk,page,W up to a multiple of 16] and v_pages (with Wv) int8; k_scale, v_scale [N,Hk] float32;
     table [rows,row_pages] int32, the pages of each sequence; lens [rows] int32, its tokens; refs [N] int32, rows that hold the
@@ -61,6 +61,12 @@ class L1PagedCache(object):
         self.device = k_pages.device
         self._desc = _drv.CacheDesc(N, page, Hk, W, Wv, rows, row_pages, *(x.data_ptr() for x in (
             k_pages, v_pages, k_scale, v_scale, table, lens, refs, free, n_free)))
+
+    def __setattr__(self, name, value):
+        # the kernels go by the tensors' addresses, taken once
+        if "_desc" in self.__dict__:
+            raise AttributeError("the state of a cache is written in place (%s.copy_(...)), or a new cache is made of other tensors" % name)
+        super(L1PagedCache, self).__setattr__(name, value)
 
     @classmethod
     def empty(cls, n_pages, page, n_key_heads, width, n_rows, row_pages, v_width=None, device=None):

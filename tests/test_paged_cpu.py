@@ -41,6 +41,14 @@ def test_state_is_checked(no_gpu):
         m.L1PagedCache(**{**good, "k_pages": odd})
 
 
+def test_state_is_not_exchanged(no_gpu):
+    c = _cache()
+    with pytest.raises(AttributeError, match="in place"):
+        c.lens = torch.zeros_like(c.lens)
+    c.lens.copy_(torch.ones_like(c.lens))
+    assert c.lens.tolist() == [1, 1, 1]
+
+
 def test_calls_are_checked(no_gpu):
     import l1attn_paged_cuda as m
     c = _cache()

@@ -238,6 +238,21 @@ def test_two_calls_at_once(H):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("H", [2, 12])
+def test_a_pool_that_the_caller_filled(H, dtype):
+    # every code there is, and scales of either sign
+    c = Pair(N=30, P=16, Hk=2, W=64, Wv=64, rows=2, M=10, dtype=dtype, seed=8)
+    c.append(2, 150, counts=[150, 20])
+    for to, codes in ((c.gpu.k_pages, c.plain.pages[0]), (c.gpu.v_pages, c.plain.pages[1])):
+        codes.copy_(torch.randint(-128, 128, codes.shape, generator=c.g).to(torch.int8))
+        to.copy_(codes)
+    for to, scale in ((c.gpu.k_scale, c.plain.scale[0]), (c.gpu.v_scale, c.plain.scale[1])):
+        scale.copy_((torch.rand(scale.shape, generator=c.g) - 0.5) / 64)
+        to.copy_(scale)
+    c.attend(2, 2, H)
+
+
 def test_pages_that_are_not_there_give_no_tokens():
     c = Pair(N=40, rows=2, M=8)
     c.append(2, 100)
