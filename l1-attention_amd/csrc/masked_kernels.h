@@ -58,7 +58,7 @@ template <typename ST> constexpr bool k16 = sizeof(ST) == 2;
 // type, 2^-12 (float16) and 2^-9 (bfloat16) on average
 template <typename ST> constexpr float kRange = 24.f;
 template <> constexpr float kRange<__bf16> = 160.f;
-// what a weight is multiplied by: p <= 1, and is rounded to 16 bits for the products; float16 has no room below 2^-14
+// what a weight is multiplied by: p <= 1, and goes into the products as 16-bit numbers; float16 has no room below 2^-14
 template <typename ST> constexpr float kWeight = 1.f;
 template <> constexpr float kWeight<_Float16> = 16384.f;
 
@@ -516,25 +516,30 @@ __device__ __forceinline__ f4 mma16(const uint4& a, const uint4& b, f4 c)
 }
 
 // Weights of half a tile into the wave's scratch, and acc[tb][wb] += sum over its 32 columns c of value[c][16 wb + ..] * p[owner][c].
-// 16 bits: rounded to the type (a relative error of half a step of the type in each weight, as the
-// product's other factor has).
+// 16 bits: a weight is the sum of two numbers of the type, itself rounded and what that leaves out: one alone, half a step off, made
+// the results half as inexact again as their own rounding.
 // `bad` (values that are not finite in a tile of which some is hidden): a hidden pair's weight of zero must not meet them, which
 // a matrix instruction cannot leave out.
 template <typename ST, int NB, int TB>
 __device__ __forceinline__ void weigh(f4 (&acc)[2][NB], char* scr, const char* y, const char* yt, int sy, int Wv, const float (&p)[4][4], int half,
                                       int i, int j, int l16, int g, bool bad)
 {
-	constexpr int pitch = k16<ST> ? 80 : kPad * 4;  // bytes of an owner's 32 weights: odd chunks
+	constexpr int pitch = kPad * 4;  // bytes of an owner's 32 weights, of 16 bits the second parts behind the first: odd chunks
 	wave_sync();
 #pragma unroll
 	for (int a = 0; a < 4; a++) {
 		if constexpr (k16<ST>) {
-			ST w[4];
+			ST w[4], rest[4];
 #pragma unroll
-			for (int e = 0; e < 4; e++) w[e] = (ST)p[a][e];
+			for (int e = 0; e < 4; e++) {
+				w[e] = (ST)p[a][e];
+				rest[e] = (ST)(p[a][e] - (float)w[e]);
+			}
 			uint2 packed;
 			__builtin_memcpy(&packed, w, 8);
 			*reinterpret_cast<uint2*>(scr + (i + 8 * a) * pitch + 8 * j) = packed;
+			__builtin_memcpy(&packed, rest, 8);
+			*reinterpret_cast<uint2*>(scr + (i + 8 * a) * pitch + 64 + 8 * j) = packed;
 		} else {
 			const f4 w = {p[a][0], p[a][1], p[a][2], p[a][3]};
 			*reinterpret_cast<f4*>(scr + (i + 8 * a) * pitch + 16 * j) = w;
@@ -545,7 +550,8 @@ __device__ __forceinline__ void weigh(f4 (&acc)[2][NB], char* scr, const char* y
 		for (int c = 0; c < 32; c++)
 #pragma unroll
 			for (int tb = 0; tb < 2; tb++) {
-				const float w = to_f(*reinterpret_cast<const ST*>(scr + (l16 + 16 * tb) * pitch + (int)sizeof(ST) * c));
+				const char* at = scr + (l16 + 16 * tb) * pitch + (int)sizeof(ST) * c;
+				const float w = to_f(*reinterpret_cast<const ST*>(at)) + (k16<ST> ? to_f(*reinterpret_cast<const ST*>(at + 64)) : 0.f);
 				if (w != 0.f)
 #pragma unroll
 					for (int wb = 0; wb < NB; wb++)
@@ -577,15 +583,18 @@ __device__ __forceinline__ void weigh(f4 (&acc)[2][NB], char* scr, const char* y
 		}
 	} else {
 		const int blocks = (Wv + 15) >> 4;
-		uint4 pb[2];
+		uint4 pb[2], rest[2];
 #pragma unroll
-		for (int tb = 0; tb < 2; tb++) pb[tb] = *reinterpret_cast<const uint4*>(scr + (l16 + 16 * tb) * pitch + 16 * g);
+		for (int tb = 0; tb < 2; tb++) {
+			pb[tb] = *reinterpret_cast<const uint4*>(scr + (l16 + 16 * tb) * pitch + 16 * g);
+			rest[tb] = *reinterpret_cast<const uint4*>(scr + (l16 + 16 * tb) * pitch + 64 + 16 * g);
+		}
 #pragma unroll
 		for (int wb = 0; wb < NB; wb++) {
 			if (wb >= blocks) break;
 			const uint4 av = *reinterpret_cast<const uint4*>(yt + (16 * wb + l16) * kPitch(TB) * 2 + 64 * half + 16 * g);
 #pragma unroll
-			for (int tb = 0; tb < 2; tb++) acc[tb][wb] = mma16<ST>(av, pb[tb], acc[tb][wb]);
+			for (int tb = 0; tb < 2; tb++) acc[tb][wb] = mma16<ST>(av, rest[tb], mma16<ST>(av, pb[tb], acc[tb][wb]));
 		}
 	}
 }

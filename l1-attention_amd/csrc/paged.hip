@@ -11,10 +11,11 @@
 // scales of the workgroup's pages allow (128 times the largest); a code is off by half a step at most, which moves a logit by
 // 0.41 steps on average.  Past a range of 24 (float16; 160 bfloat16), where that would reach the type's own rounding, or where a
 // row or scale is not finite, float32.
-// Sums.  Weight times scale is rounded to the rows' type (float16 at 2^14 over the power of two above the step's largest scale),
-// a code is exact in it, and matrix instructions add them in float32; float32 has its own matrix instruction.
-// What bounds it: for few rows latency and the reads (32 sequences of about 2050 tokens, 4 rows, W 64, bfloat16: 34 MB in 17 us),
-// for many the vector ALU (16 of about 20480, 16 rows, W 128, float16: 137 us at 2.4 TB/s; 43 of 100 vector instructions are
+// Sums.  Weight times scale is two numbers of the rows' type, itself rounded and what that leaves out (float16 at 2^14 over the
+// power of two above the step's largest scale; one number alone made results 1.6 times as inexact as their own rounding), a code is
+// exact in it, and matrix instructions add them in float32; float32 has its own matrix instruction.
+// What bounds it: for few rows latency and the reads (32 sequences of about 2050 tokens, 4 rows, W 64, bfloat16: 34 MB in 17 us, and 4 for the join),
+// for many the vector ALU (16 of about 20480, 16 rows, W 128, float16: 140 us at 2.4 TB/s; 43 of 100 vector instructions are
 // v_sad_u16, which issue in about 4.2 cycles each; the rest makes codes and float16 of the cache's bytes, and weights).  With
 // one token a lane instead of two at 16 rows a row's codes would be read from LDS twice as often.
 #include "paged.h"
@@ -132,9 +133,10 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 	constexpr bool LATE = RB >= 8;  // values are asked for behind the distances: registers hold the rows' codes read ahead (183 -> 164 us)
 	constexpr int U = RB <= 4 ? 1 : 2, VG = NC / 4, KB = RB >= 8 ? 2 : 4;  // KB: pieces of 16 bytes of a key row under way
 	constexpr int pitch = 64 * U + (F32 ? 4 : 8);                          // between two rows' weights: an odd number of 16-byte pieces
-	using PT = ST;  // weights are rounded to the type of the rows
+	using PT = ST;
 	constexpr int TR = 256 / RB;  // threads of a row before and behind the loop
-	constexpr int pool = 4 * RB * pitch * (int)sizeof(PT), join = 2 * RB * 128 * 4;
+	constexpr int plane = F32 ? 0 : RB * pitch;  // 16-bit weights: what their rounding leaves out lies behind them
+	constexpr int pool = 4 * (RB * pitch + plane) * (int)sizeof(PT), join = 2 * RB * 128 * 4;
 	__shared__ __align__(16) float qs[RB * 128];
 	__shared__ __align__(16) unsigned qc[CODED ? RB * 64 : 1];
 	__shared__ __align__(16) char shared_pool[pool > join ? pool : join];
@@ -223,7 +225,7 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 		}
 	}
 	__syncthreads();
-	PT* ps = reinterpret_cast<PT*>(shared_pool) + wave * RB * pitch;
+	PT* ps = reinterpret_cast<PT*>(shared_pool) + wave * (RB * pitch + plane);
 	const int kchunks = FULL ? NC : pk / 16;
 	float den[RB];
 	f4 acc[VG][4];
@@ -421,7 +423,10 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 				const float w = exponential<ST>(__builtin_fmaf(-slope[r], (float)(place[r] - t), dist[u][r]));
 				const float p = sees <= place[r] ? w : 0.f;
 				den[r] += p;
-				ps[r * pitch + 64 * u + lane] = (PT)(p != 0.f ? p * scale : 0.f);  // the scale of a hidden token has no influence
+				const float both = p != 0.f ? p * scale : 0.f;  // the scale of a hidden token has no influence
+				const PT first = (PT)both;
+				ps[r * pitch + 64 * u + lane] = first;
+				if constexpr (!F32) ps[plane + r * pitch + 64 * u + lane] = (PT)(both - (float)first);
 			}
 		}
 		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -434,6 +439,7 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 #pragma unroll
 			for (int kc = 0; kc < 16 * U / VT; kc++) {
 				const uint4 pa = *reinterpret_cast<const uint4*>(ps + l16 % RB * pitch + 4 * VT * kc + VT * g);
+				const uint4 rest = *reinterpret_cast<const uint4*>(ps + plane + l16 % RB * pitch + 4 * VT * kc + VT * g);
 				if constexpr (F32) {
 					const float a[4] = {__builtin_bit_cast(float, pa.x), __builtin_bit_cast(float, pa.y), __builtin_bit_cast(float, pa.z), __builtin_bit_cast(float, pa.w)};
 #pragma unroll
@@ -461,8 +467,12 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 							}
 						}
 						const uint4 pb = make_uint4(x[0], x[1], x[2], x[3]);
-						if constexpr (HALF) y[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, pa), __builtin_bit_cast(h8, pb), y[e], 0, 0, 0);
-						else y[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, pa), __builtin_bit_cast(b8, pb), y[e], 0, 0, 0);
+#pragma unroll
+						for (int d = 0; d < 2; d++) {
+							const uint4 w = d ? rest : pa;
+							if constexpr (HALF) y[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, w), __builtin_bit_cast(h8, pb), y[e], 0, 0, 0);
+							else y[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, w), __builtin_bit_cast(b8, pb), y[e], 0, 0, 0);
+						}
 					}
 				}
 			}
