@@ -113,9 +113,12 @@ def _masked_desc(q, k, v, doc, prefix, causal, softcap, slopes):
     if not (1 <= W <= 128 and 1 <= Wv <= 128):
         raise RuntimeError("widths of masked attention are 1 to 128, got %d and %d" % (W, Wv))
     _check_rule(H, softcap, slopes)
-    return MaskedDesc(B, T, S, H, Hk, W, Wv, DTYPES[q.dtype], int(bool(causal)), softcap,
-                      None if slopes is None else ctypes.addressof(_slopes_array(slopes)),
-                      _index_tensor(doc, "doc", (B, S), q), _index_tensor(prefix, "prefix", (B,), q))
+    numbers = None if slopes is None else _slopes_array(slopes)
+    d = MaskedDesc(B, T, S, H, Hk, W, Wv, DTYPES[q.dtype], int(bool(causal)), softcap,
+                   None if slopes is None else ctypes.addressof(numbers),
+                   _index_tensor(doc, "doc", (B, S), q), _index_tensor(prefix, "prefix", (B,), q))
+    d.numbers = numbers  # lives as long as the address
+    return d
 
 
 def masked_forward(q, k, v, doc=None, prefix=None, causal=True, softcap=0.0, slopes=None, want_lse=True):
@@ -265,7 +268,8 @@ def cache_attend(desc, device, q, seqs=None, counts=None, softcap=0.0, slopes=No
         raise RuntimeError("attend: %d sequences without a list, but the cache has %d rows" % (B, desc.rows))
     _check_rule(H, softcap, slopes)
     sp, cp = _row_list(seqs, "seqs", B, device), _row_list(counts, "counts", B, device)
-    a = AttendDesc(B, n, H, DTYPES[q.dtype], softcap, None if slopes is None else ctypes.addressof(_slopes_array(slopes)))
+    numbers = None if slopes is None else _slopes_array(slopes)
+    a = AttendDesc(B, n, H, DTYPES[q.dtype], softcap, None if slopes is None else ctypes.addressof(numbers))
     o = torch.empty((B, n, H, desc.Wv), dtype=q.dtype, device=device)
     L, d, ap = lib(), ctypes.addressof(desc), ctypes.addressof(a)
     with torch.cuda.device(device):
