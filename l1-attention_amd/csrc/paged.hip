@@ -254,6 +254,7 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 		a = there ? x : 0.f;
 		c = there ? y : 0.f;
 	};
+	if (first < hi)  // else the pool may have no page
 #pragma unroll
 	for (int u = 0; u < U; u++) {
 		locate(page[u], pg[u], krow[u], ks[u], vs[u]);
@@ -397,8 +398,9 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 		// exponents reach as far as float32's
 		float up = 1.f, down = 1.f;
 		if constexpr (HALF) {
-			float most = __builtin_fabsf(vs[0]);
-			if constexpr (U == 2) most = fmaxf(most, __builtin_fabsf(vs[1]));
+			float most = 0.f;
+#pragma unroll
+			for (int u = 0; u < U; u++) most = fmaxf(most, __builtin_fabsf(vs[u]) <= 3.402823466e38f ? __builtin_fabsf(vs[u]) : 0.f);  // a hidden token's may be anything
 #pragma unroll
 			for (int k = 32; k; k >>= 1) most = fmaxf(most, __shfl_xor(most, k));
 			const int ve = most > 0.f ? max(__builtin_amdgcn_frexp_expf(most), -100) : 0;

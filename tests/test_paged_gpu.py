@@ -214,10 +214,14 @@ def test_scales_of_hidden_tokens_have_no_influence(H, dtype):
     c.append(2, 100, counts=[100, 90])
     q = torch.randn(1, 40, H, 64, generator=c.g).to(dtype).cuda()
     want = c.m.l1attn_paged(q, c.gpu)
+    if dtype == F16:  # weights times scale that float16 holds only at the right power of two: values up to 2000
+        c.gpu.v_scale.mul_(512)
+        want = c.m.l1attn_paged(q, c.gpu)
     last = int(c.gpu.table[0, 6])  # tokens 96 to 99: the last four query tokens see them
     c.gpu.k_scale[last], c.gpu.v_scale[last] = float("nan"), float("inf")
     got = c.m.l1attn_paged(q, c.gpu)
-    tol = 2 * (torch.finfo(dtype).eps + 2.0 ** -24 * (3 * 64 + 64)) * 4.5  # both within the bound of lm_forms, of values up to 4.5
+    big = 4.5 * (512 if dtype == F16 else 1)
+    tol = 2 * (torch.finfo(dtype).eps + 2.0 ** -24 * (3 * 64 + 64)) * big  # both within the bound of lm_forms, of values up to `big`
     assert (got[:, :36].float() - want[:, :36].float()).abs().max() <= tol
 
 
