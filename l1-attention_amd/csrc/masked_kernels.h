@@ -518,11 +518,11 @@ __device__ __forceinline__ f4 mma16(const uint4& a, const uint4& b, f4 c)
 // Weights of half a tile into the wave's scratch, and acc[tb][wb] += sum over its 32 columns c of value[c][16 wb + ..] * p[owner][c].
 // 16 bits: a weight is the sum of two numbers of the type, itself rounded and what that leaves out: one alone, half a step off, made
 // the results half as inexact again as their own rounding.
-// `bad` (values that are not finite in a tile of which some is hidden): a hidden pair's weight of zero must not meet them, which
-// a matrix instruction cannot leave out.
+// far: 0, or what is visible of a tile with values that are not finite, 2 if some of it is hidden: a hidden pair's weight of zero must
+// not meet them, which a matrix instruction cannot leave out; 1 if nothing is: a weight's second part, zero, must not meet them.
 template <typename ST, int NB, int TB>
 __device__ __forceinline__ void weigh(f4 (&acc)[2][NB], char* scr, const char* y, const char* yt, int sy, int Wv, const float (&p)[4][4], int half,
-                                      int i, int j, int l16, int g, bool bad)
+                                      int i, int j, int l16, int g, int far)
 {
 	constexpr int pitch = kPad * 4;  // bytes of an owner's 32 weights, of 16 bits the second parts behind the first: odd chunks
 	wave_sync();
@@ -546,13 +546,13 @@ __device__ __forceinline__ void weigh(f4 (&acc)[2][NB], char* scr, const char* y
 		}
 	}
 	wave_sync();
-	if (bad) {
+	if (far) {
 		for (int c = 0; c < 32; c++)
 #pragma unroll
 			for (int tb = 0; tb < 2; tb++) {
 				const char* at = scr + (l16 + 16 * tb) * pitch + (int)sizeof(ST) * c;
 				const float w = to_f(*reinterpret_cast<const ST*>(at)) + (k16<ST> ? to_f(*reinterpret_cast<const ST*>(at + 64)) : 0.f);
-				if (w != 0.f)
+				if (w != 0.f || far == 1)
 #pragma unroll
 					for (int wb = 0; wb < NB; wb++)
 #pragma unroll
@@ -889,7 +889,7 @@ __global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* 
 			                   A.vec & 4, s0, A.S, tid, threads);
 			next = next_tile(cls, next + 1, n);
 			if (next < n) F.fetch(kh, kpitch, A.W, A.vec & 2, vh, vpitch, A.Wv, A.vec & 4, (t0 + step * next) * kTile<TB>, A.S, doc, nullptr, nullptr, 0, tid, threads);
-			bad = __syncthreads_or(bad && kind == 2);
+			const int far = __syncthreads_or(bad && (k16<ST> || kind == 2)) ? kind : 0;
 			int mykind = row0 < A.T ? kind : 0;
 			if (mykind == 2) {
 				mykind = place_class<false>(A, prefix, my_lo, my_hi, s0, min(s0 + kTile<TB>, A.S) - 1, s0 + kTile<TB> <= A.S);
@@ -943,8 +943,8 @@ __global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* 
 				for (int bb = 0; bb < 4; bb++)
 #pragma unroll
 					for (int a = 0; a < 4; a++) den[a] += p[a][bb];
-				if constexpr (k16<ST>) weigh<ST, NB, TB>(out, scr, y, yt, Y.sy, A.Wv, p, half, i, j, l16, g, bad);
-				else weigh<ST, NB, TB>(tile, scr, y, yt, Y.sy, A.Wv, p, half, i, j, l16, g, bad);
+				if constexpr (k16<ST>) weigh<ST, NB, TB>(out, scr, y, yt, Y.sy, A.Wv, p, half, i, j, l16, g, far);
+				else weigh<ST, NB, TB>(tile, scr, y, yt, Y.sy, A.Wv, p, half, i, j, l16, g, far);
 			}
 			if constexpr (!k16<ST>)
 #pragma unroll
@@ -1226,7 +1226,7 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 				                   str_y, y_pitch, A.Wv, y_vec, s0, K.str_rows, tid, threads);
 				next = next_tile(cls, next + 1, n);
 				if (next < n) F.fetch(str_x, str_pitch, A.W, str_vec, str_y, y_pitch, A.Wv, y_vec, (t0 + step * next) * kTile<TB>, K.str_rows, str_doc, lh, Dh, A.H, tid, threads);
-				bad = __syncthreads_or(bad && kind == 2);
+				const int far = __syncthreads_or(bad && (k16<ST> || kind == 2)) ? kind : 0;
 				int mykind = row0 < K.own_rows ? kind : 0;
 				if (mykind == 2) {
 					mykind = place_class<OWNK>(A, prefix, my_lo, my_hi, K.str_place0 + s0, K.str_place0 + min(s0 + kTile<TB>, K.str_rows) - 1, s0 + kTile<TB> <= K.str_rows);
@@ -1277,7 +1277,7 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 							}
 						}
 					}
-					if constexpr (OWNK) weigh<ST, NY, TB>(dyv, scr, y, yt, Y.sy, A.Wv, p, half, i, j, l16, g, bad);
+					if constexpr (OWNK) weigh<ST, NY, TB>(dyv, scr, y, yt, Y.sy, A.Wv, p, half, i, j, l16, g, far);
 					// dp of this half's 32 columns
 					f4 dp[2][2];
 #pragma unroll

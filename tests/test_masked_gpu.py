@@ -102,6 +102,22 @@ def test_what_is_hidden_may_hold_anything(bad, dtype):
         assert (x.cpu()[0][hidden] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("causal", [True, False])
+def test_what_is_visible_may_be_infinite(causal, dtype):
+    # a weight is not zero at these distances: infinity, as of the formula, in the rows that see it, and in no other place
+    q, k, v, do = _inputs(1, 100, 100, 2, 2, 32, 48, dtype, 21)
+    ref, terms = lf.masked(q, k, v, causal=causal)
+    v[0, 70, 1, 5], v[0, 3, 0, 7] = float("inf"), -float("inf")
+    o = _op(causal=causal)(q, k, v).double().cpu()
+    want = ref[0]
+    want[0, 70 if causal else 0:, 1, 5] = float("inf")
+    want[0, 3 if causal else 0:, 0, 7] = -float("inf")
+    inf = torch.isinf(want)
+    assert torch.equal(o[inf], want[inf])
+    lf.check([o.where(~inf, torch.zeros(())).to(dtype)], [want.where(~inf, torch.zeros((), dtype=torch.float64))], terms, dtype, 32)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_the_future_may_hold_anything(dtype):
     # values behind a query's own place: not finite, and yet not seen by the rows before them
