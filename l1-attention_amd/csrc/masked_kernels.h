@@ -31,8 +31,8 @@
 // not go by these codes but by the bits of the values themselves, as integers in order: sign(q - k) is exact.
 //
 // What bounds it: the vector ALU's issue, with about a quarter of the time waits (1.8 waves a SIMD: sums, codes and tiles fill the
-// registers).  4096 tokens, 16 heads, W 64, every pair visible: bfloat16 forward 574 us (v_sad_u16 alone 264), gradients of q
-// 1716 and of k and v 1801; float32 1371, 2484 and 2849.
+// registers).  4096 tokens, 16 heads, W 64, every pair visible: bfloat16 forward 652 us (v_sad_u16 alone 264), gradients of q
+// 1838 and of k and v 1989; float32 1344, 2540 and 2879.
 #pragma once
 #include "common.h"
 #include "masked.h"
