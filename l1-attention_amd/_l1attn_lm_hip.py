@@ -73,7 +73,6 @@ def slopes_of(slopes):
 
 @functools.lru_cache(maxsize=64)
 def _slopes_array(slopes):
-    slopes = slopes_of(slopes)
     return (ctypes.c_float * len(slopes))(*slopes)
 
 
@@ -87,10 +86,16 @@ def _index_tensor(x, name, shape, q):
 
 
 def _check_rule(H, softcap, slopes):
+    """The slopes of a call as a C array, or None.  Arrays are kept by the slopes' values: numbers first, since what the caller
+    holds may be tensors, which are the same objects when their values are others."""
     if not 0.0 <= softcap <= 3e38:
         raise ValueError("softcap must be a finite number >= 0 (0: none), got %r" % (softcap,))
-    if slopes is not None and len(slopes) != H:
+    if slopes is None:
+        return None
+    slopes = slopes_of(slopes)
+    if len(slopes) != H:
         raise ValueError("slopes must hold one number for each of the %d query heads, got %d" % (H, len(slopes)))
+    return _slopes_array(slopes)
 
 
 def _masked_desc(q, k, v, doc, prefix, causal, softcap, slopes):
@@ -112,8 +117,7 @@ def _masked_desc(q, k, v, doc, prefix, causal, softcap, slopes):
         raise RuntimeError("n_heads must be a multiple of n_key_heads, got %d and %d" % (H, Hk))
     if not (1 <= W <= 128 and 1 <= Wv <= 128):
         raise RuntimeError("widths of masked attention are 1 to 128, got %d and %d" % (W, Wv))
-    _check_rule(H, softcap, slopes)
-    numbers = None if slopes is None else _slopes_array(slopes)
+    numbers = _check_rule(H, softcap, slopes)
     d = MaskedDesc(B, T, S, H, Hk, W, Wv, DTYPES[q.dtype], int(bool(causal)), softcap,
                    None if slopes is None else ctypes.addressof(numbers),
                    _index_tensor(doc, "doc", (B, S), q), _index_tensor(prefix, "prefix", (B,), q))
@@ -266,9 +270,8 @@ def cache_attend(desc, device, q, seqs=None, counts=None, softcap=0.0, slopes=No
     B, n, H, _ = q.shape
     if seqs is None and B > desc.rows:
         raise RuntimeError("attend: %d sequences without a list, but the cache has %d rows" % (B, desc.rows))
-    _check_rule(H, softcap, slopes)
+    numbers = _check_rule(H, softcap, slopes)
     sp, cp = _row_list(seqs, "seqs", B, device), _row_list(counts, "counts", B, device)
-    numbers = None if slopes is None else _slopes_array(slopes)
     a = AttendDesc(B, n, H, DTYPES[q.dtype], softcap, None if slopes is None else ctypes.addressof(numbers))
     o = torch.empty((B, n, H, desc.Wv), dtype=q.dtype, device=device)
     L, d, ap = lib(), ctypes.addressof(desc), ctypes.addressof(a)

@@ -28,6 +28,7 @@ class L1AttnMaskedFn(Function):
     @staticmethod
     def forward(ctx, q, k, v, doc=None, prefix=None, causal=True, softcap=0.0, slopes=None):
         q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+        slopes = None if slopes is None else _drv.slopes_of(slopes)  # as numbers: the backward's are the forward's
         o, lse = _drv.masked_forward(q, k, v, doc, prefix, causal, softcap, slopes, any(ctx.needs_input_grad[:3]))
         ctx.save_for_backward(q, k, v, o, lse, doc, prefix)
         ctx.rule = (causal, softcap, slopes)

@@ -103,7 +103,7 @@ def l1attn_paged(q, cache, seqs=None, counts=None, softcap=0.0, slopes=None):
     tokens give zeros.  For serving: there is no gradient."""
     if torch.is_grad_enabled() and q.requires_grad:
         raise RuntimeError("l1attn_paged has no gradient: call it under torch.no_grad(), or on q.detach()")
-    return _drv.cache_attend(cache._desc, cache.device, q.contiguous(), seqs, counts, softcap, None if slopes is None else tuple(slopes))
+    return _drv.cache_attend(cache._desc, cache.device, q.contiguous(), seqs, counts, softcap, slopes)
 
 
 class L1AttnPaged(nn.Module):

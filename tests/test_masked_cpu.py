@@ -45,6 +45,19 @@ def test_slopes_are_constants_of_the_module():
             m.L1AttnMasked(slopes=bad)
 
 
+def test_slopes_are_taken_by_their_values():
+    # lists, tuples, tensors, and tensors as elements; an element that was changed in place is a new number
+    for slopes in ([0.5, 0.25], (0.5, 0.25), torch.tensor([0.5, 0.25]), torch.tensor([0.5, 0.25]).numpy()):
+        assert list(drv._check_rule(2, 0.0, slopes)) == [0.5, 0.25]
+    t = (torch.tensor(0.5), torch.tensor(0.25))
+    assert list(drv._check_rule(2, 0.0, t)) == [0.5, 0.25]
+    t[0].fill_(3.0)
+    assert list(drv._check_rule(2, 0.0, t)) == [3.0, 0.25]
+    assert drv._check_rule(2, 0.0, None) is None
+    with pytest.raises(ValueError, match="slopes"):
+        drv._check_rule(2, 0.0, (torch.tensor(-1.0), torch.tensor(0.0)))
+
+
 def test_c_entry_codes():
     L = drv.lib()
     one = ctypes.c_void_p(16)

@@ -298,6 +298,18 @@ def test_a_run_of_serving_calls_matches_the_training_operator():
         assert (o - want).abs().max() <= 2 * 2.0 ** -24 * (3 * 64 + 64 + 1) * v.abs().max()
 
 
+def test_slopes_as_tensors_that_change_in_place():
+    c = Pair(rows=1)
+    c.append(1, 60)
+    q = torch.randn(1, 1, 2, 32, generator=c.g).to(BF16).cuda()
+    slopes = (torch.tensor(0.5), torch.tensor(0.25))
+    for x in (0.5, 3.0):
+        slopes[0].fill_(x)
+        want = c.m.l1attn_paged(q, c.gpu, slopes=[x, 0.25])
+        assert torch.equal(c.m.l1attn_paged(q, c.gpu, slopes=slopes), want)
+        assert torch.equal(c.m.l1attn_paged(q, c.gpu, slopes=torch.stack(slopes)), want)
+
+
 def test_graph_of_a_decode_step_and_other_streams():
     import l1attn_paged_cuda as m
 
