@@ -36,6 +36,7 @@
 #pragma once
 #include "common.h"
 #include "masked.h"
+#include "softcap.h"
 #include <math.h>
 
 namespace {
@@ -788,24 +789,54 @@ __device__ __forceinline__ void tile_distances(char* own, char* str, const float
 	}
 }
 
-// capped score in those units and, in fac, its derivative by the score, from the distance over sqrt(W) (in those units without a cap)
-template <typename ST, bool CAP>
-__device__ __forceinline__ float score(float dist, float cap, float icap, float& fac)
+// Capped scores in those units of half a tile and, in fac, their derivatives by the score, from the distances over sqrt(W) (in
+// those units without a cap).
+template <typename ST, bool CAP, int TB>
+__device__ __forceinline__ void scores(float (&c)[4][4], float (&fac)[4][4], const float (&x)[4][TB], int half, float cap, float icap)
 {
 	if constexpr (!CAP) {
-		fac = 1.f;
-		return -dist;
+#pragma unroll
+		for (int bb = 0; bb < 4; bb++)
+#pragma unroll
+			for (int a = 0; a < 4; a++) {
+				c[a][bb] = -x[a][4 * half + bb];
+				fac[a][bb] = 1.f;
+			}
+	} else if constexpr (!k16<ST>) {
+#pragma unroll
+		for (int bb = 0; bb < 4; bb++)
+#pragma unroll
+			for (int a = 0; a < 4; a++) {
+				const float th = tanhf(-x[a][4 * half + bb] * icap);
+				fac[a][bb] = 1.f - th * th;
+				c[a][bb] = cap * th;
+			}
 	} else {
-		float th;
-		if constexpr (k16<ST>) {
-			// tanh(y) = (e^2y - 1) / (e^2y + 1) for y <= 0: off by 2^-23 absolutely, which is what a 16-bit result sees
-			const float e = __builtin_amdgcn_exp2f(dist * (-2.885390082f * icap));
-			th = (e - 1.f) * __builtin_amdgcn_rcpf(e + 1.f);
+		unsigned least = 0x7f800000;  // distances are not negative: their bits are in their order
+#pragma unroll
+		for (int bb = 0; bb < 4; bb++)
+#pragma unroll
+			for (int a = 0; a < 4; a++) least = min(least, __builtin_bit_cast(unsigned, x[a][4 * half + bb]));
+		if (__any(__builtin_bit_cast(float, least) * icap < kCapSeries)) {
+#pragma unroll
+			for (int bb = 0; bb < 4; bb++)
+#pragma unroll
+				for (int a = 0; a < 4; a++) {
+					const float d = x[a][4 * half + bb], y = d * icap, r = l1_tanh_near(y), t = l1_tanh_far(-y);
+					const float th = y < kCapSeries ? -y * r : t;
+					fac[a][bb] = 1.f - th * th;
+					c[a][bb] = (y < kCapSeries ? -d * r : cap * t) * kUnit<ST>;
+				}
 		} else {
-			th = tanhf(-dist * icap);
+#pragma unroll
+			for (int bb = 0; bb < 4; bb++)
+#pragma unroll
+				for (int a = 0; a < 4; a++) {
+					const float th = l1_tanh_far(-x[a][4 * half + bb] * icap);
+					fac[a][bb] = 1.f - th * th;
+					c[a][bb] = cap * kUnit<ST> * th;
+				}
 		}
-		fac = 1.f - th * th;
-		return cap * kUnit<ST> * th;
 	}
 }
 
@@ -908,14 +939,8 @@ __global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* 
 					for (int wb = 0; wb < NB; wb++) tile[tb][wb] = (f4)(0.f);
 #pragma unroll
 			for (int half = 0; half < TB / 4; half++) {
-				float p[4][4];
-#pragma unroll
-				for (int bb = 0; bb < 4; bb++)
-#pragma unroll
-					for (int a = 0; a < 4; a++) {
-						float fac;
-						p[a][bb] = score<ST, CAP>(x[a][4 * half + bb], A.cap, A.icap, fac);
-					}
+				float p[4][4], fac[4][4];
+				scores<ST, CAP, TB>(p, fac, x, half, A.cap, A.icap);
 				if (slope != 0.f) {
 					asm volatile("");  // a branch
 #pragma unroll
@@ -1240,15 +1265,15 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 				for (int half = 0; half < TB / 4; half++) {
 					const int lane = here(tid & 63), i = lane & 7, j = lane >> 3, l16 = lane & 15, g = lane >> 4;
 					float p[4][4], pf[4][4];  // weights, and the derivative of their argument by the distance's sum
+					scores<ST, CAP, TB>(p, pf, x, half, A.cap, A.icap);
 #pragma unroll
 					for (int bb = 0; bb < 4; bb++) {
 						const int b = 4 * half + bb, r = j + 8 * b;
 						const float sl = OWNK ? slse[r] : 0.f;
 #pragma unroll
 						for (int a = 0; a < 4; a++) {
-							float fac;
-							p[a][bb] = score<ST, CAP>(x[a][b], A.cap, A.icap, fac) - (OWNK ? sl : olse[a]);
-							pf[a][bb] = (CAP ? fac : 1.f) * grw;
+							p[a][bb] -= OWNK ? sl : olse[a];
+							pf[a][bb] *= grw;
 						}
 					}
 					if (slope != 0.f) {

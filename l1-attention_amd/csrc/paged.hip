@@ -19,6 +19,7 @@
 // v_sad_u16, which issue in about 4.2 cycles each; the rest makes codes and float16 of the cache's bytes, and weights).  With
 // one token a lane instead of two at 16 rows a row's codes would be read from LDS twice as often.
 #include "paged.h"
+#include "softcap.h"
 #include <math.h>
 #include <type_traits>
 
@@ -101,13 +102,7 @@ __device__ __forceinline__ void codes4(int word, float (&x)[4])
 	x[3] = (float)(word >> 24);
 }
 
-// c(a) = cap tanh(a / cap) of a logit a <= 0, and exp(a)
-template <typename ST> __device__ __forceinline__ float capped(float a, float cap, float icap)
-{
-	if constexpr (sizeof(ST) == 4) return cap * tanhf(a * icap);
-	const float e = __builtin_amdgcn_exp2f(a * (2.885390082f * icap));
-	return cap * (e - 1.f) * __builtin_amdgcn_rcpf(e + 1.f);
-}
+// exp(a)
 template <typename ST> __device__ __forceinline__ float exponential(float a)
 {
 	if constexpr (sizeof(ST) == 4) return expf(a);
@@ -411,11 +406,28 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 		for (int u = 0; u < U; u++)
 #pragma unroll
 			for (int r = 0; r < RB; r++) dist[u][r] *= -m;
-		if (A.cap > 0.f)
+		if (A.cap > 0.f) {  // see softcap.h
+			float near = -3.402823466e38f;
+			if constexpr (!F32)
 #pragma unroll
-			for (int u = 0; u < U; u++)
+				for (int u = 0; u < U; u++)
 #pragma unroll
-				for (int r = 0; r < RB; r++) dist[u][r] = capped<ST>(dist[u][r], A.cap, A.icap);
+					for (int r = 0; r < RB; r++) near = fmaxf(near, dist[u][r]);
+			if (!F32 && __any(near * A.icap > -kCapSeries)) {
+#pragma unroll
+				for (int u = 0; u < U; u++)
+#pragma unroll
+					for (int r = 0; r < RB; r++) {
+						const float y = dist[u][r] * A.icap;
+						dist[u][r] = y > -kCapSeries ? dist[u][r] * l1_tanh_near(y) : A.cap * l1_tanh_far(y);
+					}
+			} else {
+#pragma unroll
+				for (int u = 0; u < U; u++)
+#pragma unroll
+					for (int r = 0; r < RB; r++) dist[u][r] = A.cap * (F32 ? tanhf(dist[u][r] * A.icap) : l1_tanh_far(dist[u][r] * A.icap));
+			}
+		}
 #pragma unroll
 		for (int u = 0; u < U; u++) {
 			const int t = t0 + 64 * u + lane, sees = pg[u] >= 0 ? t : 0x7fffffff;

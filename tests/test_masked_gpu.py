@@ -136,6 +136,13 @@ def test_small_and_large_inputs(scale, dtype):
     _check(*_inputs(1, 120, 120, 2, 2, 64, 64, dtype, 11, scale))
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("cap", [1e3, 1e5, 1e6, 1e8, 1e12, 1e30, 3e38])
+def test_large_caps(cap, dtype):
+    # the capped score goes to the score itself: an absolute error of the tanh would be multiplied by the cap
+    _check(*_inputs(1, 100, 120, 2, 1, 64, 48, dtype, 51, 0.3), cap=cap)
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("shift,W,Wv", [(0.0, 64, 64), (300.0, 64, 64), (0.0, 100, 128)])
 def test_a_few_far_values(shift, W, Wv, dtype):

@@ -191,6 +191,15 @@ def test_small_and_large_inputs(H, n, W, scale, dtype):
     c.attend(3, n, H, q=near + 0.1 * scale * torch.randn(near.shape, generator=c.g))
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("H", [2, 12])
+@pytest.mark.parametrize("cap", [1e3, 1e5, 1e6, 1e8, 1e12, 1e30, 3e38])
+def test_large_caps(cap, H, dtype):
+    c = Pair(N=40, P=16, Hk=2, W=64, Wv=48, rows=2, M=12, dtype=dtype, seed=21)
+    c.append(2, 150, counts=[150, 9], scale=0.3)
+    c.attend(2, 2, H, cap=cap, q=0.3 * torch.randn(2, 2, H, 64, generator=c.g))
+
+
 @pytest.mark.parametrize("B,H,n", [(300, 2, 1), (300, 4, 5), (513, 2, 2)])
 def test_many_entries(B, H, n):
     # every row of the table many times, in no order, some that are not there; uneven lengths over several steps
