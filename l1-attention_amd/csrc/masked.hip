@@ -1,6 +1,7 @@
 // Entry points of the masked L1 attention: checks, how a launch is cut, workspaces.  The kernels: masked_kernels.h.
 #include "common.h"
 #include "masked.h"
+#include "softcap.h"
 #include <math.h>
 
 namespace {
@@ -33,7 +34,7 @@ L1MaskedArgs args_of(const l1attn_masked_desc* d, const void* q, const void* k, 
 {
 	L1MaskedArgs A;
 	A.B = (int)d->B; A.T = (int)d->T; A.S = (int)d->S; A.H = (int)d->H; A.Hk = (int)d->Hk; A.W = (int)d->W; A.Wv = (int)d->Wv;
-	A.causal = d->causal; A.cap = d->softcap; A.icap = d->softcap > 0.f ? 1.f / d->softcap : 0.f;
+	A.causal = d->causal; A.cap = d->softcap; A.icap = l1_icap(d->softcap);
 	A.rw = (float)(1.0 / sqrt((double)d->W));
 	A.doc = d->doc; A.prefix = d->causal ? d->prefix : nullptr; A.has_slopes = d->slopes != nullptr;
 	for (int h = 0; h < L1_MASKED_HEADS; h++) A.slopes[h] = d->slopes && h < d->H ? d->slopes[h] : 0.f;

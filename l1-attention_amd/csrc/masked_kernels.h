@@ -874,7 +874,7 @@ __global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* 
 	unsigned char* cls = reinterpret_cast<unsigned char*>(red + 64);
 	const int* doc = A.doc ? A.doc + (int64_t)K.b * A.S : nullptr;
 	const int prefix = A.prefix ? A.prefix[K.b] : 0;
-	const float slope = A.has_slopes ? A.slopes[K.h] * kUnit<ST> : 0.f;
+	const float slope = A.has_slopes ? fminf(A.slopes[K.h] * kUnit<ST>, kMax) : 0.f;  // finite: a distance of zero is multiplied by it
 	const int64_t qpitch = (int64_t)A.H * A.W, kpitch = (int64_t)A.Hk * A.W, vpitch = (int64_t)A.Hk * A.Wv;
 	const ST* qh = q + ((int64_t)K.b * A.T * A.H + K.h) * A.W;
 	const ST* kh = k + ((int64_t)K.b * A.S * A.Hk + K.hk) * A.W;
@@ -1198,7 +1198,7 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 
 	for (int hg = 0; hg < (OWNK ? group : 1); hg++) {
 		const int h = OWNK ? K.hk * group + hg : K.h;
-		const float slope = A.has_slopes ? A.slopes[h] * kUnit<ST> : 0.f;
+		const float slope = A.has_slopes ? fminf(A.slopes[h] * kUnit<ST>, kMax) : 0.f;
 		const ST* qh = q + ((int64_t)K.b * A.T * A.H + h) * A.W;
 		const ST* oh = dout + ((int64_t)K.b * A.T * A.H + h) * A.Wv;
 		const ST* str_x = OWNK ? qh : kh;

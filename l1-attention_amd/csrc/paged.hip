@@ -604,7 +604,7 @@ int check_attend(const l1attn_cache* cache, const l1attn_attend_desc* d, AttendA
 			if (!(d->slopes[h] >= 0.f) || !(d->slopes[h] <= 3e38f)) return L1ATTN_ERR_ARG;
 	A->B = (int)d->B; A->n = (int)d->n; A->H = (int)d->H; A->G = (int)(d->H / A->C.Hk);
 	if (l1_cdiv(d->n * A->G, 8) > 65535) return L1ATTN_ERR_RANGE;
-	A->cap = d->softcap; A->icap = d->softcap > 0.f ? 1.f / d->softcap : 0.f;
+	A->cap = d->softcap; A->icap = l1_icap(d->softcap);
 	A->rw = (float)(1.0 / sqrt((double)A->C.W));
 	for (int h = 0; h < 256; h++) A->slopes[h] = d->slopes && h < d->H ? d->slopes[h] : 0.f;
 	if (d->B == 0 || d->n == 0) return 1;

@@ -10,6 +10,10 @@
 
 constexpr float kCapSeries = 0.125f;  // below this |y|
 
+// 1 / cap as the kernels take it: finite, since a distance of zero is multiplied by it (and by 2 log2(e) besides).  Below a cap of
+// 1e-38 it is not the reciprocal any more, and the capped logits, no larger than the cap, are nothing beside the no-op's.
+static inline float l1_icap(float cap) { return cap > 1e-38f ? 1.f / cap : cap > 0.f ? 1e38f : 0.f; }
+
 __device__ __forceinline__ float l1_tanh_far(float y)
 {
 	const float e = __builtin_amdgcn_exp2f(y * 2.885390082f);

@@ -143,6 +143,21 @@ def test_large_caps(cap, dtype):
     _check(*_inputs(1, 100, 120, 2, 1, 64, 48, dtype, 51, 0.3), cap=cap)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("cap", [1e-45, 1e-39, 1e-38, 1e-30, 1e-3])
+def test_tiny_caps(cap, dtype):
+    # keys that equal queries: a distance of zero over a cap whose reciprocal is beyond float32
+    q, k, v, do = _inputs(1, 70, 70, 2, 2, 32, 32, dtype, 52)
+    k[:, ::3] = q[:, ::3]
+    _check(q, k, v, do, cap=cap)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("slope", [2e38, 2.5e38, 3e38])
+def test_largest_slopes(slope, dtype):
+    _check(*_inputs(1, 70, 90, 2, 1, 32, 32, dtype, 54), slopes=(slope, 0.25))
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("shift,W,Wv", [(0.0, 64, 64), (300.0, 64, 64), (0.0, 100, 128)])
 def test_a_few_far_values(shift, W, Wv, dtype):

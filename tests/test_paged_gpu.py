@@ -200,6 +200,20 @@ def test_large_caps(cap, H, dtype):
     c.attend(2, 2, H, cap=cap, q=0.3 * torch.randn(2, 2, H, 64, generator=c.g))
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("H", [2, 12])
+@pytest.mark.parametrize("cap,slope", [(1e-45, 0.0), (1e-39, 0.0), (1e-38, 1.0), (0.3, 0.0), (0.0, 2.5e38), (0.0, 3e38)])
+def test_tiny_caps_and_largest_slopes(cap, slope, H, dtype):
+    # distances of zero, over a cap whose reciprocal is beyond float32
+    c = Pair(N=40, P=16, Hk=2, W=64, Wv=48, rows=2, M=12, dtype=dtype, seed=21)
+    k, v = c.data(2, 150, 0.3)
+    k[:, :8] = 0.0
+    c.append(2, 150, counts=[150, 9], data=(k, v))
+    q = 0.3 * torch.randn(2, 2, H, 64, generator=c.g)
+    q[1] = 0.0
+    c.attend(2, 2, H, cap=cap, q=q, slopes=(slope,) * H)
+
+
 @pytest.mark.parametrize("B,H,n", [(300, 2, 1), (300, 4, 5), (513, 2, 2)])
 def test_many_entries(B, H, n):
     # every row of the table many times, in no order, some that are not there; uneven lengths over several steps
