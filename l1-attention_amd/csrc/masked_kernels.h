@@ -807,9 +807,9 @@ __device__ __forceinline__ void scores(float (&c)[4][4], float (&fac)[4][4], con
 		for (int bb = 0; bb < 4; bb++)
 #pragma unroll
 			for (int a = 0; a < 4; a++) {
-				const float th = tanhf(-x[a][4 * half + bb] * icap);
-				fac[a][bb] = 1.f - th * th;
-				c[a][bb] = cap * th;
+				const float y = -x[a][4 * half + bb] * icap, e = expf(2.f * y), d = 1.f + e;
+				fac[a][bb] = 4.f * e / (d * d);  // 1 - tanh^2, with all of its digits
+				c[a][bb] = cap * tanhf(y);
 			}
 	} else {
 		unsigned least = 0x7f800000;  // distances are not negative: their bits are in their order
@@ -822,9 +822,9 @@ __device__ __forceinline__ void scores(float (&c)[4][4], float (&fac)[4][4], con
 			for (int bb = 0; bb < 4; bb++)
 #pragma unroll
 				for (int a = 0; a < 4; a++) {
-					const float d = x[a][4 * half + bb], y = d * icap, r = l1_tanh_near(y), t = l1_tanh_far(-y);
-					const float th = y < kCapSeries ? -y * r : t;
-					fac[a][bb] = 1.f - th * th;
+					float f;
+					const float d = x[a][4 * half + bb], y = d * icap, r = l1_tanh_near(y), t = l1_tanh_far(-y, f);
+					fac[a][bb] = y < kCapSeries ? 1.f - y * y * r * r : f;
 					c[a][bb] = (y < kCapSeries ? -d * r : cap * t) * kUnit<ST>;
 				}
 		} else {
@@ -832,9 +832,7 @@ __device__ __forceinline__ void scores(float (&c)[4][4], float (&fac)[4][4], con
 			for (int bb = 0; bb < 4; bb++)
 #pragma unroll
 				for (int a = 0; a < 4; a++) {
-					const float th = l1_tanh_far(-x[a][4 * half + bb] * icap);
-					fac[a][bb] = 1.f - th * th;
-					c[a][bb] = cap * kUnit<ST> * th;
+					c[a][bb] = cap * kUnit<ST> * l1_tanh_far(-x[a][4 * half + bb] * icap, fac[a][bb]);
 				}
 		}
 	}

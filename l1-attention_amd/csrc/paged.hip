@@ -418,14 +418,18 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 				for (int u = 0; u < U; u++)
 #pragma unroll
 					for (int r = 0; r < RB; r++) {
+						float d;  // the derivative, of which there is no use
 						const float y = dist[u][r] * A.icap;
-						dist[u][r] = y > -kCapSeries ? dist[u][r] * l1_tanh_near(y) : A.cap * l1_tanh_far(y);
+						dist[u][r] = y > -kCapSeries ? dist[u][r] * l1_tanh_near(y) : A.cap * l1_tanh_far(y, d);
 					}
 			} else {
 #pragma unroll
 				for (int u = 0; u < U; u++)
 #pragma unroll
-					for (int r = 0; r < RB; r++) dist[u][r] = A.cap * (F32 ? tanhf(dist[u][r] * A.icap) : l1_tanh_far(dist[u][r] * A.icap));
+					for (int r = 0; r < RB; r++) {
+					float d;
+					dist[u][r] = A.cap * (F32 ? tanhf(dist[u][r] * A.icap) : l1_tanh_far(dist[u][r] * A.icap, d));
+				}
 			}
 		}
 #pragma unroll

@@ -14,10 +14,12 @@ constexpr float kCapSeries = 0.125f;  // below this |y|
 // 1e-38 it is not the reciprocal any more, and the capped logits, no larger than the cap, are nothing beside the no-op's.
 static inline float l1_icap(float cap) { return cap > 1e-38f ? 1.f / cap : cap > 0.f ? 1e38f : 0.f; }
 
-__device__ __forceinline__ float l1_tanh_far(float y)
+// tanh(y), and in d its derivative as 4 e / (1 + e)^2: 1 - tanh^2 has none of its digits left where the cap is a fraction of the logits
+__device__ __forceinline__ float l1_tanh_far(float y, float& d)
 {
-	const float e = __builtin_amdgcn_exp2f(y * 2.885390082f);
-	return (e - 1.f) * __builtin_amdgcn_rcpf(e + 1.f);
+	const float e = __builtin_amdgcn_exp2f(y * 2.885390082f), r = __builtin_amdgcn_rcpf(e + 1.f);
+	d = 4.f * e * r * r;
+	return (e - 1.f) * r;
 }
 
 // tanh(y) / y

@@ -153,6 +153,20 @@ def test_tiny_caps(cap, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("cap", [0.3, 1.0, 2.0])
+def test_gradients_of_saturated_caps(cap, dtype):
+    # the tanh's derivative is 1e-26 to 1e-2 here, and the gradients have its digits.  The formula's own 1 - (c/cap)^2 is off by
+    # 2^-52 in 64 bits; that much of a score's gradient, 1/8 p (|do||v| + 2 |do||o|) with p <= 1, |o| <= max |v| and 32 columns,
+    # comes in for each of up to 90 pairs
+    q, k, v, do = _inputs(1, 70, 90, 2, 2, 64, 32, dtype, 53)
+    ref, terms = lf.masked(q, k, v, do, cap=cap)
+    of_the_formula = 2.0 ** -52 * 90 / 8 * 3 * 32 * float(v.abs().max()) * float(do.abs().max())
+    for t in terms[1:3]:
+        t += of_the_formula / (2.0 ** -24 * (3 * 64 + 64))  # check() multiplies the terms by this
+    lf.check(_run(q, k, v, do, cap=cap), ref, terms, dtype, 64)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("slope", [2e38, 2.5e38, 3e38])
 def test_largest_slopes(slope, dtype):
     _check(*_inputs(1, 70, 90, 2, 1, 32, 32, dtype, 54), slopes=(slope, 0.25))
