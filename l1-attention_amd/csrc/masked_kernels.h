@@ -25,10 +25,10 @@
 // 16-bit inputs: distances are sums of |difference| of 16-bit codes (v_sad_u16: two pair-elements an instruction; 2.5 cycles per
 // 64 pair-elements against 5.2 in float32).  The codes are a grid over the range [lo, hi] of the workgroup's owner rows; a stream
 // value x outside of it counts as |x - clip(x)|, summed per stream row, plus the code of clip(x): for an owner q within
-// the range |q - x| = |q - clip(x)| + |clip(x) - x|.  Each code is off by half a step u = (hi - lo) / 65535 at most, which moves a
-// logit by u * sqrt(1/6) = 0.41 u on average: below the rounding of p to 16 bits as long as hi - lo is at most kRange.  A
-// workgroup whose owners spread further (or are not finite) takes float32 distances, half of the columns at a time.  Signs do
-// not go by these codes but by the bits of the values themselves, as integers in order: sign(q - k) is exact.
+// the range |q - x| = |q - clip(x)| + |clip(x) - x|.  What the codes' roundings do to a logit, and the widest range hi - lo that
+// they are taken for: codes.h.  A workgroup whose owners spread further (or are not finite) takes float32 distances, half of the
+// columns at a time.  Signs do not go by these codes but by the bits of the values themselves, as integers in order: sign(q - k)
+// is exact.
 //
 // What bounds it: the vector ALU's issue, with about a quarter of the time waits (1.8 waves a SIMD: sums, codes and tiles fill the
 // registers).  4096 tokens, 16 heads, W 64, every pair visible: bfloat16 forward 652 us (v_sad_u16 alone 264), gradients of q
@@ -37,6 +37,7 @@
 #include "common.h"
 #include "masked.h"
 #include "softcap.h"
+#include "codes.h"
 #include <math.h>
 
 namespace {
@@ -55,10 +56,6 @@ constexpr int kClasses = 1024;  // tiles whose visibility is worked out at a tim
 constexpr float kMax = 3.402823466e38f;
 
 template <typename ST> constexpr bool k16 = sizeof(ST) == 2;
-// widest range of the owners' values for which 16-bit codes are fine enough: 0.41 * range / 65535 against half a step of the
-// type, 2^-12 (float16) and 2^-9 (bfloat16) on average
-template <typename ST> constexpr float kRange = 24.f;
-template <> constexpr float kRange<__bf16> = 160.f;
 // what a weight is multiplied by: p <= 1, and goes into the products as 16-bit numbers; float16 has no room below 2^-14
 template <typename ST> constexpr float kWeight = 1.f;
 template <> constexpr float kWeight<_Float16> = 16384.f;
@@ -313,19 +310,20 @@ __device__ __forceinline__ void stage32(char* dst, const ST* __restrict__ x, int
 }
 
 // the grid of a workgroup's codes
-// x -> x * sc + b in [0, 1], which is 65535 steps; inv: one step
+// x -> x * sc + b, and the column's offset, in [0, 1], which is 65535 steps; inv: one step
 struct Grid { float sc, b, inv; };
 
-// eight values as codes, those behind the first n as zero; over: plus what lies outside of [0, 1]
+// eight values, the c-th of a row, as codes, those behind the first n as zero; over: plus what lies outside of [0, 1]
 template <typename ST>
-__device__ __forceinline__ uint4 codes_of(const uint4& bits, int n, const Grid& G, float& over)
+__device__ __forceinline__ uint4 codes_of(const uint4& bits, int c, int n, const Grid& G, float& over)
 {
+	const float b = G.b + l1_code_eight(c);
 	float v[8];
 	unpack<ST>(bits, v);
 	unsigned w[4];
 #pragma unroll
 	for (int e = 0; e < 8; e++) {
-		v[e] = __builtin_fmaf(v[e], G.sc, G.b);
+		v[e] = __builtin_fmaf(v[e], G.sc, b + l1_code_column(e));
 		if (n < 8) v[e] = e < n ? v[e] : 0.f;
 		over += __builtin_fabsf(v[e] - __builtin_amdgcn_fmed3f(v[e], 0.f, 1.f));
 	}
@@ -355,7 +353,7 @@ __device__ __forceinline__ void stage_own16(char* dst, char* raw, const ST* __re
 			uint4 bits = make_uint4(0, 0, 0, 0);
 			if (r0 + r < L) bits = load_raw(x + (int64_t)(r0 + r) * pitch + 8 * c, W - 8 * c, vec);
 			float over = 0.f;
-			*reinterpret_cast<uint4*>(dst + r * stride + 16 * c) = codes_of<ST>(bits, W - 8 * c, G, over);
+			*reinterpret_cast<uint4*>(dst + r * stride + 16 * c) = codes_of<ST>(bits, c, W - 8 * c, G, over);
 			if (raw) *reinterpret_cast<uint4*>(raw + r * rstride + 16 * c) = ordered8(bits);
 		}
 }
@@ -427,7 +425,7 @@ struct Stream {
 			} else {
 				if (cg == 0) out = 0.f;
 				if (c < chunks) {
-					*reinterpret_cast<uint4*>(str + r * Y.so + 16 * c) = codes_of<ST>(bits, W - 8 * c, G, out);
+					*reinterpret_cast<uint4*>(str + r * Y.so + 16 * c) = codes_of<ST>(bits, c, W - 8 * c, G, out);
 					if (raw) *reinterpret_cast<uint4*>(raw + r * Y.sr + 16 * c) = ordered8(bits);
 				}
 				if (cg == ncg - 1) {
@@ -727,12 +725,12 @@ __device__ __forceinline__ bool owner_grid(const ST* __restrict__ x, const int* 
 	// a margin of 2^-20 on both sides, or the roundings of x * sc + b would put an owner outside
 	const float span = (hi - lo) * (1.f + 0x1p-19f);
 	lo -= (hi - lo) * 0x1p-20f;
-	G.sc = span > 0.f ? 1.f / span : 0.f;
+	G.inv = span * (1.f / kCodeSteps);
+	G.sc = span > 0.f ? 1.f / (G.inv * 65535.f) : 0.f;
 	G.b = -lo * G.sc;
-	G.inv = span / 65535.f;
 	// b is rounded by 2^-21 at most up to 8, which the margin covers: values that lie further from zero than that, for their
 	// span, or next to nothing apart, or all the same, go without codes
-	return all_finite && span <= kRange<ST> && span > 0.f && G.sc <= 1e30f && __builtin_fabsf(G.b) <= 8.f;
+	return all_finite && span <= kCodeRange<ST> && span > 0.f && G.sc <= 1e30f && __builtin_fabsf(G.b) <= 8.f;
 }
 
 // A wave's distances of one tile, acc[a][b] >= 0 scaled by 1/sqrt(W), NaN where a value is.  Called by all waves of the

@@ -8,9 +8,8 @@
 // order.  Every byte of the cache is read once for up to 16 rows.
 // Distances.  Up to 4 rows, and float32: float32, two instructions an element and row.  From 5 rows of 16 bits on: sums of
 // |difference| of 16-bit codes (v_sad_u16, two elements an instruction) on one grid over the rows' values and over what the
-// scales of the workgroup's pages allow (128 times the largest); a code is off by half a step at most, which moves a logit by
-// 0.41 steps on average.  Past a range of 24 (float16; 160 bfloat16), where that would reach the type's own rounding, or where a
-// row or scale is not finite, float32.
+// scales of the workgroup's pages allow (128 times the largest); what that does to a logit: codes.h.  Past the range that is
+// allowed there, or where a row or scale is not finite, float32.
 // Sums.  Weight times scale is two numbers of the rows' type, itself rounded and what that leaves out (float16 at 2^14 over the
 // power of two above the step's largest scale; one number alone made results 1.6 times as inexact as their own rounding), a code is
 // exact in it, and matrix instructions add them in float32; float32 has its own matrix instruction.
@@ -20,6 +19,7 @@
 // one token a lane instead of two at 16 rows a row's codes would be read from LDS twice as often.
 #include "paged.h"
 #include "softcap.h"
+#include "codes.h"
 #include <math.h>
 #include <type_traits>
 
@@ -209,14 +209,17 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 #pragma unroll
 		for (int w = 0; w < 4; w++) { least = fminf(least, red[2 * w]); most = fmaxf(most, red[2 * w + 1]); }
 		const float span = (most - least) * (1.f + 0x1p-19f);
-		coded = finite && span > 1e-30f && span <= (std::is_same_v<ST, _Float16> ? 24.f : 160.f);
-		sc = coded ? 1.f / span : 0.f;
+		coded = finite && span > 1e-30f && span <= kCodeRange<ST>;
+		const float step = span * (1.f / kCodeSteps);
+		sc = coded ? 1.f / (step * 65535.f) : 0.f;
 		off = coded ? -(least - (most - least) * 0x1p-20f) * sc : 0.f;
 		if (coded) {
-			m = span * (1.f / 65535.f) * A.rw;
-			for (int w = my0; w < pk / 2; w += TR)
-				qc[my * 64 + w] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pknorm_u16(__builtin_fmaf(qs[my * 128 + 2 * w], sc, off),
-				                                                                             __builtin_fmaf(qs[my * 128 + 2 * w + 1], sc, off)));
+			m = step * A.rw;
+			for (int w = my0; w < pk / 2; w += TR) {
+				const float b = off + l1_code_eight(w >> 2), b0 = b + l1_code_column(2 * (w & 3)), b1 = b + l1_code_column(2 * (w & 3) + 1);
+				qc[my * 64 + w] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pknorm_u16(__builtin_fmaf(qs[my * 128 + 2 * w], sc, b0),
+				                                                                             __builtin_fmaf(qs[my * 128 + 2 * w + 1], sc, b1)));
+			}
 		}
 	}
 	__syncthreads();
@@ -300,6 +303,7 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 #pragma unroll
 				for (int i = 0; i < KB; i++) {
 					const int c = c0 + i;
+					const float b[2] = {off + l1_code_eight(2 * c), off + l1_code_eight(2 * c + 1)};
 					unsigned kc[U][8];
 #pragma unroll
 					for (int u = 0; u < U; u++) {
@@ -311,8 +315,10 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 						for (int d = 0; d < 4; d++) {
 							float x[4];
 							codes4(word[d], x);
-							kc[u][2 * d] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pknorm_u16(__builtin_fmaf(x[0], f, off), __builtin_fmaf(x[1], f, off)));
-							kc[u][2 * d + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pknorm_u16(__builtin_fmaf(x[2], f, off), __builtin_fmaf(x[3], f, off)));
+#pragma unroll
+							for (int e = 0; e < 4; e++) x[e] = __builtin_fmaf(x[e], f, b[d >> 1] + l1_code_column(4 * (d & 1) + e));
+							kc[u][2 * d] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pknorm_u16(x[0], x[1]));
+							kc[u][2 * d + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pknorm_u16(x[2], x[3]));
 						}
 					}
 					if (FULL || c < kchunks)

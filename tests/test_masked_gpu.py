@@ -182,6 +182,26 @@ def test_a_few_far_values(shift, W, Wv, dtype):
     _check(q, k, v, do)
 
 
+def _few_values(dtype, rng, W, seed, T=128, H=4):
+    # rows of one value, keys at distances that leave a weight; a far pair of columns in every 32 rows makes the range
+    g = torch.Generator().manual_seed(seed)
+    a = (torch.rand(1, T, H, 1, generator=g) - 0.5) * 0.9 * rng
+    q = a.expand(1, T, H, W).clone()
+    k = (a + (torch.rand(1, T, H, 1, generator=g) - 0.5) * 8 / W ** 0.5).expand(1, T, H, W).clone()
+    for x in (q, k):
+        x[:, ::32, :, 0], x[:, 1::32, :, 0] = rng / 2, -rng / 2
+    v, do = torch.randn(1, T, H, 32, generator=g), torch.randn(1, T, H, 32, generator=g)
+    return [x.to(dtype).cuda() for x in (q, k, v, do)]
+
+
+@pytest.mark.parametrize("dtype,rng", [(F16, 23.5), (F16, 11.8), (F16, 8.0), (BF16, 158.0), (BF16, 94.0), (BF16, 30.0)])
+@pytest.mark.parametrize("W", [16, 64, 96, 128])
+def test_rows_of_few_values(W, dtype, rng):
+    # a document of its own for each token: one weight alone is in a result, and all columns' roundings in its logit
+    q, k, v, do = _few_values(dtype, rng, W, W)
+    _check(q, k, v, do, doc=torch.arange(128, dtype=torch.int32)[None].cuda())
+
+
 def test_a_prefix_changes_nothing_without_causal():
     q, k, v, do = _inputs(2, 70, 70, 2, 1, 33, 40, BF16, 32)
     prefix = torch.tensor([30, 0], dtype=torch.int32).cuda()

@@ -214,6 +214,23 @@ def test_tiny_caps_and_largest_slopes(cap, slope, H, dtype):
     c.attend(2, 2, H, cap=cap, q=q, slopes=(slope,) * H)
 
 
+@pytest.mark.parametrize("dtype,rng", [(F16, 23.5), (F16, 11.8), (F16, 8.0), (BF16, 158.0), (BF16, 94.0), (BF16, 30.0)])
+@pytest.mark.parametrize("W", [16, 64, 96, 128])
+def test_rows_of_few_values(W, dtype, rng):
+    # one token a sequence: its weight alone is in the result
+    B, H = 48, 8
+    c = Pair(N=64, P=16, Hk=1, W=W, Wv=32, rows=B, M=2, dtype=F32, seed=W)
+    top = rng / 2 / 128 * 127 * 0.999  # the grid is over the 128-fold of the scale
+    a = (torch.rand(B, 1, 1, 1, generator=c.g) - 0.5) * 2 * top
+    k = a.expand(B, 1, 1, W).clone()
+    k[:, :, :, 1] = top
+    v = torch.randn(B, 1, 1, 32, generator=c.g)
+    c.append(B, 1, data=(k, v))
+    q = (a + (torch.rand(B, 1, H, 1, generator=c.g) - 0.5) * 8 / W ** 0.5).clamp(-top, top).expand(B, 1, H, W).clone()
+    q[:, :, :, 1] = top
+    c.attend(B, 1, H, dtype=dtype, q=q)
+
+
 @pytest.mark.parametrize("B,H,n", [(300, 2, 1), (300, 4, 5), (513, 2, 2)])
 def test_many_entries(B, H, n):
     # every row of the table many times, in no order, some that are not there; uneven lengths over several steps
