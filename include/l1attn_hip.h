@@ -396,6 +396,9 @@ int l1attn_sparse_bidi_bwd_bf16(const void* dvo, const void* vf, const void* vb,
  * visible has no influence, whatever its values; a row that sees nothing is zero.
  * q [B,T,H,W], k [B,S,Hk,W], v [B,S,Hk,Wv], o and d_o [B,T,H,Wv], lse [B,T,H] float32 (log of the denominator; the forward
  * takes NULL for it).  dtype 0 float32, 1 float16, 2 bfloat16; sums and softmax are float32 in each.
+ * o_rest: [B,T,H,Wv] of the inputs' type or NULL (float32: not used): the forward writes what the rounding of o left out, the
+ * backward adds it to o for sum d_o * o, which is taken off each d_o . v: without it the rounding of o alone moves dq and dk by
+ * several times their own rounding where the values v have a part in common.
  * doc [B,S] and prefix [B] are device pointers to int32 or NULL; slopes is a HOST pointer to H numbers >= 0, or NULL, read
  * during the call.  T <= S <= 4194240, W and Wv <= 128, H <= 256.  Deterministic.
  */
@@ -406,6 +409,7 @@ typedef struct l1attn_masked_desc {
     const float* slopes;
     const int32_t* doc;
     const int32_t* prefix;
+    void *o_rest;
 } l1attn_masked_desc;
 
 size_t l1attn_masked_fwd_workspace_bytes(const l1attn_masked_desc* desc);

@@ -60,7 +60,7 @@ class MaskedDesc(ctypes.Structure):
     """l1attn_masked_desc of the C header."""
     _fields_ = [(n, _c_i64) for n in ("B", "T", "S", "H", "Hk", "W", "Wv")] + [
         ("dtype", ctypes.c_int32), ("causal", ctypes.c_int32), ("softcap", ctypes.c_float), ("slopes", _c_p), ("doc", _c_p),
-        ("prefix", _c_p)]
+        ("prefix", _c_p), ("o_rest", _c_p)]
 
 
 def slopes_of(slopes):
@@ -125,38 +125,52 @@ def _masked_desc(q, k, v, doc, prefix, causal, softcap, slopes):
     return d
 
 
+def _kept(d):
+    """Floats of what a forward keeps for its backward, and where among them the output's rests begin: [B,T,H] logarithms of the
+    denominators, and for 16-bit types, on the next 16 bytes, what the rounding of o left out, as numbers of the type."""
+    rows = d.B * d.T * d.H
+    rest = -(-rows // 4) * 4
+    return (rows, None) if d.dtype == 0 else (rest + -(-rows * d.Wv // 2), rest)
+
+
 def masked_forward(q, k, v, doc=None, prefix=None, causal=True, softcap=0.0, slopes=None, want_lse=True):
-    """Masked L1 attention -> [o, lse]; lse [B,T,H] float32 is what the backward reads (None if not wanted)."""
+    """Masked L1 attention -> [o, kept]; kept, a row of float32, is what the backward reads (None if not wanted)."""
     d = _masked_desc(q, k, v, doc, prefix, causal, softcap, slopes)
     o = torch.empty((d.B, d.T, d.H, d.Wv), dtype=q.dtype, device=q.device)
-    lse = torch.empty((d.B, d.T, d.H), dtype=torch.float32, device=q.device) if want_lse else None
+    floats, rest = _kept(d)
+    kept = torch.empty(floats, dtype=torch.float32, device=q.device) if want_lse else None
+    if want_lse and rest is not None:
+        d.o_rest = kept.data_ptr() + 4 * rest
     L = lib()
     with torch.cuda.device(q.device):
         n = L.l1attn_masked_fwd_workspace_bytes(ctypes.addressof(d))
         ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
         rc = L.l1attn_masked_fwd(ctypes.addressof(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-                                 None if lse is None else lse.data_ptr(), ws.data_ptr() if n else None, n, stream_of(q))
+                                 None if kept is None else kept.data_ptr(), ws.data_ptr() if n else None, n, stream_of(q))
     check(rc, "l1attn_masked_fwd")
-    return [o, lse]
+    return [o, kept]
 
 
-def masked_backward(d_o, q, k, v, o, lse, doc=None, prefix=None, causal=True, softcap=0.0, slopes=None):
-    """Gradients of masked_forward -> [dq, dk, dv] from its o and lse."""
+def masked_backward(d_o, q, k, v, o, kept, doc=None, prefix=None, causal=True, softcap=0.0, slopes=None):
+    """Gradients of masked_forward -> [dq, dk, dv] from its o and what it kept."""
     d = _masked_desc(q, k, v, doc, prefix, causal, softcap, slopes)
-    for x, n in ((d_o, "d_o"), (o, "o"), (lse, "lse")):
+    for x, n in ((d_o, "d_o"), (o, "o"), (kept, "kept")):
         check_input(x, n)
     shape = (d.B, d.T, d.H, d.Wv)
     for x, n in ((d_o, "d_o"), (o, "o")):
         if tuple(x.shape) != shape or x.dtype != q.dtype or x.device != q.device:
             raise RuntimeError("%s must be [batch, n_query, n_heads, value width] with the dtype and device of q" % n)
-    if tuple(lse.shape) != shape[:3] or lse.dtype != torch.float32 or lse.device != q.device:
-        raise RuntimeError("lse must be the [batch, n_query, n_heads] float32 tensor that the forward returned")
+    floats, rest = _kept(d)
+    if tuple(kept.shape) != (floats,) or kept.dtype != torch.float32 or kept.device != q.device:
+        raise RuntimeError("kept must be the %d float32 numbers that the forward returned beside o" % floats)
+    if rest is not None:
+        d.o_rest = kept.data_ptr() + 4 * rest
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
     L = lib()
     with torch.cuda.device(q.device):
         n = L.l1attn_masked_bwd_workspace_bytes(ctypes.addressof(d))
         ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-        rc = L.l1attn_masked_bwd(ctypes.addressof(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(),
+        rc = L.l1attn_masked_bwd(ctypes.addressof(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), kept.data_ptr(),
                                  d_o.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), n, stream_of(q))
     check(rc, "l1attn_masked_bwd")
     return [dq, dk, dv]

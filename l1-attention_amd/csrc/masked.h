@@ -13,6 +13,7 @@ struct L1MaskedArgs {
 	float cap, icap, rw;  // rw = 1/sqrt(W)
 	const int32_t* doc;
 	const int32_t* prefix;
+	void* rest;           // what the rounding of o to 16 bits left out, NULL where it is not wanted
 	float slopes[L1_MASKED_HEADS];
 };
 
@@ -21,7 +22,7 @@ struct L1MaskedPlan { int waves, splits; };
 
 struct L1MaskedTable {
 	int (*fwd)(L1MaskedArgs&, const L1MaskedPlan&, const void* q, const void* k, const void* v, void* o, float* lse, float* part, hipStream_t);
-	int (*rows)(const void* d_o, const void* o, float* D, int64_t rows, int Wv, hipStream_t);
+	int (*rows)(const void* d_o, const void* o, const void* rest, float* D, int64_t rows, int Wv, hipStream_t);
 	int (*side_q)(L1MaskedArgs&, const L1MaskedPlan&, const void* q, const void* k, const void* v, const void* d_o, const float* lse, const float* D, void* dq,
 	              float* part, hipStream_t);
 	int (*side_k)(L1MaskedArgs&, const L1MaskedPlan&, const void* q, const void* k, const void* v, const void* d_o, const float* lse, const float* D, void* dk,

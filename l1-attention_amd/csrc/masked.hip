@@ -37,6 +37,7 @@ L1MaskedArgs args_of(const l1attn_masked_desc* d, const void* q, const void* k, 
 	A.causal = d->causal; A.cap = d->softcap; A.icap = l1_icap(d->softcap);
 	A.rw = (float)(1.0 / sqrt((double)d->W));
 	A.doc = d->doc; A.prefix = d->causal ? d->prefix : nullptr; A.has_slopes = d->slopes != nullptr;
+	A.rest = d->dtype == 0 ? nullptr : d->o_rest;
 	for (int h = 0; h < L1_MASKED_HEADS; h++) A.slopes[h] = d->slopes && h < d->H ? d->slopes[h] : 0.f;
 	const int per = d->dtype == 0 ? 4 : 8;
 	A.vec = (d->W % per == 0 && !((uintptr_t)q & 15) ? 1 : 0) | (d->W % per == 0 && !((uintptr_t)k & 15) ? 2 : 0) |
@@ -97,6 +98,7 @@ int l1attn_masked_fwd(const l1attn_masked_desc* desc, const void* q, const void*
 	const size_t need = l1attn_masked_fwd_workspace_bytes(desc);
 	if (need && (!workspace || workspace_bytes < need)) return L1ATTN_ERR_WORKSPACE;
 	L1MaskedArgs A = args_of(desc, q, k, v, o);
+	if ((uintptr_t)A.rest & 15) A.vec &= ~8;
 	return table_of(desc->dtype).fwd(A, plan_fwd(desc), q, k, v, o, lse, need ? (float*)workspace : nullptr, (hipStream_t)stream);
 }
 
@@ -134,7 +136,7 @@ int l1attn_masked_bwd(const l1attn_masked_desc* desc, const void* q, const void*
 	const int64_t rows = desc->B * desc->T * desc->H;
 	float* D = (float*)workspace;
 	float* part = (float*)((char*)workspace + l1_align_up((size_t)rows * sizeof(float), 256));
-	int e = t.rows(d_o, o, D, rows, A.Wv, st);
+	int e = t.rows(d_o, o, A.rest, D, rows, A.Wv, st);
 	if (e == L1ATTN_OK) e = t.side_q(A, plan_q(desc), q, k, v, d_o, lse, D, dq, part, st);
 	if (e == L1ATTN_OK) e = t.side_k(A, plan_k(desc), q, k, v, d_o, lse, D, dk, dv, part, st);
 	return e;

@@ -14,6 +14,9 @@ causal is off, or s <= i, or s < prefix[b] (int32 [B]: a prefix that sees all of
 and, with doc (int32 [B,S]), where both are of one document: equal numbers >= 0; a negative number is padding, which sees
 nothing and is seen by nothing.  A row that sees nothing is zero, as are its gradients.  The 1 in the denominator is the framework's no-op logit.
 
+For its backward a forward keeps the inputs, o and 4 bytes for each row and head, and for 16-bit types what the rounding of o left
+out, as large as o.
+
 slopes: H numbers >= 0 (constants, no gradient).  softcap >= 0, 0 for none.  Calls on several streams and in graph capture
 are fine: a call keeps nothing.  As with any operator, a backward pass is captured with no eager graph of the same leaves alive.
 """
@@ -29,16 +32,16 @@ class L1AttnMaskedFn(Function):
     def forward(ctx, q, k, v, doc=None, prefix=None, causal=True, softcap=0.0, slopes=None):
         q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
         slopes = None if slopes is None else _drv.slopes_of(slopes)  # as numbers: the backward's are the forward's
-        o, lse = _drv.masked_forward(q, k, v, doc, prefix, causal, softcap, slopes, any(ctx.needs_input_grad[:3]))
-        ctx.save_for_backward(q, k, v, o, lse, doc, prefix)
+        o, kept = _drv.masked_forward(q, k, v, doc, prefix, causal, softcap, slopes, any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(q, k, v, o, kept, doc, prefix)
         ctx.rule = (causal, softcap, slopes)
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_o):
-        q, k, v, o, lse, doc, prefix = ctx.saved_tensors
-        dq, dk, dv = _drv.masked_backward(d_o.contiguous(), q, k, v, o, lse, doc, prefix, *ctx.rule)
+        q, k, v, o, kept, doc, prefix = ctx.saved_tensors
+        dq, dk, dv = _drv.masked_backward(d_o.contiguous(), q, k, v, o, kept, doc, prefix, *ctx.rule)
         return dq, dk, dv, None, None, None, None, None
 
 

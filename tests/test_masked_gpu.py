@@ -202,6 +202,25 @@ def test_rows_of_few_values(W, dtype, rng):
     _check(q, k, v, do, doc=torch.arange(128, dtype=torch.int32)[None].cuda())
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("B,T,H,Wv", [(1, 512, 2, 64), (1, 512, 2, 37), (8, 150, 32, 64), (8, 150, 32, 33)])
+def test_values_with_a_common_part(B, T, H, Wv, dtype):
+    # do . v and do . o nearly cancel.  With u the half step: the gradients' own rounding is u of them at most, so u rms; of the terms
+    # (which hold 2 |do||o|) u^2 is what two numbers of the type leave of o, and 32 * 2^-24 covers, rms, float32 sums of up to 512
+    # terms (their roundings add as a square root), of 64 differences, and exp.  Far values in each 32 rows keep 16-bit codes out.
+    q, k, v, do = _inputs(B, T, T, H, H, 64, Wv, dtype, 55, 0.1)
+    v += 16
+    q[:, ::32, :, 0], k[:, 1::32, :, 0] = 100.0, 100.0
+    got = _run(q, k, v, do)
+    u = torch.finfo(dtype).eps / 2
+    rms = lambda x: float(x.double().square().mean().sqrt())  # noqa: E731
+    for b, h in {(0, 0), (B - 1, H - 1)}:
+        ref, terms = lf.masked(*(x[b:b + 1, :, h:h + 1] for x in (q, k, v, do)))
+        for n, x, r, t in zip(("dq", "dk"), got[1:3], ref[1:3], terms[1:3]):
+            off, room = rms(x[b:b + 1, :, h:h + 1].cpu() - r), u * rms(r) + (u * u + 32 * 2.0 ** -24) * rms(t)
+            assert off <= room, "%s: off by %.3g of its size rms where %.3g is allowed" % (n, off / rms(r), room / rms(r))
+
+
 def test_a_prefix_changes_nothing_without_causal():
     q, k, v, do = _inputs(2, 70, 70, 2, 1, 33, 40, BF16, 32)
     prefix = torch.tensor([30, 0], dtype=torch.int32).cuda()
