@@ -10,9 +10,10 @@
 // |difference| of 16-bit codes (v_sad_u16, two elements an instruction) on one grid over the rows' values and over what the
 // scales of the workgroup's pages allow (128 times the largest); what that does to a logit: codes.h.  Past the range that is
 // allowed there, or where a row or scale is not finite, float32.
-// Sums.  Weight times scale is two numbers of the rows' type, itself rounded and what that leaves out (float16 at 2^14 over the
-// power of two above the step's largest scale; one number alone made results 1.6 times as inexact as their own rounding), a code is
-// exact in it, and matrix instructions add them in float32; float32 has its own matrix instruction.
+// Sums.  For 16-bit rows weight times scale is two bfloat16 numbers, itself rounded and what that leaves out (2^-18 of it at most; one
+// number alone made results 1.6 times as inexact as their own rounding), a code is exact in bfloat16, and matrix instructions add
+// them in float32.  Not float16 for float16 rows: it would want a power of two over all tokens of a step, where one token's large
+// scale takes the digits of the others' weights, also in rows that do not see it.  float32 has its own matrix instruction.
 // What bounds it: for few rows latency and the reads (32 sequences of about 2050 tokens, 4 rows, W 64, bfloat16: 34 MB in 17 us, and 4 for the join),
 // for many the vector ALU (16 of about 20480, 16 rows, W 128, float16: 140 us at 2.4 TB/s; 43 of 100 vector instructions are
 // v_sad_u16, which issue in about 4.2 cycles each; the rest makes codes and float16 of the cache's bytes, and weights).  With
@@ -26,9 +27,7 @@
 namespace {
 
 typedef float f4 __attribute__((ext_vector_type(4)));
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
 struct AttendArgs {
 	L1Cache C;
@@ -124,11 +123,11 @@ template <typename ST, int RB, int NC, bool FULL, int MINW>
 __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST* __restrict__ q, const int32_t* __restrict__ seqs,
                                                           const int32_t* __restrict__ counts, ST* __restrict__ o, float* __restrict__ part, int2* __restrict__ spans)
 {
-	constexpr bool F32 = sizeof(ST) == 4, HALF = std::is_same_v<ST, _Float16>, CODED = !F32 && RB >= 8;
+	constexpr bool F32 = sizeof(ST) == 4, CODED = !F32 && RB >= 8;
 	constexpr bool LATE = RB >= 8;  // values are asked for behind the distances: registers hold the rows' codes read ahead (183 -> 164 us)
 	constexpr int U = RB <= 4 ? 1 : 2, VG = NC / 4, KB = RB >= 8 ? 2 : 4;  // KB: pieces of 16 bytes of a key row under way
 	constexpr int pitch = 64 * U + (F32 ? 4 : 8);                          // between two rows' weights: an odd number of 16-byte pieces
-	using PT = ST;
+	using PT = std::conditional_t<F32, float, __bf16>;                      // of the weights
 	constexpr int TR = 256 / RB;  // threads of a row before and behind the loop
 	constexpr int plane = F32 ? 0 : RB * pitch;  // 16-bit weights: what their rounding leaves out lies behind them
 	constexpr int pool = 4 * (RB * pitch + plane) * (int)sizeof(PT), join = 2 * RB * 128 * 4;
@@ -395,19 +394,6 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 			}
 		}
 		if constexpr (LATE) load_values();
-		// float16 weights: times 2^14 over the power of two above the largest scale of the step's values, and back; the other types'
-		// exponents reach as far as float32's
-		float up = 1.f, down = 1.f;
-		if constexpr (HALF) {
-			float most = 0.f;
-#pragma unroll
-			for (int u = 0; u < U; u++) most = fmaxf(most, __builtin_fabsf(vs[u]) <= 3.402823466e38f ? __builtin_fabsf(vs[u]) : 0.f);  // a hidden token's may be anything
-#pragma unroll
-			for (int k = 32; k; k >>= 1) most = fmaxf(most, __shfl_xor(most, k));
-			const int ve = most > 0.f ? max(__builtin_amdgcn_frexp_expf(most), -100) : 0;
-			up = __builtin_amdgcn_ldexpf(1.f, 14 - ve);
-			down = __builtin_amdgcn_ldexpf(1.f, ve - 14);
-		}
 #pragma unroll
 		for (int u = 0; u < U; u++)
 #pragma unroll
@@ -433,21 +419,20 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 				for (int u = 0; u < U; u++)
 #pragma unroll
 					for (int r = 0; r < RB; r++) {
-					float d;
-					dist[u][r] = A.cap * (F32 ? tanhf(dist[u][r] * A.icap) : l1_tanh_far(dist[u][r] * A.icap, d));
-				}
+						float d;
+						dist[u][r] = A.cap * (F32 ? tanhf(dist[u][r] * A.icap) : l1_tanh_far(dist[u][r] * A.icap, d));
+					}
 			}
 		}
 #pragma unroll
 		for (int u = 0; u < U; u++) {
 			const int t = t0 + 64 * u + lane, sees = pg[u] >= 0 ? t : 0x7fffffff;
-			const float scale = vs[u] * up;
 #pragma unroll
 			for (int r = 0; r < RB; r++) {
 				const float w = exponential<ST>(__builtin_fmaf(-slope[r], (float)(place[r] - t), dist[u][r]));
 				const float p = sees <= place[r] ? w : 0.f;
 				den[r] += p;
-				const float both = p != 0.f ? p * scale : 0.f;  // the scale of a hidden token has no influence
+				const float both = p != 0.f ? p * vs[u] : 0.f;  // the scale of a hidden token has no influence
 				const PT first = (PT)both;
 				ps[r * pitch + 64 * u + lane] = first;
 				if constexpr (!F32) ps[plane + r * pitch + 64 * u + lane] = (PT)(both - (float)first);
@@ -457,9 +442,6 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 		__builtin_amdgcn_wave_barrier();
 #pragma unroll
 		for (int wg = 0; wg < VG; wg++) {
-			f4 y[4];
-#pragma unroll
-			for (int e = 0; e < 4; e++) y[e] = HALF ? (f4)(0.f) : acc[wg][e];
 #pragma unroll
 			for (int kc = 0; kc < 16 * U / VT; kc++) {
 				const uint4 pa = *reinterpret_cast<const uint4*>(ps + l16 % RB * pitch + 4 * VT * kc + VT * g);
@@ -471,7 +453,7 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 						float x[4];
 						codes4((int)vr[kc][wg][d], x);
 #pragma unroll
-						for (int e = 0; e < 4; e++) y[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[d], x[e], y[e], 0, 0, 0);
+						for (int e = 0; e < 4; e++) acc[wg][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[d], x[e], acc[wg][e], 0, 0, 0);
 					}
 				} else {
 #pragma unroll
@@ -480,28 +462,16 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 #pragma unroll
 						for (int d = 0; d < 4; d++) {
 							const unsigned v0 = vr[kc][wg][2 * d], v1 = vr[kc][wg][2 * d + 1];
-							if constexpr (HALF) {
-								// byte e of two tokens, plus 128, behind the bits of 1024: then without the 1152
-								const unsigned two = __builtin_amdgcn_perm(v1 ^ 0x80808080u, v0 ^ 0x80808080u, 0x0c040c00u + 0x00010001u * e) | 0x64006400u;
-								x[d] = __builtin_bit_cast(unsigned, __builtin_bit_cast(h2, two) - (h2){(_Float16)1152.f, (_Float16)1152.f});
-							} else {
-								// a code's float32 ends in 16 zero bits
-								const float a = (float)(int8_t)(v0 >> 8 * e), c = (float)(int8_t)(v1 >> 8 * e);
-								x[d] = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, c), __builtin_bit_cast(unsigned, a), 0x07060302u);
-							}
+							// a code's float32 ends in 16 zero bits
+							const float a = (float)(int8_t)(v0 >> 8 * e), c = (float)(int8_t)(v1 >> 8 * e);
+							x[d] = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, c), __builtin_bit_cast(unsigned, a), 0x07060302u);
 						}
 						const uint4 pb = make_uint4(x[0], x[1], x[2], x[3]);
 #pragma unroll
-						for (int d = 0; d < 2; d++) {
-							const uint4 w = d ? rest : pa;
-							if constexpr (HALF) y[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, w), __builtin_bit_cast(h8, pb), y[e], 0, 0, 0);
-							else y[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, w), __builtin_bit_cast(b8, pb), y[e], 0, 0, 0);
-						}
+						for (int d = 0; d < 2; d++) acc[wg][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, d ? rest : pa), __builtin_bit_cast(b8, pb), acc[wg][e], 0, 0, 0);
 					}
 				}
 			}
-#pragma unroll
-			for (int e = 0; e < 4; e++) acc[wg][e] = HALF ? acc[wg][e] + y[e] * down : y[e];
 		}
 		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 		__builtin_amdgcn_wave_barrier();

@@ -265,6 +265,20 @@ def test_scales_of_hidden_tokens_have_no_influence(H, dtype):
     assert (got[:, :36].float() - want[:, :36].float()).abs().max() <= tol
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("H", [2, 20])
+def test_hidden_scales_that_are_large(H, dtype):
+    # the last page's values are finite and beyond float16; the tokens before it do not see them
+    c = Pair(N=40, P=16, Hk=2, W=64, Wv=64, rows=1, M=8, dtype=F32, seed=3)
+    c.append(1, 96)
+    k, v = c.data(1, 4)
+    c.append(1, 4, data=(k, v * 1e30))
+    q = torch.randn(1, 40, H, 64, generator=c.g).to(dtype)
+    o = c.m.l1attn_paged(q.cuda(), c.gpu)[:, :36]
+    ref, terms = c.plain.attend(q)
+    lf.check([o], [ref[:, :36]], [terms[:, :36]], dtype, 64, names=("o",))
+
+
 @pytest.mark.parametrize("H", [2, 12])
 def test_two_calls_at_once(H):
     c = Pair(N=80, P=32, Hk=2, W=64, Wv=64, rows=4, M=40, seed=4)
