@@ -435,7 +435,8 @@ __global__ void __launch_bounds__(256, MINW) paged_attend(AttendArgs A, const ST
 				const float both = p != 0.f ? p * vs[u] : 0.f;  // the scale of a hidden token has no influence
 				const PT first = (PT)both;
 				ps[r * pitch + 64 * u + lane] = first;
-				if constexpr (!F32) ps[plane + r * pitch + 64 * u + lane] = (PT)(both - (float)first);
+				const float rest = both - (float)first;  // an infinite weight has none: infinity less itself is NaN
+				if constexpr (!F32) ps[plane + r * pitch + 64 * u + lane] = (PT)(__builtin_fabsf(rest) <= 3.402823466e38f ? rest : 0.f);
 			}
 		}
 		__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

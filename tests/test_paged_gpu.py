@@ -279,6 +279,22 @@ def test_hidden_scales_that_are_large(H, dtype):
     lf.check([o], [ref[:, :36]], [terms[:, :36]], dtype, 64, names=("o",))
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("H", [2, 20])
+def test_visible_infinite_scales(H, dtype):
+    # infinity times a code that is not zero, of one sign in each column: infinity, as of the formula
+    c = Pair(N=40, P=16, Hk=2, W=64, Wv=64, rows=1, M=8, dtype=dtype, seed=5)
+    k, v = c.data(1, 100)
+    v = v.abs() + 1.0
+    v[:, :, :, 1::2] *= -1
+    c.append(1, 100, data=(k, v))
+    page = int(c.gpu.table[0, 2])
+    c.gpu.v_scale[page] = float("inf")
+    q = torch.randn(1, 3, H, 64, generator=c.g).to(dtype).cuda()
+    o = c.m.l1attn_paged(q, c.gpu)
+    assert (o[..., 0::2] == float("inf")).all() and (o[..., 1::2] == -float("inf")).all()
+
+
 @pytest.mark.parametrize("H", [2, 12])
 def test_two_calls_at_once(H):
     c = Pair(N=80, P=32, Hk=2, W=64, Wv=64, rows=4, M=40, seed=4)
