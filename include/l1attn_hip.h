@@ -400,7 +400,8 @@ int l1attn_sparse_bidi_bwd_bf16(const void* dvo, const void* vf, const void* vb,
  * backward adds it to o for sum d_o * o, which is taken off each d_o . v: without it the rounding of o alone moves dq and dk by
  * several times their own rounding where the values v have a part in common.
  * doc [B,S] and prefix [B] are device pointers to int32 or NULL; slopes is a HOST pointer to H numbers >= 0, or NULL, read
- * during the call.  T <= S <= 4194240, W and Wv <= 128, H <= 256.  Deterministic.
+ * during the call.  T <= S <= 4194240, W and Wv <= 128, H <= 256, B <= 4194304 and B H <=
+ * 16777215 (8388607 for float32 of widths up to 64).  Deterministic.
  */
 typedef struct l1attn_masked_desc {
     int64_t B, T, S, H, Hk, W, Wv;

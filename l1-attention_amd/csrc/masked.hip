@@ -8,11 +8,15 @@ namespace {
 
 __global__ void __launch_bounds__(256) masked_zero(uint16_t* __restrict__ x, int64_t n)
 {
-	const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-	if (at < n) x[at] = 0;
+	for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < n; at += (int64_t)gridDim.x * 256) x[at] = 0;
 }
 
+unsigned zero_blocks(int64_t n) { return (unsigned)(n < 256 << 16 ? l1_cdiv(n, 256) : 1 << 16); }
+
 bool fits(int64_t x, int64_t most) { return x >= 0 && x <= most; }
+
+// waves of a workgroup: as many as share what they stage, see plan_of
+int most_waves(const l1attn_masked_desc* d) { return d->dtype == 0 && d->W <= 64 && d->Wv <= 64 ? 8 : 4; }
 
 // 0, an error, or 1 for a call with nothing to do
 int check_desc(const l1attn_masked_desc* d)
@@ -21,8 +25,9 @@ int check_desc(const l1attn_masked_desc* d)
 	if (d->B < 0 || d->T < 0 || d->S < d->T || d->H < 1 || d->Hk < 1 || d->H % d->Hk || d->W < 1 || d->Wv < 1) return L1ATTN_ERR_ARG;
 	if (d->dtype < 0 || d->dtype > 2 || (d->causal != 0 && d->causal != 1)) return L1ATTN_ERR_ARG;
 	if (!(d->softcap >= 0.f) || !(d->softcap <= 3e38f)) return L1ATTN_ERR_ARG;
-	// 65535 rows of the grid at two waves of 32 rows; batch * heads is the grid's other side
-	if (d->W > 128 || d->Wv > 128 || d->H > L1_MASKED_HEADS || !fits(d->S, 64 * 65535) || !fits(d->B, 1 << 22) || !fits(d->B * d->H, 1 << 30))
+	// 65535 rows of the grid at two waves of 32 rows; batch * heads is the grid's other side, which has 2^32 - 1 threads at most
+	if (d->W > 128 || d->Wv > 128 || d->H > L1_MASKED_HEADS || !fits(d->S, 64 * 65535) || !fits(d->B, 1 << 22) ||
+	    !fits(d->B * d->H, 0xffffffffll / (64 * most_waves(d))))
 		return L1ATTN_ERR_RANGE;
 	if (d->slopes)
 		for (int64_t h = 0; h < d->H; h++)
@@ -57,7 +62,7 @@ L1MaskedPlan plan_of(const L1MaskedTable& t, int64_t owners, int64_t stream, int
 {
 	L1MaskedPlan p;
 	const int W = (int)d->W, Wv = (int)d->Wv;
-	p.waves = d->dtype == 0 && W <= 64 && Wv <= 64 ? 8 : 4;
+	p.waves = most_waves(d);
 	while (p.waves > 2 && (t.lds(W, Wv, p.waves, backward, weigh) > 160 * 1024 || heads * l1_cdiv(owners, 32 * p.waves) < 256)) p.waves >>= 1;
 	int64_t s = l1_cdiv(1024, heads * l1_cdiv(owners, 32 * p.waves));
 	if (s > l1_cdiv(stream, 64) / 2) s = l1_cdiv(stream, 64) / 2;
@@ -125,9 +130,9 @@ int l1attn_masked_bwd(const l1attn_masked_desc* desc, const void* q, const void*
 	hipStream_t st = (hipStream_t)stream;
 	if (rc == 1) {  // keys that no query reads
 		const int64_t half = desc->dtype == 0 ? 2 : 1, nk = desc->B * desc->S * desc->Hk * desc->W * half, nv = nk / desc->W * desc->Wv;
-		hipLaunchKernelGGL(masked_zero, dim3((unsigned)l1_cdiv(nk, 256)), dim3(256), 0, st, (uint16_t*)dk, nk);
+		hipLaunchKernelGGL(masked_zero, dim3(zero_blocks(nk)), dim3(256), 0, st, (uint16_t*)dk, nk);
 		L1_LAUNCH_CHECK();
-		hipLaunchKernelGGL(masked_zero, dim3((unsigned)l1_cdiv(nv, 256)), dim3(256), 0, st, (uint16_t*)dv, nv);
+		hipLaunchKernelGGL(masked_zero, dim3(zero_blocks(nv)), dim3(256), 0, st, (uint16_t*)dv, nv);
 		L1_LAUNCH_CHECK();
 		return L1ATTN_OK;
 	}

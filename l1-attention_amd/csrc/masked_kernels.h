@@ -1072,14 +1072,16 @@ template <typename ST>
 __global__ void __launch_bounds__(256) masked_bwd_rows(const ST* __restrict__ dout, const ST* __restrict__ o, const ST* __restrict__ rest,
                                                        float* __restrict__ D, int64_t rows, int Wv)
 {
-	const int64_t row = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
-	float s = 0.f;
-	if (row < rows)
-		for (int w = threadIdx.x & 7; w < Wv; w += 8) s += to_f(dout[row * Wv + w]) * (to_f(o[row * Wv + w]) + (k16<ST> && rest ? to_f(rest[row * Wv + w]) : 0.f));
-	s += __shfl_xor(s, 1);
-	s += __shfl_xor(s, 2);
-	s += __shfl_xor(s, 4);
-	if (row < rows && (threadIdx.x & 7) == 0) D[row] = s;
+	for (int64_t first = (int64_t)blockIdx.x * 32; first < rows; first += (int64_t)gridDim.x * 32) {  // the same steps for all threads
+		const int64_t row = first + (threadIdx.x >> 3);
+		float s = 0.f;
+		if (row < rows)
+			for (int w = threadIdx.x & 7; w < Wv; w += 8) s += to_f(dout[row * Wv + w]) * (to_f(o[row * Wv + w]) + (k16<ST> && rest ? to_f(rest[row * Wv + w]) : 0.f));
+		s += __shfl_xor(s, 1);
+		s += __shfl_xor(s, 2);
+		s += __shfl_xor(s, 4);
+		if (row < rows && (threadIdx.x & 7) == 0) D[row] = s;
+	}
 }
 
 // sum of the splits' gradients, in their order
@@ -1480,7 +1482,8 @@ struct MaskedImpl {
 	}
 	static int rows(const void* dout, const void* o, const void* rest, float* D, int64_t rows, int Wv, hipStream_t st)
 	{
-		hipLaunchKernelGGL(masked_bwd_rows<ST>, dim3((unsigned)l1_cdiv(rows, 32)), dim3(256), 0, st, (const ST*)dout, (const ST*)o, (const ST*)rest, D, rows, Wv);
+		const int64_t blocks = l1_cdiv(rows, 32), most = 1 << 23;  // a grid has 2^32 - 1 threads at most
+		hipLaunchKernelGGL(masked_bwd_rows<ST>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, st, (const ST*)dout, (const ST*)o, (const ST*)rest, D, rows, Wv);
 		L1_LAUNCH_CHECK();
 		return L1ATTN_OK;
 	}

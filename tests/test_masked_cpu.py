@@ -92,6 +92,19 @@ def test_c_entry_codes():
     assert L.l1attn_masked_bwd(ctypes.addressof(d), one, None, *[one] * 8, n, None) == -1
 
 
+def test_batches_past_a_launch_are_refused():
+    # a launch has 2^32 - 1 threads at most along batch and heads
+    L = drv.lib()
+    one = ctypes.c_void_p(16)
+    for kw in (dict(B=1 << 20, H=16, Hk=16, dtype=1), dict(B=1 << 19, H=16, Hk=1), dict(B=1 << 20, H=16, Hk=16, W=65)):
+        d = drv.MaskedDesc(**{**dict(B=1, T=1, S=1, H=2, Hk=2, W=8, Wv=8, dtype=0, causal=1), **kw})
+        a = ctypes.addressof(d)
+        assert L.l1attn_masked_fwd(a, one, one, one, one, None, None, 0, None) == -3, kw
+        assert L.l1attn_masked_bwd(a, *[one] * 10, 1 << 40, None) == -3, kw
+        d.B -= 1  # the largest batch: looked at as far as the workspace
+        assert L.l1attn_masked_bwd(a, *[one] * 10, 0, None) == -2, kw
+
+
 def test_the_plain_statement_is_the_framework_s_own():
     # without masks it is what the fused operator's closed form says, and its gradients are autograd's
     import closed_forms as cf

@@ -378,6 +378,30 @@ def test_empty():
     assert g[0].shape == q.shape and (g[1] == 0).all()
 
 
+def test_a_large_batch_of_small_rows():
+    # more than 2^29 rows of queries
+    B, T, H = 1048575, 33, 16
+    g = torch.Generator(device="cuda").manual_seed(57)
+    q, k, v, do = (torch.randn(B, T, H, 1, generator=g, device="cuda", dtype=F16) for _ in range(4))
+    got = _run(q, k, v, do)
+    for b in (0, B // 2, B - 1):
+        ref, terms = lf.masked(*(x[b:b + 1] for x in (q, k, v, do)))
+        lf.check([x[b:b + 1] for x in got], ref, terms, F16, 1)
+
+
+def test_no_queries_for_many_keys():
+    # more than 2^32 numbers of dk, on memory that holds others
+    k = torch.ones(1, 4194240, 8, 128, dtype=F16, device="cuda")
+    ones = torch.ones_like(k)
+    del ones
+    k.requires_grad_()
+    v = torch.ones(1, 4194240, 8, 1, dtype=F16, device="cuda", requires_grad=True)
+    q = torch.zeros(1, 0, 8, 128, dtype=F16, device="cuda", requires_grad=True)
+    o = _op()(q, k, v)
+    for x in torch.autograd.grad(o, (k, v), torch.zeros_like(o)):
+        assert not x.any()
+
+
 def test_it_trains():
     torch.manual_seed(0)
     lin = torch.nn.Linear(32, 3 * 64).cuda()
