@@ -446,6 +446,7 @@ typedef struct l1attn_cache {
  * behind sequence seqs[b] (b without seqs).  A page's scale is its values' largest magnitude over 127; where new tokens make
  * it grow, the codes that are there become rint(code * old / new).  A partly filled page that others hold too is copied.
  * Served as long as the pages last, in the order of the entries, and where the row of the table has room.
+ * B * (ceil(n / page) + 1) <= 16777215.
  */
 size_t l1attn_cache_append_workspace_bytes(const l1attn_cache* cache, int64_t B, int64_t n);
 int l1attn_cache_append(const l1attn_cache* cache, int dtype, const void* k, const void* v, const int32_t* seqs, const int32_t* counts,

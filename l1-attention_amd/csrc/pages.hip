@@ -453,7 +453,7 @@ int l1attn_cache_append(const l1attn_cache* cache, int dtype, const void* k, con
 	if (B == 0) return L1ATTN_OK;
 	if (!served || (n && (!k || !v))) return L1ATTN_ERR_ARG;
 	const int J = pages_of(n, C.P);
-	if ((int64_t)B * J > 0x7fffffff) return L1ATTN_ERR_RANGE;
+	if ((int64_t)B * J > 0xffffff) return L1ATTN_ERR_RANGE;  // 2^32 - 1 threads of the second launch: refused before the first one
 	if (!workspace || workspace_bytes < l1attn_cache_append_workspace_bytes(cache, B, n)) return L1ATTN_ERR_WORKSPACE;
 	hipStream_t st = (hipStream_t)stream;
 	int4* plan = (int4*)workspace;

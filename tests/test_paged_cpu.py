@@ -122,6 +122,17 @@ def test_c_entry_codes():
     assert attend(B=0) == 0 and attend(n=0) == 0
 
 
+def test_appends_past_a_launch_are_refused():
+    # a workgroup of 256 threads for each page of each entry, 2^32 - 1 threads at most: refused while the cache is as it was
+    L = drv.lib()
+    p = 4096  # never read
+    c = drv.CacheDesc(n_pages=4, page=16, Hk=2, W=16, Wv=16, rows=64, row_pages=5,
+                      **{n: p for n in ("k_pages", "v_pages", "k_scale", "v_scale", "table", "lens", "refs", "free_pages", "n_free")})
+    a = ctypes.addressof(c)
+    for B, n, rc in ((64, 16 * ((1 << 18) - 1), -3), (1, 1 << 28, -3), (64, 16 * ((1 << 18) - 2), -2)):
+        assert L.l1attn_cache_append(a, 1, p, p, None, None, B, n, p, p, 0, None) == rc, (B, n)
+
+
 def test_the_plain_model_keeps_its_pages_together():
     import random
     r = random.Random(1)
