@@ -325,10 +325,10 @@ __global__ void __launch_bounds__(256) cache_move(L1Cache C, const int32_t* __re
 // third part: the tables
 __global__ void __launch_bounds__(256) cache_rename(L1Cache C, const int32_t* __restrict__ map)
 {
-	const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x;
-	if (x >= (int64_t)C.rows * C.M) return;
-	const int page = C.table[x];
-	if (page >= 0 && page < C.N) C.table[x] = map[page];
+	for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < (int64_t)C.rows * C.M; x += (int64_t)gridDim.x * 256) {
+		const int page = C.table[x];
+		if (page >= 0 && page < C.N) C.table[x] = map[page];
+	}
 }
 
 // ------------------------------------------------------------------------------------------------------------ new tokens
@@ -548,7 +548,8 @@ int l1attn_cache_compact(const l1attn_cache* cache, int32_t* live, void* workspa
 	hipLaunchKernelGGL(cache_move, dim3(2048), dim3(256), 0, st, C, order, holes, map, sums);
 	L1_LAUNCH_CHECK();
 	if ((int64_t)C.rows * C.M) {
-		hipLaunchKernelGGL(cache_rename, dim3((unsigned)l1_cdiv((int64_t)C.rows * C.M, 256)), dim3(256), 0, st, C, map);
+		const int64_t blocks = l1_cdiv((int64_t)C.rows * C.M, 256), most = 1 << 23;  // a grid has 2^32 - 1 threads at most
+		hipLaunchKernelGGL(cache_rename, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, st, C, map);
 		L1_LAUNCH_CHECK();
 	}
 	return L1ATTN_OK;

@@ -418,6 +418,24 @@ def test_graph_of_a_decode_step_and_other_streams():
             assert all(torch.equal(x, y) for x, y in zip(state(c), state(eager)))
 
 
+def test_compact_with_a_table_of_more_than_2_32_entries():
+    import l1attn_paged_cuda as m
+    M = 1 << 24
+    N, rows = 8, 260
+    z = lambda *s, dtype=torch.int32: torch.zeros(*s, dtype=dtype, device="cuda")  # noqa: E731
+    table = torch.full((rows, M), -1, dtype=torch.int32, device="cuda")
+    c = m.L1PagedCache(z(N, 1, 16, 16, dtype=torch.int8), z(N, 1, 16, 16, dtype=torch.int8), z(N, 1, dtype=F32), z(N, 1, dtype=F32), table, z(rows), z(N),
+                       torch.arange(N - 1, -1, -1, dtype=torch.int32, device="cuda"), z(1) + N)
+    x = torch.randn(2, 20, 1, 16, generator=torch.Generator().manual_seed(1)).cuda()
+    assert c.append(x, x, seqs=torch.tensor([3, 259], dtype=torch.int32, device="cuda")).all()  # pages 0, 1 and 2, 3
+    q = x[:, -1:].contiguous()
+    seqs = torch.tensor([259], dtype=torch.int32, device="cuda")
+    want = m.l1attn_paged(q[1:], c, seqs=seqs)
+    c.free(torch.tensor([3], dtype=torch.int32, device="cuda"))
+    assert int(c.compact()) == 2 and table[259, :3].tolist() == [0, 1, -1]
+    assert torch.equal(m.l1attn_paged(q[1:], c, seqs=seqs), want)
+
+
 def test_random_walk():
     import random
     r = random.Random(5)
