@@ -291,12 +291,16 @@ __device__ __forceinline__ void distances16(const char* own, const char* str, in
 
 // --------------------------------------------------------------------------------------------------------------- staging
 
-// columns [w0, w0 + width) of rows [r0, r0 + n) of x as float32 rows of `stride` bytes
+// Whether a float32 is below 2^-104 and not zero: two of these may differ by less than 2^-128 (others are multiples of 2^-128).
+__device__ __forceinline__ bool is_tiny(unsigned bits) { return (bits & 0x7fffffffu) - 1 < __builtin_bit_cast(unsigned, 0x1p-104f) - 1; }
+
+// columns [w0, w0 + width) of rows [r0, r0 + n) of x as float32 rows of `stride` bytes; whether a value is tiny
 template <typename ST>
-__device__ __forceinline__ void stage32(char* dst, const ST* __restrict__ x, int r0, int n, int L, int64_t pitch, int w0, int width,
+__device__ __forceinline__ bool stage32(char* dst, const ST* __restrict__ x, int r0, int n, int L, int64_t pitch, int w0, int width,
                                         int stride, bool vec, int tid, int threads)
 {
 	const int chunks = (width + 3) >> 2, j = tid & 7;
+	bool tiny = false;
 	for (int r = tid >> 3; r < n; r += threads >> 3) {
 		const ST* row = x + (int64_t)(r0 + r) * pitch + w0;
 		for (int c = j; c < chunks; c += 8) {
@@ -313,8 +317,11 @@ __device__ __forceinline__ void stage32(char* dst, const ST* __restrict__ x, int
 				}
 			}
 			*reinterpret_cast<f4*>(dst + r * stride + 16 * c) = y;
+#pragma unroll
+			for (int e = 0; e < 4; e++) tiny |= is_tiny(__builtin_bit_cast(unsigned, y[e]));
 		}
 	}
+	return tiny;
 }
 
 // the grid of a workgroup's codes
@@ -416,8 +423,9 @@ struct Stream {
 		}
 	}
 
-	// str: distance rows; raw, over, y, yt, slse, sD: see Layout, NULL where not wanted.  Whether a value was not finite.
-	__device__ __forceinline__ bool place(char* str, char* raw, float* over, char* ydst, char* yt, int* docs, float* slse, float* sD, const Layout& Y,
+	// str: distance rows; raw, over, y, yt, slse, sD: see Layout, NULL where not wanted; tiny (float32, or NULL) is set where a value
+	// is.  Whether a value was not finite.
+	__device__ __forceinline__ bool place(char* str, char* raw, float* over, char* ydst, char* yt, int* docs, float* slse, float* sD, int* tiny, const Layout& Y,
 	                                      const Grid& G, const ST* __restrict__ x, int64_t xpitch, int W, bool xvec, const ST* __restrict__ y,
 	                                      int64_t ypitch, int Wv, bool yvec, int s0, int L, int tid, int threads)
 	{
@@ -430,6 +438,7 @@ struct Stream {
 			if (r >= kTile<TB>) return;  // eight lanes at a time: a row's sum is still formed by all of its lanes
 			if constexpr (!k16<ST>) {
 				if (c < chunks) *reinterpret_cast<uint4*>(str + r * Y.so + 16 * c) = bits;
+				if (tiny && (is_tiny(bits.x) | is_tiny(bits.y) | is_tiny(bits.z) | is_tiny(bits.w))) *tiny = 1;
 			} else {
 				if (cg == 0) out = 0.f;
 				if (c < chunks) {
@@ -920,7 +929,7 @@ __global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* 
 			const int kind = __builtin_amdgcn_readfirstlane(cls[next]), s0 = (t0 + step * next) * kTile<TB>;
 			const int tid = here(threadIdx.x), lane = tid & 63, i = lane & 7, j = lane >> 3, l16 = lane & 15, g = lane >> 4;
 			__syncthreads();
-			bool bad = F.place(str, nullptr, over, k16<ST> ? nullptr : y, yt, docs, nullptr, nullptr, Y, G, kh, kpitch, A.W, A.vec & 2, vh, vpitch, A.Wv,
+			bool bad = F.place(str, nullptr, over, k16<ST> ? nullptr : y, yt, docs, nullptr, nullptr, nullptr, Y, G, kh, kpitch, A.W, A.vec & 2, vh, vpitch, A.Wv,
 			                   A.vec & 4, s0, A.S, tid, threads);
 			next = next_tile(cls, next + 1, n);
 			if (next < n) F.fetch(kh, kpitch, A.W, A.vec & 2, vh, vpitch, A.Wv, A.vec & 4, (t0 + step * next) * kTile<TB>, A.S, doc, nullptr, nullptr, 0, tid, threads);
@@ -1098,15 +1107,28 @@ __global__ void __launch_bounds__(256) masked_bwd_join(const float* __restrict__
 // Signs of one half tile: sum[u][r] += h * g over its 32 columns c, h = 1, 1/2, 0 for owner >, ==, < stream in column w = lane + 64 u.
 // Owner r = 4 i' + a' is row i' + 8 a'; scr: the gradients g [c][r].
 // 16 bits: the values as integers in order, own + 1/2: h = clamp(own + 1/2 - str, 0, 1), exact.  float32: h =
-// clamp((own - str) * 2^127 + 1/2, 0, 1), exact but for differences below 2^-128, which count in part.
+// clamp((own - str) * 2^127 + 1/2, 0, 1), exact but for differences below 2^-128; where the workgroup has met tiny values, times
+// 2^276 instead (v_ldexp takes longer: 4 % of a step, if it were taken always).
 template <typename ST, int WL>
-__device__ __forceinline__ void signs(float (&sum)[WL][32], const float (&ov)[WL][32], const float* sc, const char* str, int stride, int half, int lane, int W)
+__device__ __forceinline__ void signs(float (&sum)[WL][32], const float (&ov)[WL][32], const float* sc, const char* str, int stride, int half, int lane, int W,
+                                      bool tiny)
 {
 	const auto value = [&](int c, int u) {
 		const char* at = str + row_of(32 * half + c) * stride + (int)sizeof(ST) * min(lane + 64 * u, W - 1);
 		if constexpr (k16<ST>) return (float)*reinterpret_cast<const short*>(at);
 		else return *reinterpret_cast<const float*>(at);
 	};
+	if (!k16<ST> && tiny) {
+		for (int c = 0; c < 32; c++)
+#pragma unroll
+			for (int u = 0; u < WL; u++) {
+				const float s = value(c, u);
+#pragma unroll
+				for (int r = 0; r < 32; r++)
+					sum[u][r] = __builtin_fmaf(__builtin_amdgcn_fmed3f(__builtin_amdgcn_ldexpf(ov[u][r] - s, 276) + 0.5f, 0.f, 1.f), sc[c * kPad + r], sum[u][r]);
+			}
+		return;
+	}
 	f4 g[4], gn[4];  // the gradients of 16 owners, and of the next 16
 	float s[WL];
 #pragma unroll
@@ -1186,6 +1208,8 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 	const int64_t own_pitch = OWNK ? kpitch : qpitch, str_pitch = OWNK ? qpitch : kpitch;
 	const bool own_vec = A.vec & (OWNK ? 2 : 1), str_vec = A.vec & (OWNK ? 1 : 2);
 
+	int* tiny = reinterpret_cast<int*>(over);  // float32 has no other use of this: whether the workgroup has met tiny values
+	if (!k16<ST> && tid == 0) *tiny = 0;
 	Span mine, all;
 	bool mine_whole, all_whole;
 	owner_docs(doc, K, row0, reinterpret_cast<int*>(red), lane, wave, waves, mine, mine_whole, all, all_whole);
@@ -1195,7 +1219,7 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 		coded = owner_grid(own_x, doc, K, row0, own_pitch, A.W, own_vec, red + 32, lane, wave, waves, G);
 		stage_own16(own, lds + Y.oraw + wave * kOwn * Y.sr, own_x, row0, K.own_rows, own_pitch, A.W, Y.so, Y.sr, G, own_vec, lane);
 	} else {
-		stage32(own, own_x, row0, kOwn, K.own_rows, own_pitch, 0, A.W, Y.so, own_vec, lane, 64);
+		if (stage32(own, own_x, row0, kOwn, K.own_rows, own_pitch, 0, A.W, Y.so, own_vec, lane, 64)) *tiny = 1;
 	}
 	const int own_lo = K.own_place0 + K.own0, own_hi = K.own_place0 + min(K.own0 + K.nown, K.own_rows) - 1;
 	const int my_lo = K.own_place0 + row0, my_hi = K.own_place0 + min(row0 + kOwn, K.own_rows) - 1;
@@ -1269,11 +1293,12 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 				const int tid = here(threadIdx.x), lane = tid & 63, i = lane & 7, j = lane >> 3, l16 = lane & 15, g = lane >> 4;
 				__syncthreads();
 				// without a grid the codes come out as nonsense that nobody reads; the ordered integers are wanted all the same
-				bool bad = F.place(str, raw, over, y, k16<ST> && OWNK ? yt : nullptr, docs, OWNK ? slse : nullptr, sD, Y, G, str_x, str_pitch, A.W, str_vec,
+				bool bad = F.place(str, raw, over, y, k16<ST> && OWNK ? yt : nullptr, docs, OWNK ? slse : nullptr, sD, k16<ST> ? nullptr : tiny, Y, G, str_x, str_pitch, A.W, str_vec,
 				                   str_y, y_pitch, A.Wv, y_vec, s0, K.str_rows, tid, threads);
 				next = next_tile(cls, next + 1, n);
 				if (next < n) F.fetch(str_x, str_pitch, A.W, str_vec, str_y, y_pitch, A.Wv, y_vec, (t0 + step * next) * kTile<TB>, K.str_rows, str_doc, lh, Dh, A.H, tid, threads);
 				const int far = __syncthreads_or(bad && (k16<ST> || kind == 2)) ? kind : 0;
+				const bool exact = !k16<ST> && __builtin_amdgcn_readfirstlane(*tiny);
 				int mykind = row0 < K.own_rows ? kind : 0;
 				if (mykind == 2) {
 					mykind = place_class<OWNK>(A, prefix, my_lo, my_hi, K.str_place0 + s0, K.str_place0 + min(s0 + kTile<TB>, K.str_rows) - 1, s0 + kTile<TB> <= K.str_rows);
@@ -1383,7 +1408,7 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 							else ov[u][r] = *reinterpret_cast<const float*>(own + row * Y.so + 4 * w);
 						}
 					if constexpr (k16<ST>) {
-						signs<ST, WL>(sum, ov, sc, raw, Y.sr, half, lane, A.W);
+						signs<ST, WL>(sum, ov, sc, raw, Y.sr, half, lane, A.W, false);
 					} else {
 						// half a tile's sum on its own, then to the total: the roundings of either are fewer
 						float part[WL][32];
@@ -1391,7 +1416,7 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 						for (int u = 0; u < WL; u++)
 #pragma unroll
 							for (int r = 0; r < 32; r++) part[u][r] = 0.f;
-						signs<ST, WL>(part, ov, sc, str, Y.so, half, lane, A.W);
+						signs<ST, WL>(part, ov, sc, str, Y.so, half, lane, A.W, exact);
 #pragma unroll
 						for (int u = 0; u < WL; u++)
 #pragma unroll

@@ -288,6 +288,16 @@ def test_ties_have_no_sign():
         assert out[1].abs().max() <= 1e-5 and out[2].abs().max() <= 1e-5
 
 
+def test_signs_of_the_smallest_differences():
+    # below float32's normal numbers: a difference is a difference
+    g = torch.Generator().manual_seed(56)
+    q, k = ((torch.randn(1, 60, 2, 32, generator=g) * 1e-40).cuda() for _ in range(2))
+    k[:, :, :, ::2] = (torch.randint(-3, 4, (1, 60, 2, 16), generator=g) * 1.5e-45).cuda()
+    q[:, :, :, ::4] = 0.0
+    v, do = (torch.randn(1, 60, 2, 32, generator=g).cuda() for _ in range(2))
+    _check(q, k, v, do)
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 def test_unaligned_and_strided_inputs(dtype):
     B, T, H, W = 1, 70, 2, 64
