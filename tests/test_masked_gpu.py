@@ -315,6 +315,28 @@ def test_unaligned_and_strided_inputs(dtype):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("T,S,H,Hk,W,Wv", [(130, 130, 32, 32, 16, 24), (300, 300, 32, 32, 24, 16), (290, 333, 32, 16, 40, 72), (270, 270, 32, 32, 72, 40)])
+@pytest.mark.parametrize("rule", ["causal", "docs", "prefix"])
+def test_wide_workgroups(rule, T, S, H, Hk, W, Wv, dtype):
+    # batch and heads that fill the chip: workgroups of four waves, and of eight (float32, widths up to 64), with and without splits,
+    # the last one partly filled, over several tiles
+    B = 8 if Hk == 32 else 16
+    q, k, v, do = _inputs(B, T, S, H, Hk, W, Wv, dtype, T + W)
+    kw = {}
+    if rule == "docs":
+        kw["doc"] = _docs(B, S, 4, 5, pad=11)
+    if rule == "prefix":
+        kw = dict(prefix=torch.randint(0, S, (B,), generator=torch.Generator().manual_seed(1)).to(torch.int32).cuda(), cap=9.0, slopes=SLOPES(H))
+    got = _run(q, k, v, do, **kw)
+    G = H // Hk
+    for b, hk in ((0, 0), (B // 2, Hk // 2), (B - 1, Hk - 1)):
+        hs = slice(hk * G, hk * G + G)
+        sub = {n: x[b:b + 1] if torch.is_tensor(x) else x[hs] if n == "slopes" else x for n, x in kw.items()}
+        ref, terms = lf.masked(q[b:b + 1, :, hs], k[b:b + 1, :, hk:hk + 1], v[b:b + 1, :, hk:hk + 1], do[b:b + 1, :, hs], **sub)
+        lf.check([got[0][b:b + 1, :, hs], got[1][b:b + 1, :, hs], got[2][b:b + 1, :, hk:hk + 1], got[3][b:b + 1, :, hk:hk + 1]], ref, terms, dtype, W)
+
+
 def test_repeats_bit_for_bit_and_large_grids():
     q, k, v, do = _inputs(2, 1100, 1100, 8, 2, 64, 64, BF16, 13)
     doc = _docs(2, 1100, 4, 6)
