@@ -444,7 +444,8 @@ typedef struct l1attn_cache {
 /*
  * The first counts[b] (all n without counts) rows of k [B,n,Hk,W], v [B,n,Hk,Wv] (dtype 0 float32, 1 float16, 2 bfloat16)
  * behind sequence seqs[b] (b without seqs).  A page's scale is its values' largest magnitude over 127; where new tokens make
- * it grow, the codes that are there become rint(code * old / new).  A partly filled page that others hold too is copied.
+ * it grow, the codes that are there become rint(code * old / new).  A scale that the caller made negative becomes positive, its codes
+ * change their sign.  A partly filled page that others hold too is copied.
  * Served as long as the pages last, in the order of the entries, and where the row of the table has room.
  * B * (ceil(n / page) + 1) <= 16777215.
  */

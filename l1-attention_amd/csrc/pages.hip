@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(256) cache_write(L1Cache C, const ST* __restri
 	const float held = base < start ? scales[(int64_t)src * C.Hk + h] : 0.f;
 	__syncthreads();
 	top = fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3]));
-	const float now = fmaxf(held, top * (1.f / 127.f));
+	const float now = fmaxf(__builtin_fabsf(held), top * (1.f / 127.f));  // a scale of a pool that the caller filled may be negative
 	const float ratio = now > 0.f ? held / now : 0.f, div = now > 0.f ? now : 1.f;
 	const bool again = base < start && (copy || ratio != 1.f);
 #pragma unroll
@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(256) cache_write(L1Cache C, const ST* __restri
 		if (place < start) {
 			__builtin_memcpy(code, from + t * pitch + w, G);
 #pragma unroll
-			for (int e = 0; e < G; e++) code[e] = (int8_t)rintf((float)code[e] * ratio);
+			for (int e = 0; e < G; e++) code[e] = (int8_t)fminf(rintf((float)code[e] * ratio), 127.f);  // -128 has no opposite
 		} else {
 #pragma unroll
 			for (int e = 0; e < G; e++) {

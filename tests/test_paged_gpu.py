@@ -327,6 +327,33 @@ def test_a_pool_that_the_caller_filled(H, dtype):
     c.attend(2, 2, H)
 
 
+@pytest.mark.parametrize("new", [0.01, 3.0, 100.0])
+def test_append_to_a_pool_that_the_caller_filled(new):
+    # scales of either sign: what the old tokens are stays, to half a step of the page's new scale and its float32 roundings (to a
+    # whole step for the code -128, which has no opposite), and so do the new ones
+    c = Pair(N=30, P=16, Hk=2, W=64, Wv=64, rows=2, M=10, dtype=F32, seed=8)
+    c.append(2, 150, counts=[150, 20])
+    for x in (c.gpu.k_pages, c.gpu.v_pages):
+        x.copy_(torch.randint(-128, 128, x.shape, generator=c.g).to(torch.int8))
+    for x in (c.gpu.k_scale, c.gpu.v_scale):
+        x.copy_((torch.rand(x.shape, generator=c.g) - 0.5) / 16)
+
+    def last_page(row, place):
+        page = int(c.gpu.table[row, place // 16])
+        return [(codes[page].cpu(), scale[page].double().cpu()[:, None, None]) for codes, scale in ((c.gpu.k_pages, c.gpu.k_scale), (c.gpu.v_pages, c.gpu.v_scale))]
+    before = [last_page(row, n) for row, n in ((0, 150), (1, 20))]
+    kv = c.data(2, 3, new)
+    assert c.gpu.append(kv[0].cuda(), kv[1].cuda()).all()
+    for row, n in ((0, 150), (1, 20)):
+        at = n % 16
+        for (was, old), (now, scale), x in zip(before[row], last_page(row, n), kv):
+            assert (scale >= old.abs()).all()
+            step = scale * (1 + 2.0 ** -15)
+            room = torch.where(was == -128, step, step / 2)
+            assert ((now * scale - was * old)[:, :at].abs() <= room[:, :at]).all()
+            assert ((now * scale)[:, at:at + 3] - x[row].double().transpose(0, 1)).abs().le(step / 2).all()
+
+
 def test_pages_that_are_not_there_give_no_tokens():
     c = Pair(N=40, rows=2, M=8)
     c.append(2, 100)
