@@ -56,22 +56,23 @@ constexpr int kClasses = 1024;  // tiles whose visibility is worked out at a tim
 constexpr float kMax = 3.402823466e38f;
 
 template <typename ST> constexpr bool k16 = sizeof(ST) == 2;
-// what a weight is multiplied by: p <= 1, and goes into the products as 16-bit numbers; float16 has no room below 2^-14
-template <typename ST> constexpr float kWeight = 1.f;
-template <> constexpr float kWeight<_Float16> = 16384.f;
-
 // What the weights' exponents are counted in: 16-bit rows take 2^x, so that everything but the distance's factor is multiplied by
-// log2(e) once per row instead of once per pair; and p times kWeight, which is an addition to the exponent.
+// log2(e) once per row instead of once per pair.
 template <typename ST> constexpr float kUnit = k16<ST> ? 1.442695041f : 1.f;
-template <typename ST> constexpr float kShift = 0.f;
-template <> constexpr float kShift<_Float16> = 14.f;
+
+// The products with weights go through bfloat16 matrix instructions for float16 rows as well: float16 has no room for weights below
+// 2^-28 (at 2^14 times their value), which large values and gradients make seen.  A float16 value is two bfloat16 numbers, exactly.
+template <typename ST> constexpr bool kTwoParts = __is_same(ST, _Float16);
 
 // an odd number of 16-byte chunks for n of them: neighbouring rows start in different banks
 __host__ __device__ __forceinline__ int odd_chunks(int n) { return n | 1; }
 
+// transposed values of a tile as 16-bit numbers
+__host__ __device__ __forceinline__ int plane_bytes(int Wv, int TB) { return (Wv + 15) / 16 * 16 * kPitch(TB) * 2; }
+
 // LDS of a workgroup in bytes from the front, the same on host and device.  Rows: own/str distances' rows, oraw/raw the same
 // rows' ordered integers (16-bit backward), y the stream's values (float32: rows in product order; 16-bit: rows in product order in
-// the backward), yt the same transposed (16-bit, where they are multiplied by p).
+// the backward), yt the same transposed (16-bit, where they are multiplied by p), as bfloat16 numbers, for float16 the second parts behind the first.
 struct Layout {
 	int own, oraw, str, raw, y, yt, scratch, rows, total;
 	int so, sr, sy;  // bytes of a row of own/str, oraw/raw, y
@@ -91,7 +92,7 @@ __host__ __device__ inline Layout masked_layout(int W, int Wv, int waves, bool b
 	l.raw = l.str + kTile<TB> * l.so;
 	l.y = l.raw + (k16<ST> && backward ? kTile<TB> * l.sr : 0);
 	l.yt = l.y + (!k16<ST> || backward ? kTile<TB> * l.sy : 0);
-	l.scratch = l.yt + (k16<ST> && weigh ? (Wv + 15) / 16 * 16 * kPitch(TB) * 2 : 0);
+	l.scratch = l.yt + (k16<ST> && weigh ? plane_bytes(Wv, TB) * (kTwoParts<ST> ? 2 : 1) : 0);
 	l.rows = l.scratch + waves * kScratch;  // documents, lse, D, what lies outside of the range (64 each), 64 words for reductions, classes
 	l.total = l.rows + (4 * kTile<TB> + 64) * 4 + kClasses;
 	return l;
@@ -498,10 +499,22 @@ struct Stream {
 					if (8 * ch < tcols) {
 						char* to = yt + 8 * ch * kPitch(TB) * 2 + 4 * c2;
 #pragma unroll
-						for (int e = 0; e < 4; e++) {
-							*reinterpret_cast<unsigned*>(to + 2 * e * kPitch(TB) * 2) = __builtin_amdgcn_perm(b[e], a[e], 0x05040100u);
-							*reinterpret_cast<unsigned*>(to + (2 * e + 1) * kPitch(TB) * 2) = __builtin_amdgcn_perm(b[e], a[e], 0x07060302u);
-						}
+						for (int e = 0; e < 4; e++)
+#pragma unroll
+							for (int h = 0; h < 2; h++) {
+								const unsigned two = __builtin_amdgcn_perm(b[e], a[e], h ? 0x07060302u : 0x05040100u);
+								char* at = to + (2 * e + h) * kPitch(TB) * 2;
+								if constexpr (kTwoParts<ST>) {
+									_Float16 v[2];
+									__builtin_memcpy(v, &two, 4);
+									const __bf16 first[2] = {(__bf16)(float)v[0], (__bf16)(float)v[1]};
+									const __bf16 second[2] = {(__bf16)((float)v[0] - (float)first[0]), (__bf16)((float)v[1] - (float)first[1])};
+									__builtin_memcpy(at, first, 4);
+									__builtin_memcpy(at + plane_bytes(Wv, TB), second, 4);
+								} else {
+									*reinterpret_cast<unsigned*>(at) = two;
+								}
+							}
 					}
 				}
 			};
@@ -515,7 +528,7 @@ struct Stream {
 		}
 		if (tid < kTile<TB>) {
 			docs[tid] = d;
-			if (slse) { slse[tid] = l * kUnit<ST> - kShift<ST>; sD[tid] = dd; }
+			if (slse) { slse[tid] = l * kUnit<ST>; sD[tid] = dd; }
 		}
 		return bad;
 	}
@@ -532,8 +545,9 @@ __device__ __forceinline__ f4 mma16(const uint4& a, const uint4& b, f4 c)
 }
 
 // Weights of half a tile into the wave's scratch, and acc[tb][wb] += sum over its 32 columns c of value[c][16 wb + ..] * p[owner][c].
-// 16 bits: a weight is the sum of two numbers of the type, itself rounded and what that leaves out: one alone, half a step off, made
-// the results half as inexact again as their own rounding.
+// 16 bits: a weight is the sum of two bfloat16 numbers, itself rounded and what that leaves out: one alone, half a step off, made
+// the results half as inexact again as their own rounding; two leave 2^-18 of it.  Second part times a float16 value's second part,
+// 2^-18 of the product at most, is left out.
 // far: 0, or what is visible of a tile with values that are not finite, 2 if some of it is hidden: a hidden pair's weight of zero must
 // not meet them, which a matrix instruction cannot leave out; 1 if nothing is: a weight's second part, zero, must not meet them.
 template <typename ST, int NB, int TB>
@@ -541,15 +555,16 @@ __device__ __forceinline__ void weigh(f4 (&acc)[2][NB], char* scr, const char* y
                                       int i, int j, int l16, int g, int far)
 {
 	constexpr int pitch = kPad * 4;  // bytes of an owner's 32 weights, of 16 bits the second parts behind the first: odd chunks
+	const int plane = plane_bytes(Wv, TB);
 	wave_sync();
 #pragma unroll
 	for (int a = 0; a < 4; a++) {
 		if constexpr (k16<ST>) {
-			ST w[4], rest[4];
+			__bf16 w[4], rest[4];
 #pragma unroll
 			for (int e = 0; e < 4; e++) {
-				w[e] = (ST)p[a][e];
-				rest[e] = (ST)(p[a][e] - (float)w[e]);
+				w[e] = (__bf16)p[a][e];
+				rest[e] = (__bf16)(p[a][e] - (float)w[e]);
 			}
 			uint2 packed;
 			__builtin_memcpy(&packed, w, 8);
@@ -563,18 +578,23 @@ __device__ __forceinline__ void weigh(f4 (&acc)[2][NB], char* scr, const char* y
 	}
 	wave_sync();
 	if (far) {
+		const auto number = [](const char* at) { return k16<ST> ? to_f(*reinterpret_cast<const __bf16*>(at)) : *reinterpret_cast<const float*>(at); };
 		for (int c = 0; c < 32; c++)
 #pragma unroll
 			for (int tb = 0; tb < 2; tb++) {
 				const char* at = scr + (l16 + 16 * tb) * pitch + (int)sizeof(ST) * c;
-				const float w = to_f(*reinterpret_cast<const ST*>(at)) + (k16<ST> ? to_f(*reinterpret_cast<const ST*>(at + 64)) : 0.f);
+				const float w = number(at) + (k16<ST> ? number(at + 64) : 0.f);
 				if (w != 0.f || far == 1)
 #pragma unroll
 					for (int wb = 0; wb < NB; wb++)
 #pragma unroll
 						for (int e = 0; e < 4; e++) {
 							const int col = 16 * wb + 4 * g + e;
-							if (col < Wv) acc[tb][wb][e] += w * to_f(*reinterpret_cast<const ST*>(k16<ST> ? yt + col * kPitch(TB) * 2 + 64 * half + 2 * c : y + (32 * half + c) * sy + 4 * col));
+							if (col >= Wv) continue;
+							const char* from = k16<ST> ? yt + col * kPitch(TB) * 2 + 64 * half + 2 * c : y + (32 * half + c) * sy + 4 * col;
+							float v = number(from);
+							if (kTwoParts<ST> && __builtin_fabsf(v) <= kMax) v += number(from + plane);
+							acc[tb][wb][e] += w * v;
 						}
 			}
 		return;
@@ -608,9 +628,15 @@ __device__ __forceinline__ void weigh(f4 (&acc)[2][NB], char* scr, const char* y
 #pragma unroll
 		for (int wb = 0; wb < NB; wb++) {
 			if (wb >= blocks) break;
-			const uint4 av = *reinterpret_cast<const uint4*>(yt + (16 * wb + l16) * kPitch(TB) * 2 + 64 * half + 16 * g);
+			const char* from = yt + (16 * wb + l16) * kPitch(TB) * 2 + 64 * half + 16 * g;
+			const uint4 av = *reinterpret_cast<const uint4*>(from);
 #pragma unroll
-			for (int tb = 0; tb < 2; tb++) acc[tb][wb] = mma16<ST>(av, rest[tb], mma16<ST>(av, pb[tb], acc[tb][wb]));
+			for (int tb = 0; tb < 2; tb++) acc[tb][wb] = mma16<__bf16>(av, rest[tb], mma16<__bf16>(av, pb[tb], acc[tb][wb]));
+			if constexpr (kTwoParts<ST>) {
+				const uint4 second = *reinterpret_cast<const uint4*>(from + plane);
+#pragma unroll
+				for (int tb = 0; tb < 2; tb++) acc[tb][wb] = mma16<__bf16>(second, pb[tb], acc[tb][wb]);
+			}
 		}
 	}
 }
@@ -966,7 +992,7 @@ __global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* 
 #pragma unroll
 				for (int bb = 0; bb < 4; bb++)
 #pragma unroll
-					for (int a = 0; a < 4; a++) p[a][bb] = weight<ST>(p[a][bb] + kShift<ST>);
+					for (int a = 0; a < 4; a++) p[a][bb] = weight<ST>(p[a][bb]);
 				if (mykind == 2) {
 					asm volatile("");  // a branch: the compiler would rather compare in every tile and select
 #pragma unroll
@@ -1008,12 +1034,12 @@ __global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* 
 #pragma unroll
 	for (int tb = 0; tb < 2; tb++) {
 		const int t = row0 + 16 * tb + l16;
-		const float d = sc[16 * tb + l16] * (1.f / kWeight<ST>);
+		const float d = sc[16 * tb + l16];
 		if (t >= A.T) continue;
 		const int64_t row = ((int64_t)K.b * A.T + t) * A.H + K.h;
 		const int wp = (A.Wv + 3) & ~3;
 		float* to = part ? part + (blockIdx.z * rows + row) * wp : nullptr;
-		const float r = (part ? 1.f : 1.f / (1.f + d)) * (1.f / kWeight<ST>);
+		const float r = part ? 1.f : 1.f / (1.f + d);
 		if (g == 0) {
 			if (part) part[gridDim.z * rows * wp + blockIdx.z * rows + row] = d;
 			else if (lse) lse[row] = log1pf(d);
@@ -1232,7 +1258,6 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 #pragma unroll
 	for (int a = 0; a < 4; a++) od4[a] = doc && row0 + i + 8 * a < K.own_rows ? doc[my_lo + i + 8 * a] : -1;
 	float gsum[4] = {0.f, 0.f, 0.f, 0.f};
-	const float grw = A.rw * (1.f / kWeight<ST>);
 	constexpr int NY = OWNK ? NB : 1;
 	f4 dyv[2][NY];
 #pragma unroll
@@ -1266,7 +1291,7 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 		for (int a = 0; a < 4; a++) {
 			const int t = row0 + i + 8 * a;
 			const bool in = !OWNK && t < A.T;
-			olse[a] = in ? lse[((int64_t)K.b * A.T + t) * A.H + h] * kUnit<ST> - kShift<ST> : 0.f;
+			olse[a] = in ? lse[((int64_t)K.b * A.T + t) * A.H + h] * kUnit<ST> : 0.f;
 			oD[a] = in ? D[((int64_t)K.b * A.T + t) * A.H + h] : 0.f;
 		}
 		int first = 0, last = (K.str_rows + kTile<TB> - 1) / kTile<TB>;
@@ -1320,7 +1345,7 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 #pragma unroll
 						for (int a = 0; a < 4; a++) {
 							p[a][bb] -= OWNK ? sl : olse[a];
-							pf[a][bb] *= grw;
+							pf[a][bb] *= A.rw;
 						}
 					}
 					if (slope != 0.f) {
@@ -1465,7 +1490,7 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 				for (int e = 0; e < 4; e++) {
 					const int w = 16 * wb + 4 * g + e;
 					if (w >= A.Wv) continue;
-					const float y1 = dyv[tb][wb][e] * (1.f / kWeight<ST>);
+					const float y1 = dyv[tb][wb][e];
 					if (py) py[(blockIdx.z * rows + row) * A.Wv + w] = y1;
 					else dy[row * A.Wv + w] = (ST)y1;
 				}

@@ -202,6 +202,19 @@ def test_rows_of_few_values(W, dtype, rng):
     _check(q, k, v, do, doc=torch.arange(128, dtype=torch.int32)[None].cuda())
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("logit", [-14.0, -19.0, -23.0, -25.0, -28.0])
+def test_weights_that_are_all_small(logit, dtype):
+    # all of a row's weights alike and down to 2^-40, under large values and gradients: results well above the type's smallest numbers
+    W, T = 64, 256
+    g = torch.Generator().manual_seed(58)
+    q = torch.zeros(1, T, 2, W)
+    k = torch.full((1, T, 2, W), -logit / W ** 0.5) * (torch.randint(0, 2, (1, T, 2, W), generator=g) * 2 - 1)
+    v, do = (2e4 + 3e4 * torch.rand(1, T, 2, 48, generator=g) for _ in range(2))
+    do *= 2.0 ** -10
+    _check(*(x.to(dtype).cuda() for x in (q, k, v, do)), causal=False)
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("B,T,H,Wv", [(1, 512, 2, 64), (1, 512, 2, 37), (8, 150, 32, 64), (8, 150, 32, 33)])
 def test_values_with_a_common_part(B, T, H, Wv, dtype):
