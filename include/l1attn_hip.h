@@ -399,8 +399,8 @@ int l1attn_sparse_bidi_bwd_bf16(const void* dvo, const void* vf, const void* vb,
  * o_rest: [B,T,H,Wv] of the inputs' type or NULL (float32: not used): the forward writes what the rounding of o left out, the
  * backward adds it to o for sum d_o * o, which is taken off each d_o . v: without it the rounding of o alone moves dq and dk by
  * several times their own rounding where the values v have a part in common.
- * doc [B,S] and prefix [B] are device pointers to int32 or NULL; slopes is a HOST pointer to H numbers >= 0, or NULL, read
- * during the call.  T <= S <= 4194240, W and Wv <= 128, H <= 256, B <= 4194304 and B H <=
+ * doc [B,S] and prefix [B] are device pointers to int32 or NULL; slopes is a HOST pointer to H numbers, or NULL, read
+ * during the call.  softcap and slopes are 0 to 3e38.  T <= S <= 4194240, W and Wv <= 128, H <= 256, B <= 4194304 and B H <=
  * 16777215 (8388607 for float32 of widths up to 64).  Deterministic.
  */
 typedef struct l1attn_masked_desc {
@@ -466,7 +466,9 @@ int l1attn_cache_compact(const l1attn_cache* cache, int32_t* live, void* workspa
 /*
  * o [B,n,H,Wv] of q [B,n,H,W]: the masked attention's formula, causal, of the last counts[b] (n without counts) tokens of
  * sequence seqs[b] over all of it; query t is at place lens - counts[b] + t, rows t >= counts[b] are zero.  Head h reads key
- * head h / (H / Hk).  slopes: H host numbers >= 0 or NULL.  H <= 256.
+ * head h / (H / Hk).  slopes: H host numbers >= 0 or NULL.  H <= 256, B <= 65535 / Hk, n <= 65536, n * H/Hk <= 524280,
+ * B * n * H < 2^31.  Deterministic: the same call gives the same bits; a sequence's sums are cut by the lengths of its whole batch,
+ * so that in another batch it may round differently.  Whether they are cut at all goes by row_pages * page (more than 512 tokens).
  */
 typedef struct l1attn_attend_desc {
     int64_t B, n, H;

@@ -10,8 +10,8 @@
 // the denominator is >= 1, partial sums over pieces of the keys add up, and a row that sees nothing comes out as zero.
 //
 // One wavefront owns 32 rows ("owners": queries in the forward and in the gradient of q, keys in that of k and v) and walks
-// the other side ("stream") in tiles of 64 rows (16-bit forward) or 32 (backward and float32, whose registers would spill at 64),
-// which the waves of a workgroup share through LDS.  Three parts of a tile use
+// the other side ("stream") in tiles of 64 rows (16-bit forward) or 32 (backward and float32, whose registers would spill far more at
+// 64), which the waves of a workgroup share through LDS.  Three parts of a tile use
 // three maps of its pairs onto the lanes, joined by a wave-private LDS scratch:
 //   distances  lane (i,j) = (lane & 7, lane >> 3) holds owners i + 8a (a < 4) and stream rows j + 8b (b < 8 or 4): 12 LDS reads
 //              of 16 bytes feed 32 pairs at b < 8; |q - k| is no contraction, so this is vector-ALU work
@@ -31,8 +31,9 @@
 // is exact.
 //
 // What bounds it: the vector ALU's issue, with about a quarter of the time waits (1.8 waves a SIMD: sums, codes and tiles fill the
-// registers).  4096 tokens, 16 heads, W 64, every pair visible: bfloat16 forward 652 us (v_sad_u16 alone 264), gradients of q
-// 1838 and of k and v 1989; float32 1344, 2540 and 2879.
+// registers; one above widths of 64).  The gradients of k and v spill: float32 65 to 68 registers up to widths of 64 and 20 at W
+// above, 16 bits 16 to 19 up to widths of 64; nothing else does.  4096 tokens, 16 heads, W 64, every pair visible: bfloat16 forward
+// 619 us (v_sad_u16 alone 264), gradients of q 1776 and of k and v 1913; float16 636, 1678 and 1892; float32 1326, 2541 and 2882.
 #pragma once
 #include "common.h"
 #include "masked.h"

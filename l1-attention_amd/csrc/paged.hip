@@ -14,10 +14,14 @@
 // number alone made results 1.6 times as inexact as their own rounding), a code is exact in bfloat16, and matrix instructions add
 // them in float32.  Not float16 for float16 rows: it would want a power of two over all tokens of a step, where one token's large
 // scale takes the digits of the others' weights, also in rows that do not see it.  float32 has its own matrix instruction.
-// What bounds it: for few rows latency and the reads (32 sequences of about 2050 tokens, 4 rows, W 64, bfloat16: 34 MB in 17 us, and 4 for the join),
-// for many the vector ALU (16 of about 20480, 16 rows, W 128, float16: 140 us at 2.4 TB/s; 43 of 100 vector instructions are
-// v_sad_u16, which issue in about 4.2 cycles each; the rest makes codes and float16 of the cache's bytes, and weights).  With
-// one token a lane instead of two at 16 rows a row's codes would be read from LDS twice as often.
+// What bounds it: for few rows latency and the reads (32 sequences of about 2050 tokens, 4 rows, W 64, bfloat16: 34 MB in 18 us, and 4
+// for the join), for many the vector ALU (16 of about 20480, 16 rows, W 128, float16: 142 us at 2.4 TB/s; 2048 of a step's 4200
+// vector instructions are v_sad_u16, which issue in about 4.2 cycles each; the rest makes codes and bfloat16 of the cache's bytes,
+// and weights).  With one token a lane instead of two at 16 rows a row's codes would be read from LDS twice as often.  Widths
+// of 64 and 128, the same for keys and values, have loops of their own (FULL); all others run the one for up to 128, which for
+// values of 64 columns or fewer loads and multiplies columns twice.
+// How the steps are dealt out, and so the order of a sequence's sums and the grid of its codes, goes by the lengths of the whole
+// batch: the same call gives the same bits, a sequence in another batch may round differently.
 #include "paged.h"
 #include "softcap.h"
 #include "codes.h"

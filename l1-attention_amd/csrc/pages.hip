@@ -335,10 +335,11 @@ __global__ void __launch_bounds__(256) cache_rename(L1Cache C, const int32_t* __
 
 template <typename ST> __device__ __forceinline__ float value(ST x) { return (float)x; }
 
-// Tokens into pages: a workgroup for each page of each row and head, keys (z 0) and values (z 1): the values are read twice, for
-// the scale and for the codes, the second time from the caches (29 us for 8 rows of up to 2000 tokens, 8 heads, W 128, bfloat16:
-// 48 MB read, 24 MB written; 4.6 us for one token of 64 rows).  The page's scale becomes
-// the larger of what it was (if it held tokens) and the new tokens' largest magnitude over 127; if it grew, or the page is a
+// Tokens into pages: a workgroup for each page of each row and head, keys (z 0) and values (z 1).  A value is read once, into
+// registers, from where it goes into the scale and, behind the workgroup's barrier, into its code: the loads of a workgroup wait for
+// the chain plan, page, and its stores for all of them (29 us for 8 rows of up to 2000 tokens, 8 heads, W 128, bfloat16: 48 MB
+// read, 24 MB written, 15.5 us at a large copy's rate; 4.9 us for one token of 64 rows).  The page's scale becomes the larger of
+// what it was (if it held tokens) and the new tokens' largest magnitude times 1/127 (in float32); if it grew, or the page is a
 // copy of a shared one, the codes that were there are written again.  A value that is not finite does not count for the
 // scale: infinities are coded as +-127, NaN as 0.  G: elements a thread holds side by side.
 template <typename ST, int G>

@@ -17,7 +17,7 @@ nothing and is seen by nothing.  A row that sees nothing is zero, as are its gra
 For its backward a forward keeps the inputs, o and 4 bytes for each row and head, and for 16-bit types what the rounding of o left
 out, as large as o.
 
-slopes: H numbers >= 0 (constants, no gradient).  softcap >= 0, 0 for none.  Calls on several streams and in graph capture
+slopes: H numbers from 0 to 3e38 (constants, no gradient).  softcap from 0 to 3e38, 0 for none.  Calls on several streams and in graph capture
 are fine: a call keeps nothing.  As with any operator, a backward pass is captured with no eager graph of the same leaves alive.
 """
 from torch import nn

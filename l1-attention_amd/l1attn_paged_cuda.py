@@ -100,7 +100,8 @@ class L1PagedCache(object):
 def l1attn_paged(q, cache, seqs=None, counts=None, softcap=0.0, slopes=None):
     """o [B,n,H,Wv] of q [B,n,H,W], the last counts[b] (n, without counts) tokens of sequence seqs[b] (b, without seqs): the
     formula of L1AttnMasked, causal, over the whole sequence as the cache holds it.  Rows behind counts[b] and sequences of no
-    tokens give zeros.  For serving: there is no gradient."""
+    tokens give zeros.  For serving: there is no gradient.  The same call gives the same bits; a sequence may round differently
+    beside others, whose lengths decide how its sums are cut."""
     if torch.is_grad_enabled() and q.requires_grad:
         raise RuntimeError("l1attn_paged has no gradient: call it under torch.no_grad(), or on q.detach()")
     return _drv.cache_attend(cache._desc, cache.device, q.contiguous(), seqs, counts, softcap, slopes)

@@ -5,9 +5,8 @@ of a type whose half step is u = finfo.eps / 2, and rounded once to that type, i
 
     u * |result| + u * terms + F * terms
 
-The first part is the output's rounding.  The second is there for 16-bit inputs: a weight p that goes through a matrix
-instruction may be rounded to the type, relative error u a term; D = sum do*o in the backward is formed from
-the rounded o, which moves each score gradient by at most p * u * sum |do*o| (in `terms` of dq and dk).  F = 2^-24 * (3 W + 64):
+The first part is the output's rounding.  The second is there for 16-bit inputs: a logit from 16-bit codes is off by up to u (6.5
+times its rms, at the widest range that codes are taken for), which is a relative error u of a term.  F = 2^-24 * (3 W + 64):
 a distance is a sum of W terms (relative error W 2^-24 in any order), a logit of magnitude L <= 20 in these tests moves by
 W 2^-24 L / W-th of that on average and exp turns it into a relative error of p; the sums over tokens add 2^-24 a partial sum."""
 import math

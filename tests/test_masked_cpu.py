@@ -38,6 +38,21 @@ def test_refusals(no_gpu, what, match):
         drv.masked_forward(**a)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_what_a_forward_kept_is_checked(no_gpu, dtype):
+    # logarithms alone in float32; for 16 bits, on the next 16 bytes, as many numbers of the type as o has
+    q, k, v = _q(1, 3, 2, 8, dtype=dtype), _q(1, 4, 2, 8, dtype=dtype), _q(1, 4, 2, 5, dtype=dtype)
+    d = drv._masked_desc(q, k, v, None, None, True, 0.0, None)
+    floats, rest = drv._kept(d)
+    assert (floats, rest) == ((6, None) if dtype == torch.float32 else (8 + 15, 8))
+    o = _q(1, 3, 2, 5, dtype=dtype)
+    for bad in (_q(1, 3, 2) if dtype != torch.float32 else _q(7), _q(floats + 1), _q(floats, dtype=torch.float64)):
+        with pytest.raises(RuntimeError, match="kept must be"):
+            drv.masked_backward(o, q, k, v, o, bad)
+    with pytest.raises(RuntimeError, match="d_o must be"):
+        drv.masked_backward(o[..., :4], q, k, v, o, _q(floats))
+
+
 def test_slopes_are_constants_of_the_module():
     import l1attn_masked_cuda as m
     for bad in ((-1.0, 0.0), (float("nan"),), (float("inf"),)):
