@@ -180,8 +180,10 @@ __device__ __forceinline__ float wave_maxf(float x)
 // ------------------------------------------------------------------------------------------------------------- distances
 
 // float32 rows, columns [0, 4 * chunks): acc[a][b] += L1 distance of owner i + 8a and stream row j + 8b.  Four terms are summed
-// as a tree before they join the sum: a quarter of the roundings there.
-template <bool AHEAD, int TB>
+// as a tree before they join the sum: a quarter of the roundings there.  TWO: every second four has a sum of its own, which halves
+// what is left of them; at widths above 64 they are most of a result's error (1.6 times the error of sums in pairs throughout, with
+// two sums 1.2).  The backward of widths up to 64 has no registers for it (1.35 to 1.5 times; its step would take 10 % longer).
+template <bool AHEAD, bool TWO, int TB>
 __device__ __forceinline__ void distances32(const char* own, const char* str, int chunks, int stride, int i, int j, float (&acc)[4][TB])
 {
 	const char *po = own + i * stride, *ps = str + j * stride;
@@ -210,13 +212,18 @@ __device__ __forceinline__ void distances32(const char* own, const char* str, in
 		for (int b = 0; b < TB; b++) s[b] = *reinterpret_cast<const f4*>(ps + 8 * b * stride + d);
 		__builtin_amdgcn_sched_barrier(0);
 	};
-	const auto work = [&](const f4(&o)[4], const f4(&s)[TB]) {
+	float odd[4][TB];
+#pragma unroll
+	for (int a = 0; a < 4; a++)
+#pragma unroll
+		for (int b = 0; b < TB; b++) odd[a][b] = 0.f;
+	const auto work = [&](const f4(&o)[4], const f4(&s)[TB], float(&sum)[4][TB]) {
 #pragma unroll
 		for (int b = 0; b < TB; b++)
 #pragma unroll
 			for (int a = 0; a < 4; a++) {
 				const float d0 = o[a][0] - s[b][0], d1 = o[a][1] - s[b][1], d2 = o[a][2] - s[b][2], d3 = o[a][3] - s[b][3];
-				acc[a][b] += (__builtin_fabsf(d0) + __builtin_fabsf(d1)) + (__builtin_fabsf(d2) + __builtin_fabsf(d3));
+				sum[a][b] += (__builtin_fabsf(d0) + __builtin_fabsf(d1)) + (__builtin_fabsf(d2) + __builtin_fabsf(d3));
 			}
 		__builtin_amdgcn_sched_barrier(0);
 	};
@@ -224,11 +231,17 @@ __device__ __forceinline__ void distances32(const char* own, const char* str, in
 	load(o0, s0, 0);
 	for (int c = 0; c < chunks; c += 2) {
 		load(o1, s1, c + 1);
-		work(o0, s0);
+		work(o0, s0, acc);
 		if (c + 1 >= chunks) break;
 		load(o0, s0, c + 2);
-		work(o1, s1);
+		if constexpr (TWO) work(o1, s1, odd);
+		else work(o1, s1, acc);
 	}
+	if constexpr (TWO)
+#pragma unroll
+		for (int a = 0; a < 4; a++)
+#pragma unroll
+			for (int b = 0; b < TB; b++) acc[a][b] += odd[a][b];
 }
 
 // Rows of 16-bit codes, eight to a chunk.  AHEAD: reads one step ahead, 48 registers more (2.5 instead of 2.75 cycles per 64
@@ -779,7 +792,7 @@ __device__ __forceinline__ bool owner_grid(const ST* __restrict__ x, const int* 
 
 // A wave's distances of one tile, acc[a][b] >= 0 scaled by 1/sqrt(W), NaN where a value is.  Called by all waves of the
 // workgroup; `active`: this wave needs them.  Without a grid 16-bit rows go through LDS as float32, half of the columns at a time.
-template <typename ST, bool AHEAD, int TB>
+template <typename ST, bool AHEAD, bool TWO, int TB>
 __device__ __forceinline__ void tile_distances(char* own, char* str, const float* over, const Layout& Y, int W, float rw, const Grid& G, bool coded,
                                                bool active, const ST* __restrict__ own_x, int own_r0, int own_rows, int64_t own_pitch,
                                                const ST* __restrict__ str_x, int s0, int str_rows, int64_t str_pitch, int i, int j, int tid, int threads,
@@ -790,7 +803,7 @@ __device__ __forceinline__ void tile_distances(char* own, char* str, const float
 		for (int a = 0; a < 4; a++)
 #pragma unroll
 			for (int b = 0; b < TB; b++) x[a][b] = 0.f;
-		if (active) distances32<AHEAD, TB>(own, str, (W + 3) >> 2, Y.so, i, j, x);
+		if (active) distances32<AHEAD, TWO, TB>(own, str, (W + 3) >> 2, Y.so, i, j, x);
 #pragma unroll
 		for (int a = 0; a < 4; a++)
 #pragma unroll
@@ -822,7 +835,7 @@ __device__ __forceinline__ void tile_distances(char* own, char* str, const float
 			stage32(own, own_x, own_r0, kOwn, own_rows, own_pitch, w0, n, Y.so, false, tid & 63, 64);
 			stage32(str, str_x, s0, kTile<TB>, str_rows, str_pitch, w0, n, Y.so, false, tid, threads);
 			__syncthreads();
-			if (active) distances32<false, TB>(own, str, (n + 3) >> 2, Y.so, i, j, x);
+			if (active) distances32<false, false, TB>(own, str, (n + 3) >> 2, Y.so, i, j, x);
 		}
 #pragma unroll
 		for (int a = 0; a < 4; a++)
@@ -968,7 +981,7 @@ __global__ void __launch_bounds__(THREADS) masked_fwd(L1MaskedArgs A, const ST* 
 			}
 			mykind = __builtin_amdgcn_readfirstlane(mykind);  // what the tile is to this wave's own rows
 			float x[4][TB];
-			tile_distances<ST, true, TB>(own, str, over, Y, A.W, CAP ? A.rw : A.rw * kUnit<ST>, G, coded, mykind, qh, row0, A.T, qpitch, kh, s0, A.S, kpitch, i, j, tid, threads, x);
+			tile_distances<ST, true, true, TB>(own, str, over, Y, A.W, CAP ? A.rw : A.rw * kUnit<ST>, G, coded, mykind, qh, row0, A.T, qpitch, kh, s0, A.S, kpitch, i, j, tid, threads, x);
 			if (!mykind) continue;
 			// float32: a tile's sum on its own, then to the total: the roundings of either are fewer
 			f4 tile[2][NB];
@@ -1332,7 +1345,7 @@ __global__ void __launch_bounds__(THREADS) masked_bwd(L1MaskedArgs A, const ST* 
 				}
 				mykind = __builtin_amdgcn_readfirstlane(mykind);  // what the tile is to this wave's own rows
 				float x[4][TB];
-				tile_distances<ST, true, TB>(own, str, over, Y, A.W, CAP ? A.rw : A.rw * kUnit<ST>, G, coded, mykind, own_x, row0, K.own_rows, own_pitch, str_x, s0, K.str_rows, str_pitch, i, j, tid, threads, x);
+				tile_distances<ST, true, WL == 2, TB>(own, str, over, Y, A.W, CAP ? A.rw : A.rw * kUnit<ST>, G, coded, mykind, own_x, row0, K.own_rows, own_pitch, str_x, s0, K.str_rows, str_pitch, i, j, tid, threads, x);
 				if (!mykind) continue;
 #pragma unroll
 				for (int half = 0; half < TB / 4; half++) {

@@ -359,6 +359,25 @@ def test_repeats_bit_for_bit_and_large_grids():
     lf.check([a[0][:1, :, :4], a[1][:1, :, :4], a[2][:1, :, :1], a[3][:1, :, :1]], ref, terms, BF16, 64)
 
 
+@pytest.mark.parametrize("W", [64, 128])
+def test_roundings_of_float32_distances(W):
+    # One key for each query (a document each) and values of one: o and dv are the weight, whose relative error is the logit's error.
+    # A logit x is 1/sqrt(W), as float32, times two sums of W / 8 parts: of a sum, the k-th rounding is 2^-24 / sqrt(3) of k parts at
+    # most, rms; with the square root of the sum of squares, and the last product's rounding, 2^-24 |x| sqrt(W / 8 / 18 + 1 / 3), and
+    # two more 2^-24 for exp and the rest.  (One sum of W / 4 parts: half as much again.)  The backward of width 64 has one sum.
+    g = torch.Generator().manual_seed(60)
+    q, k = (3 * torch.randn(1, 256, 8, W, generator=g) for _ in range(2))
+    one = torch.ones(1, 256, 8, 4, device="cuda")
+    o, _, _, dv = _run(q.cuda(), k.cuda(), one, one, doc=torch.arange(256, dtype=torch.int32)[None].cuda())
+    rw = torch.tensor(W ** -0.5, dtype=F32).double()
+    x = (q.double() - k.double()).abs().sum(3, keepdim=True) * rw
+    want = torch.exp(-x) / (1 + torch.exp(-x))
+    room = 2.0 ** -24 * (float(x.square().mean().sqrt()) * (W / 144 + 1 / 3) ** 0.5 + 2)
+    for got in (o, dv) if W > 64 else (o,):
+        off = float(((got.double().cpu() - want) / want).square().mean().sqrt())
+        assert off <= room, (off / 2.0 ** -24, room / 2.0 ** -24)
+
+
 def test_more_tiles_than_are_classified_at_a_time():
     # 70000 keys: over 1024 tiles of 64
     q, k, v, do = _inputs(1, 3, 70000, 1, 1, 32, 32, F32, 14)
