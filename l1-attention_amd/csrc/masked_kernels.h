@@ -31,9 +31,9 @@
 // is exact.
 //
 // What bounds it: the vector ALU's issue, with about a quarter of the time waits (1.8 waves a SIMD: sums, codes and tiles fill the
-// registers; one above widths of 64).  The gradients of k and v spill: float32 65 to 68 registers up to widths of 64 and 20 at W
-// above, 16 bits 16 to 19 up to widths of 64; nothing else does.  4096 tokens, 16 heads, W 64, every pair visible: bfloat16 forward
-// 619 us (v_sad_u16 alone 264), gradients of q 1776 and of k and v 1913; float16 636, 1678 and 1892; float32 1326, 2541 and 2882.
+// registers; one above widths of 64).  The gradients of k and v spill: float32 65 to 68 registers up to widths of 64 and 23 to
+// 27 at W above, 16 bits 16 to 19 up to widths of 64; nothing else does.  4096 tokens, 16 heads, W 64, every pair visible: bfloat16 forward
+// 614 us (v_sad_u16 alone 264), gradients of q 1755 and of k and v 1889; float16 633, 1673 and 1883; float32 1399, 2521 and 2867.
 #pragma once
 #include "common.h"
 #include "masked.h"
